@@ -343,8 +343,9 @@ def _plain_codes(x):
     groups = (c + GROUP - 1) // GROUP
     x = torch.nn.functional.pad(x, (0, groups * GROUP - c)).view(*x.shape[:-1], groups, GROUP)
     a = x.abs().amax(-1, keepdim=True)
-    inv = torch.where(a < TINY, 0.0, 127.0 / a)
-    return torch.round(x * inv).to(torch.int8), torch.where(a < TINY, 0.0, a / 127.0)
+    top = torch.full_like(a, 127.0)  # a tensor: torch divides by a number through its reciprocal, in two roundings
+    inv = torch.where(a < TINY, 0.0, top / a)
+    return torch.round(x * inv).to(torch.int8), torch.where(a < TINY, 0.0, a / top)
 
 
 def _plain_values(codes, scale, c):
