@@ -285,6 +285,147 @@ int lama_section_rects(const uint8_t* mask, int w, int h, int* out, int cap);
 int lama_rfft2_noalloc(int device, const float* d_feat, int batch, int channels, int h, int w, void* d_spec,
                        void* stream, char* err, int err_len);
 
+/* ---------------------------------------------------------------- token-mixer operators
+ * No counterpart in the reference.  Operators of a token-mixer block over the
+ * latent plane (or any token sequence), for inference and training next to
+ * the generator.  They need no engine: device pointers of CUDA device
+ * `device` in, work queued on `stream` (a cudaStream_t, null = legacy default
+ * stream), the caller's current device restored, nothing allocated and
+ * nothing kept after the call (a workspace, where one is needed, is the
+ * caller's).  On failure nothing is queued after the failing step, the code
+ * is returned and a message is written to err (err_len bytes, may be null).
+ * Sums, states and statistics are fp32. */
+
+/* Element types of the operators' tensors. */
+enum { LAMA_F32 = 0, LAMA_F16 = 1, LAMA_BF16 = 2 };
+
+/* Rows of one tensor [batch][tokens][heads][d]: element (b, t, h, i) at
+ * data + b * batch_stride + t * token_stride + h * head_stride + i, strides in
+ * elements.  Any strides; rows that start at multiples of 16 bytes with d a
+ * multiple of 8 are moved 16 bytes at a time, others element by element.  A
+ * tensor may have fewer heads than the operator: each is then shared by
+ * operator heads / its heads neighbouring heads. */
+typedef struct {
+  void* data;
+  long long batch_stride, token_stride, head_stride;
+  int heads;
+} lama_rows;
+
+/* Linear attention with a decay for each head:
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t.
+ * log_decay: [heads] fp32 on the device, -inf (no memory) allowed; it is a
+ * constant of the layer and has no gradient.  lengths: null, or [batch] int32
+ * on the device (values outside 0..tokens are clamped): sequence b consists of
+ * its first lengths[b] tokens, later tokens are never read and their outputs
+ * and gradients are 0.  initial_state: null (zeros) or [batch][heads][dk][dv]
+ * fp32.  dk, dv <= 128; batch * heads <= 65535. */
+typedef struct {
+  int dtype; /* of q, k, v and the output: LAMA_F32, LAMA_F16 or LAMA_BF16 */
+  int batch, tokens, heads, dk, dv;
+  lama_rows q, k, v;
+  const float* log_decay;
+  const float* initial_state;
+  const int* lengths;
+  float scale;
+} lama_attention;
+
+/* Bytes of device workspace lama_linear_attention (backward = 0) or
+ * lama_linear_attention_backward (1) needs for these arguments (0 for few
+ * tokens), or a negative LAMA_E* code.  Needs no GPU. */
+long long lama_linear_attention_workspace(const lama_attention* p, int backward, char* err, int err_len);
+
+/* out: [batch][tokens][heads][dv]; final_state: null, or
+ * [batch][heads][dk][dv] fp32, the state after each sequence's last token. */
+int lama_linear_attention(const lama_attention* p, const lama_rows* out, float* final_state, void* workspace,
+                          long long workspace_bytes, int device, void* stream, char* err, int err_len);
+
+/* Gradients for grad_out [batch][tokens][heads][dv] and, unless null, the
+ * gradient grad_final_state of the final state.  grad_q, grad_k and grad_v
+ * have the heads of q, k and v (a shared head's gradient is the sum over the
+ * heads that share it); grad_initial_state may be null. */
+typedef struct {
+  lama_rows grad_out, grad_q, grad_k, grad_v;
+  const float* grad_final_state;
+  float* grad_initial_state;
+} lama_attention_grads;
+
+int lama_linear_attention_backward(const lama_attention* p, const lama_attention_grads* g, void* workspace,
+                                   long long workspace_bytes, int device, void* stream, char* err, int err_len);
+
+/* One token of linear attention per row, the state updated on the device:
+ *   S <- exp(log_decay[h]) S + k v^T,  o = scale q S.
+ * a: tokens = 1, initial_state and lengths null (token strides are not read).
+ * state, out_state: [num_slots][heads][dk][dv] fp32; out_state may be state
+ * (in place) or a buffer that does not overlap it.  slots: null (row b uses
+ * slot b), or [batch] int32 on the device, no slot twice; a slot outside
+ * 0..num_slots-1 marks an unused row, whose output is 0. */
+int lama_linear_attention_step(const lama_attention* a, const lama_rows* out, const float* state, float* out_state,
+                               int num_slots, const int* slots, int device, void* stream, char* err, int err_len);
+
+/* The norm after a block, its gate and residual scale, the residual sum and
+ * the norm before the next block:
+ *   p = post_weight * y / sqrt(mean y^2 + eps)   (p = y where post_weight is null)
+ *   u = x + s * gate * p                         (rounded to dtype)
+ *   n = pre_weight * u / sqrt(mean u^2 + eps)    (no n where pre_weight is null)
+ * over rows of `channels` (<= 16384).  gate: null (1), or rows of the tensors'
+ * type gate_stride elements apart, gate row i for the rows i * gate_rows ..
+ * (i + 1) * gate_rows - 1 (1: a gate for each row).  s: residual_scales
+ * [channels] fp32, or the number residual_scale where that is null.  Weights
+ * are fp32. */
+typedef struct {
+  int dtype; /* of x, y, u, n, the gate and their gradients */
+  long long rows;
+  int channels;
+  const void* gate;
+  long long gate_rows, gate_stride;
+  const float *post_weight, *pre_weight, *residual_scales;
+  float residual_scale, eps;
+} lama_norm;
+
+/* x, y: rows x_stride and y_stride elements apart; u, n: [rows][channels].
+ * For the backward pass, where not null: post_rstd, pre_rstd [rows] fp32
+ * (1 / sqrt(...) of the two norms) and 8-bit checkpoints of y and u (as
+ * lama_checkpoint_store makes them; u's is needed only with pre_weight). */
+int lama_gated_residual_norm(const lama_norm* p, const void* x, long long x_stride, const void* y, long long y_stride,
+                             void* u, void* n, float* post_rstd, float* pre_rstd, int8_t* y_codes, float* y_scales,
+                             int8_t* u_codes, float* u_scales, int device, void* stream, char* err, int err_len);
+
+/* Gradients.  grad_u and grad_n may be null (zeros).  y and u are given as
+ * such, or (y_codes not null) as their 8-bit checkpoints.  grad_x, grad_y:
+ * [rows][channels]; the others may be null: grad_gate [gate rows][channels]
+ * of the tensors' type, and [channels] fp32. */
+typedef struct {
+  const void *grad_u, *grad_n, *y, *u;
+  long long grad_u_stride, grad_n_stride, y_stride, u_stride;
+  const int8_t *y_codes, *u_codes;
+  const float *y_scales, *u_scales, *post_rstd, *pre_rstd;
+  void *grad_x, *grad_y, *grad_gate;
+  float *grad_post_weight, *grad_pre_weight, *grad_residual_scales;
+} lama_norm_grads;
+
+/* Bytes of device workspace the backward pass needs, or a negative code. */
+long long lama_gated_residual_norm_workspace(const lama_norm* p, char* err, int err_len);
+
+int lama_gated_residual_norm_backward(const lama_norm* p, const lama_norm_grads* g, void* workspace,
+                                      long long workspace_bytes, int device, void* stream, char* err, int err_len);
+
+/* Activation checkpoints in 8 bits.  Per row and group of 128 channels (the
+ * last group may be shorter), with a = max |x|: code = rint(x * (127 / a)),
+ * scale = a / 127, value = code * scale, each operation rounded once in fp32.
+ * A group with a < 2^-96 is stored as zeros; a group that holds an infinity
+ * or a NaN restores to NaN throughout; fp32's largest value may restore to
+ * infinity (127 * (a / 127) rounds past it).  x: rows row_stride elements apart;
+ * codes: [rows][channels]; scales: [rows][(channels + 127) / 128]. */
+int lama_checkpoint_store(const void* x, int dtype, long long rows, int channels, long long row_stride, int8_t* codes,
+                          float* scales, int device, void* stream, char* err, int err_len);
+int lama_checkpoint_restore(const int8_t* codes, const float* scales, int dtype, long long rows, int channels,
+                            long long row_stride, void* x, int device, void* stream, char* err, int err_len);
+
+/* Waits for the device and reports whether a bounded wait of an operator's
+ * kernel ran out since the last call (LAMA_EDEVICE; its outputs are then
+ * incomplete), clearing the report. */
+int lama_operator_status(int device, char* err, int err_len);
+
 /* Free every device buffer and the engine. */
 void lama_close(lama_engine* e);
 

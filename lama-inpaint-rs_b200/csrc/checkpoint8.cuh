@@ -1,0 +1,93 @@
+// 8-bit checkpoints of activations: per row and group of 128 channels, with
+// a = max |x| over the group,
+//
+//   code = rint(x * (127 / a)),  scale = a / 127,  value = code * scale,
+//
+// each operation one rounding in fp32, so the codes are the same wherever they
+// are made.  A group with a < 2^-96 (127 / a would overflow) is stored as
+// zeros; a group that holds an infinity or a NaN restores to NaN throughout,
+// so that a step that has blown up stays visible.
+//
+// A half-warp holds a group: 16 lanes with 8 consecutive channels each.
+#pragma once
+
+#include "operators.cuh"
+
+namespace lama {
+namespace ops {
+
+constexpr int GROUP8 = 128;
+
+// Codes (packed, 8 bytes) of this lane's 8 values and the group's scale; every
+// lane of the half-warp takes part.  Channels past the row's end hold zeros.
+__device__ __forceinline__ uint2 encode8(const float* v, float& scale) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);  // NaN compares above infinity
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) a = max(a, __shfl_xor_sync(~0u, a, m));
+  const float amax = __uint_as_float(a);
+  uint32_t w[2] = {0, 0};
+  if (a >= 0x7f800000u) {
+    scale = __uint_as_float(0x7fffffffu);
+  } else if (amax < 1.2621774483536189e-29f) {  // 2^-96
+    scale = 0.f;
+  } else {
+    const float inv = __fdiv_rn(127.f, amax);
+    scale = __fdiv_rn(amax, 127.f);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      w[i >> 2] |= ((uint32_t)__float2int_rn(__fmul_rn(v[i], inv)) & 255u) << ((i & 3) * 8);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ void decode8(uint2 c, float scale, float* v) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const uint32_t w = i < 4 ? c.x : c.y;
+    v[i] = __fmul_rn((float)(int)(int8_t)((w >> ((i & 3) * 8)) & 255u), scale);
+  }
+}
+
+// 8 elements from p (or n < 8 where the row ends); `vec`: p is 16-byte (fp32:
+// two 16-byte words) aligned and n is 8.
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int n, bool vec, float* v) {
+  if (vec && n >= 8) {
+    load_vec<T, 8>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = i < n ? to_float(p[i]) : 0.f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, int n, bool vec, const float* v) {
+  if (vec && n >= 8) {
+    store_vec<T, 8>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (i < n) p[i] = from_float<T>(v[i]);
+  }
+}
+__device__ __forceinline__ uint2 load_codes(const int8_t* p, int n, bool vec) {
+  if (vec && n >= 8) return *reinterpret_cast<const uint2*>(p);
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (i < n) w[i >> 2] |= ((uint32_t)p[i] & 255u) << ((i & 3) * 8);
+  return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void store_codes(int8_t* p, int n, bool vec, uint2 c) {
+  if (vec && n >= 8) {
+    *reinterpret_cast<uint2*>(p) = c;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (i < n) p[i] = (int8_t)(((i < 4 ? c.x : c.y) >> ((i & 3) * 8)) & 255u);
+  }
+}
+
+}  // namespace ops
+}  // namespace lama

@@ -1,0 +1,844 @@
+// Linear attention with a decay for each head: whole sequences and gradients.
+//
+//   S_t = lam S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,   lam = exp(g_head)
+//
+// Chunked form.  For a chunk of n tokens with the entering state E (the state
+// of the tokens before it, decayed to its first token),
+//
+//   o_i = scale ( lam^i q_i E + sum_{j<=i} lam^{i-j} (q_i . k_j) v_j ),  i = 0..n-1
+//   X   = lam^{n-1} E + sum_j lam^{n-1-j} k_j v_j^T      (state after its last token)
+//   E'  = lam X                                          (enters the next chunk)
+//
+// so every power of lam has an exponent >= 0: no decay overflows, lam = 0
+// (g = -inf) included.  Gradients are the same recurrence on other operands:
+//
+//   dq: forward in time on  (do; v, k), state S^T
+//   dv: backward in time on (k; q, do), state D_t = lam D_{t+1} + scale q_t do_t^T (+ dS_T)
+//   dk: backward in time on (v; do, q), state D^T
+//
+// One kernel, `k_chunks`, computes all of them: it takes roles (a; b, c) with
+// S = sum b c^T and out = a S, a direction in time, and strides.  A CTA walks
+// the chunks of one segment of one (sequence, head, 64 columns of c); the
+// chunk products run on the tensor core (tcgen05, fp32 accumulators in TMEM),
+// the state stays in registers in fp32.  A sequence long enough to be cut into
+// several segments takes three launches: the state each segment adds
+// (k_chunks without outputs), the scan over segments, the outputs.
+//
+// Precision.  Operands are carried as sums of bf16 parts, as in the
+// generator's convolutions: bf16 inputs are one part (exact), fp16 inputs two
+// (exact), fp32 inputs three (24 bits), and a product keeps the pairs of
+// parts above the last part's size.  What the kernel computes itself and
+// feeds back as an operand is rounded: the decayed b to three parts always
+// (the state is an fp32 result), the scores to as many parts as the inputs
+// have, the entering state to two (three for fp32 inputs).  For bf16 inputs the
+// scores' one rounding is of the size of the output's own.
+#include <algorithm>
+
+#include "operators.cuh"
+#include "ptx.cuh"
+
+namespace lama {
+namespace ops {
+
+namespace {
+
+__device__ int g_status;
+
+constexpr int CH = 128;         // tokens of a chunk (the MMA's M)
+constexpr int THREADS = 256;
+constexpr uint32_t TILE = 128 * 128;  // bytes of 128 rows x 64 bf16, 128-byte swizzle
+constexpr uint32_t ETILE = 64 * 128;  // 64 rows x 64 bf16
+
+// One operand: element (token, d) of the head's row at
+// p + batch * sb + token * st + head * sh + d.
+struct Operand {
+  const void* p;
+  long long sb, st, sh;
+  int per;  // heads of the run that share one head of the operand
+  int vec;  // rows are 16-byte aligned and a multiple of 16 bytes long
+};
+
+struct Run {
+  Operand a, b, c;
+  void* out;  // element (token, d) of head h at out + batch * ob + token * ot + h * oh + d
+  long long ob, ot, oh;
+  int out_f32;  // out is fp32 whatever the inputs are
+  int out_vec;
+  const float* log_decay;
+  const int* lengths;
+  const float* init;  // [batch][heads] of [da][dc], element (r, c) at r * ir + c * ic
+  float* fin;
+  long long ir, ic, fr, fc;
+  float* seg;  // [batch*heads][nseg][slabs*64][blocks*64]: states of the segments
+  int* status;
+  float inter, intra, update;  // scales of a E, of the scores, of b c^T
+  int batch, tokens, heads, da, dc;
+  int reverse;     // walk backwards in time; the initial state is not decayed, the final one is
+  int nseg, chunks;  // segments of a sequence, chunks of a segment
+  int blocks;      // 64-column blocks of c
+  int slabs;       // 64-column slabs of a and b
+};
+
+__device__ __forceinline__ float power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }
+
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t lbo) {
+  // MN-major, 128-byte swizzle: 64-element blocks `lbo` bytes apart, groups of 8 k-rows 1024 apart
+  return smem_desc(saddr, 1024, 2) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16);
+}
+
+template <class T>
+struct Parts {
+  static constexpr int N = 1;
+};
+template <>
+struct Parts<__half> {
+  static constexpr int N = 2;
+};
+template <>
+struct Parts<float> {
+  static constexpr int N = 3;
+};
+
+// v[0..7] into N bf16 parts of 16 bytes each (part p holds what parts 0..p-1 left over)
+template <int N>
+__device__ __forceinline__ void split8(const float* v, uint4* out) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) r[i] = v[i];
+#pragma unroll
+  for (int p = 0; p < N; p++) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(r[2 * i], r[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      if (p + 1 < N) {
+        r[2 * i] -= __low2float(h);
+        r[2 * i + 1] -= __high2float(h);
+      }
+    }
+    out[p] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+__device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t swz(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+
+// 64 columns from d0 of the chunk's rows, as parts, zeros past the sequence
+// and past the head's size.  Row r of the chunk is token first + r * step.
+template <class T>
+__device__ void load_tile(uint32_t dst, const Operand& o, int batch, int head, long long first, int step, int n, int d0,
+                          int d) {
+  constexpr int NP = Parts<T>::N;
+  const T* base = static_cast<const T*>(o.p) + batch * o.sb + (head / o.per) * o.sh + first * o.st;
+#pragma unroll
+  for (int it = 0; it < CH * 8 / THREADS; it++) {
+    const int c = it * THREADS + (int)threadIdx.x, row = c >> 3, ck = c & 7;
+    const int col = d0 + ck * 8;
+    uint4 parts[NP];
+#pragma unroll
+    for (int p = 0; p < NP; p++) parts[p] = make_uint4(0, 0, 0, 0);
+    if (row < n && col < d) {
+      const T* src = base + (long long)row * step * o.st + col;
+      if (o.vec && NP == 1) {
+        parts[0] = *reinterpret_cast<const uint4*>(src);
+      } else {
+        float v[8];
+        if (o.vec) {
+          load_vec<T, 8>(src, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++) v[i] = col + i < d ? to_float(src[i]) : 0.f;
+        }
+        split8<NP>(v, parts);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < NP; p++) sts16(dst + p * TILE + swz(row, ck), parts[p]);
+  }
+}
+
+// D (+)= A B over K, the pairs of parts (x, y) with x + y < max(NA, NB), the
+// smallest first: the tensor core truncates each sum to fp32, so what is
+// added while the accumulator is still small loses less (fp32 inputs measured
+// 2e-6 off with the largest pair first).
+// `ka`, `kb`: byte steps of a 16-wide K step; after `kwrap` steps A moves on by `awrap` bytes instead.
+template <int NA, int NB>
+__device__ __forceinline__ void mma_parts(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int steps, uint32_t ka,
+                                          uint32_t kb, uint32_t pa, uint32_t pb, int kwrap, uint32_t awrap,
+                                          bool accumulate) {
+  constexpr int LIM = NA > NB ? NA : NB;
+  uint32_t acc = accumulate;
+#pragma unroll
+  for (int z = LIM - 1; z >= 0; z--)
+#pragma unroll
+    for (int x = 0; x < NA; x++) {
+      const int y = z - x;
+      if (y < 0 || y >= NB) continue;
+      for (int s = 0; s < steps; s++) {
+        const uint32_t ao = x * pa + (s % kwrap) * ka + (s / kwrap) * awrap, bo = y * pb + s * kb;
+        mma_bf16(d, a + (ao >> 4), b + (bo >> 4), idesc, acc);
+        acc = 1;
+      }
+    }
+}
+
+constexpr uint32_t A_MN = 1u << 15, B_MN = 1u << 16;
+
+template <class T>
+struct Plan {
+  static constexpr int NP = Parts<T>::N;
+  static constexpr int EP = NP == 1 ? 2 : NP;  // parts of the entering state
+  // a, b, c: NP tiles each; the decayed b: 3 tiles; the scores: 2 * NP tiles
+  // over the decayed b (and, for fp32 inputs, which have no room beside it,
+  // the decayed b over b and the scores over a and b); the entering state.
+  static constexpr uint32_t A = 0, B = NP * TILE, C = 2 * NP * TILE;
+  static constexpr uint32_t BD = NP == 3 ? B : 3 * NP * TILE;
+  static constexpr uint32_t P = NP == 3 ? A : BD;
+  static constexpr uint32_t W = NP == 3 ? 0 : (2 * NP > 3 ? 2 * NP : 3) * TILE;
+  static constexpr uint32_t E = 3 * NP * TILE + W;
+  static constexpr uint32_t bytes(int slabs) { return E + EP * ETILE * slabs + 1024; }
+};
+
+template <class T, bool OUT>
+__global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run r) {
+  using PL = Plan<T>;
+  constexpr int NP = PL::NP, EP = PL::EP;
+  constexpr int MAXS = 2;
+  extern __shared__ uint8_t raw[];
+  __shared__ float pw[CH + 1];
+  __shared__ uint64_t bar_mem;
+  __shared__ uint32_t tmem_slot;
+  const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t bar = smem_u32(&bar_mem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  const int segs = OUT ? r.nseg : r.nseg - 1;
+  int id = blockIdx.x;
+  const int seg = id % segs;
+  id /= segs;
+  const int blk = id % r.blocks;
+  id /= r.blocks;
+  const int head = id % r.heads, batch = id / r.heads;
+
+  const float g = r.log_decay[head];
+  int len = r.tokens;
+  if (r.lengths) len = min(max(r.lengths[batch], 0), r.tokens);
+  const int seg_tokens = r.chunks * CH;
+  const int p0 = seg * seg_tokens;
+
+  if (warp == 0) tmem_alloc(smem_u32(&tmem_slot), 256);
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    fence_mbar_init();
+  }
+  for (int i = tid; i <= CH; i += THREADS) pw[i] = power(g, i);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t t_p = tmem, t_o = tmem + 128, t_u = tmem + 192;
+  const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+  const int row = (warp & 3) * 32 + lane;            // TMEM lane: token row, or state row (twice)
+  const int srow = row & 63;                         // state row of a slab
+  const int scol = ((warp >> 2) * 2 + (row >> 6)) * 16;  // its 16 columns
+
+  float E[MAXS][16];
+  const int ld = r.blocks * 64;
+  const float lam = pw[1];
+#pragma unroll
+  for (int s = 0; s < MAXS; s++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      float v = 0.f;
+      const int er = s * 64 + srow, ec = blk * 64 + scol + i;
+      if (OUT && s < r.slabs) {
+        if (r.nseg > 1) {
+          v = r.seg[(((long long)(batch * r.heads + head) * r.nseg + seg) * (r.slabs * 64) + er) * ld + ec];
+        } else if (r.init && er < r.da && ec < r.dc) {
+          v = r.init[(long long)(batch * r.heads + head) * r.da * r.dc + er * r.ir + ec * r.ic];
+          if (!r.reverse) v *= lam;
+        }
+      }
+      E[s][i] = v;
+    }
+
+  uint32_t phase = 0;
+  bool ok = true;
+  int done = 0;  // tokens of this segment so far
+  const int step = r.reverse ? -1 : 1;
+  for (int ch = 0; ok && ch < r.chunks; ch++) {
+    const int pos = p0 + ch * CH;
+    const int n = min(CH, len - pos);
+    if (n <= 0) break;
+    const bool last = pos + n == len;
+    const long long first = r.reverse ? (long long)len - 1 - pos : pos;
+    load_tile<T>(smem + PL::C, r.c, batch, head, first, step, n, blk * 64, r.dc);
+    if (OUT) {
+#pragma unroll
+      for (int s = 0; s < MAXS; s++) {
+        if (s >= r.slabs) break;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          uint4 parts[EP];
+          split8<EP>(&E[s][h * 8], parts);
+#pragma unroll
+          for (int p = 0; p < EP; p++) sts16(smem + PL::E + (s * EP + p) * ETILE + swz(srow, (scol >> 3) + h), parts[p]);
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < MAXS; s++) {
+      if (s >= r.slabs) break;
+      if (OUT) load_tile<T>(smem + PL::A, r.a, batch, head, first, step, n, s * 64, r.da);
+      load_tile<T>(smem + PL::B, r.b, batch, head, first, step, n, s * 64, r.da);
+      if (OUT && NP == 3) {
+        // scores and a E first: the decayed b takes b's place
+        fence_async_smem();
+        __syncthreads();
+        if (tid == 0) {
+          tc_fence_after();
+          mma_parts<NP, NP>(t_p, smem_desc(smem + PL::A, 1024, 2), smem_desc(smem + PL::B, 1024, 2), idesc_bf16_f32(128),
+                            4, 32, 32, TILE, TILE, 4, 0, s > 0);
+          mma_parts<NP, EP>(t_o, smem_desc(smem + PL::A, 1024, 2), desc_mn(smem + PL::E + s * EP * ETILE, 0),
+                            idesc_bf16_f32(64) | B_MN, 4, 32, 2048, TILE, ETILE, 4, 0, s > 0);
+          mma_commit(bar);
+        }
+        ok = mbar_wait(bar, phase, r.status, 1);
+        phase ^= 1;
+        ok = __syncthreads_and(ok);
+        if (!ok) break;
+        tc_fence_after();
+      } else {
+        __syncthreads();
+      }
+      // decayed b: row j times lam^{n-1-j}, three parts
+#pragma unroll
+      for (int it = 0; it < CH * 8 / THREADS; it++) {
+        const int c = it * THREADS + tid, j = c >> 3, ck = c & 7;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = 0.f;
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          const uint4 u = lds16(smem + PL::B + p * TILE + swz(j, ck));
+          const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&u);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            v[2 * i] += __low2float(e[i]);
+            v[2 * i + 1] += __high2float(e[i]);
+          }
+        }
+        const float w = j < n ? pw[n - 1 - j] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = j < n ? v[i] * w : 0.f;
+        uint4 parts[3];
+        split8<3>(v, parts);
+#pragma unroll
+        for (int p = 0; p < 3; p++) sts16(smem + PL::BD + p * TILE + swz(j, ck), parts[p]);
+      }
+      fence_async_smem();
+      __syncthreads();
+      if (tid == 0) {
+        tc_fence_after();
+        if (OUT && NP != 3) {
+          mma_parts<NP, NP>(t_p, smem_desc(smem + PL::A, 1024, 2), smem_desc(smem + PL::B, 1024, 2), idesc_bf16_f32(128),
+                            4, 32, 32, TILE, TILE, 4, 0, s > 0);
+          mma_parts<NP, EP>(t_o, smem_desc(smem + PL::A, 1024, 2), desc_mn(smem + PL::E + s * EP * ETILE, 0),
+                            idesc_bf16_f32(64) | B_MN, 4, 32, 2048, TILE, ETILE, 4, 0, s > 0);
+        }
+        // both 64-row halves of the MMA's 128 rows read the slab's 64 columns
+        mma_parts<3, NP>(t_u, desc_mn(smem + PL::BD, 0), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | A_MN | B_MN, 8,
+                         2048, 2048, TILE, TILE, 8, 0, false);
+        mma_commit(bar);
+      }
+      ok = mbar_wait(bar, phase, r.status, 2);
+      phase ^= 1;
+      ok = __syncthreads_and(ok);
+      if (!ok) break;
+      tc_fence_after();
+      float u[16];
+      tmem_ld16(t_u + lane_base + scol, u);
+      tmem_wait_ld();
+      const float dn1 = pw[n - 1];
+#pragma unroll
+      for (int i = 0; i < 16; i++) E[s][i] = dn1 * E[s][i] + r.update * u[i];  // the state after the chunk
+      if (OUT && last && r.fin) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int er = s * 64 + srow, ec = blk * 64 + scol + i;
+          if (er < r.da && ec < r.dc)
+            r.fin[(long long)(batch * r.heads + head) * r.da * r.dc + er * r.fr + ec * r.fc] =
+                r.reverse ? lam * E[s][i] : E[s][i];
+        }
+      }
+      if (OUT || ch + 1 < r.chunks)
+#pragma unroll
+        for (int i = 0; i < 16; i++) E[s][i] *= lam;
+      tc_fence_before();
+      if (s + 1 < r.slabs) __syncthreads();  // the next slab's tiles and accumulator
+    }
+    if (!ok) break;
+    done = pos + n - p0;
+    if (OUT) {
+      // scores: decay and causal mask, rounded to NP parts
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int col0 = (warp >> 2) * 64 + h * 32;
+        float v[32];
+        tmem_ld32(t_p + lane_base + col0, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+          const int dist = row - (col0 + j);
+          v[j] = dist >= 0 ? v[j] * pw[max(dist, 0)] : 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          uint4 parts[NP];
+          split8<NP>(v + q * 8, parts);
+#pragma unroll
+          for (int p = 0; p < NP; p++)
+            sts16(smem + PL::P + (p * 2 + (warp >> 2)) * TILE + swz(row, h * 4 + q), parts[p]);
+        }
+      }
+      tc_fence_before();
+      fence_async_smem();
+      __syncthreads();
+      if (tid == 0) {
+        tc_fence_after();
+        mma_parts<NP, NP>(t_p, smem_desc(smem + PL::P, 1024, 2), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | B_MN, 8,
+                          32, 2048, 2 * TILE, TILE, 4, TILE, false);
+        mma_commit(bar);
+      }
+      ok = mbar_wait(bar, phase, r.status, 3);
+      phase ^= 1;
+      ok = __syncthreads_and(ok);
+      if (!ok) break;
+      tc_fence_after();
+      const int col0 = (warp >> 2) * 32;
+      float x[32], y[32];
+      tmem_ld32(t_o + lane_base + col0, x);
+      tmem_ld32(t_p + lane_base + col0, y);
+      tmem_wait_ld();
+      tc_fence_before();
+      const float di = pw[row] * r.inter;
+#pragma unroll
+      for (int i = 0; i < 32; i++) x[i] = di * x[i] + r.intra * y[i];
+      if (row < n) {
+        const long long at = batch * r.ob + (first + (long long)row * step) * r.ot + head * r.oh;
+        const int c0 = blk * 64 + col0;
+        if (r.out_f32) {
+          float* dst = static_cast<float*>(r.out) + at + c0;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            if (r.out_vec && c0 + i + 8 <= r.dc)
+              store_vec<float, 8>(dst + i, x + i);
+            else
+              for (int j = 0; j < 8; j++)
+                if (c0 + i + j < r.dc) dst[i + j] = x[i + j];
+        } else {
+          T* dst = static_cast<T*>(r.out) + at + c0;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            if (r.out_vec && c0 + i + 8 <= r.dc)
+              store_vec<T, 8>(dst + i, x + i);
+            else
+              for (int j = 0; j < 8; j++)
+                if (c0 + i + j < r.dc) dst[i + j] = from_float<T>(x[i + j]);
+        }
+      }
+    }
+    __syncthreads();  // the next chunk's tiles
+  }
+
+  if (ok && OUT) {
+    // tokens past the sequence's end
+    const int end = min(p0 + seg_tokens, r.tokens);
+    const int width = min(64, r.dc - blk * 64);
+    for (int i = tid; i < (end - p0 - done) * 64; i += THREADS) {
+      const int t = p0 + done + (i >> 6), c = i & 63;
+      if (c >= width) continue;
+      const long long at = batch * r.ob + (long long)t * r.ot + head * r.oh + blk * 64 + c;
+      if (r.out_f32)
+        static_cast<float*>(r.out)[at] = 0.f;
+      else
+        static_cast<T*>(r.out)[at] = from_float<T>(0.f);
+    }
+    if (len == 0 && seg == 0 && r.fin) {
+      for (int i = tid; i < r.da * 64; i += THREADS) {
+        const int er = i >> 6, ec = blk * 64 + (i & 63);
+        const long long base = (long long)(batch * r.heads + head) * r.da * r.dc;
+        if (ec < r.dc) r.fin[base + er * r.fr + ec * r.fc] = r.init ? r.init[base + er * r.ir + ec * r.ic] : 0.f;
+      }
+    }
+  }
+  if (ok && !OUT) {
+#pragma unroll
+    for (int s = 0; s < MAXS; s++)
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        if (s < r.slabs)
+          r.seg[(((long long)(batch * r.heads + head) * r.nseg + seg) * (r.slabs * 64) + s * 64 + srow) * ld + blk * 64 +
+                scol + i] = E[s][i];
+  }
+  if (!ok) mbar_wait_drain(bar, phase ^ 1);  // the products still in flight
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) {
+    tmem_relinquish();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+// seg[s]: the state segment s adds -> the state that enters it.
+__global__ void k_scan(const __grid_constant__ Run r) {
+  const int rows = r.slabs * 64, cols = r.blocks * 64;
+  const long long per = (long long)rows * cols;
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= per) return;
+  const int bh = blockIdx.y, head = bh % r.heads, batch = bh / r.heads;
+  const int er = (int)(i / cols), ec = (int)(i % cols);
+  const float g = r.log_decay[head];
+  int len = r.tokens;
+  if (r.lengths) len = min(max(r.lengths[batch], 0), r.tokens);
+  const float lam = power(g, 1);
+  float e = 0.f;
+  if (r.init && er < r.da && ec < r.dc) {
+    e = r.init[(long long)bh * r.da * r.dc + er * r.ir + ec * r.ic];
+    if (!r.reverse) e *= lam;
+  }
+  float* p = r.seg + (long long)bh * r.nseg * per + i;
+  const int seg_tokens = r.chunks * CH;
+  for (int s = 0; s < r.nseg; s++) {
+    const int n = min(max(len - s * seg_tokens, 0), seg_tokens);
+    const float x = s + 1 < r.nseg ? p[s * per] : 0.f;
+    p[s * per] = e;
+    if (n > 0) e = lam * x + power(g, n) * e;
+  }
+}
+
+// Sum over the heads that share one head of the operand: src fp32
+// [rows][heads][d] -> dst [rows][heads / per][d] with strides.
+template <class T>
+__global__ void k_share(const float* src, T* dst, long long rows, int tokens, int heads, int per, int d, long long sb,
+                        long long st, long long sh) {
+  const int nh = heads / per;
+  const long long total = rows * nh * d;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    const int c = (int)(i % d);
+    const long long rh = i / d;
+    const int h = (int)(rh % nh);
+    const long long row = rh / nh;
+    const float* s = src + (row * heads + (long long)h * per) * d + c;
+    float v = 0.f;
+    for (int k = 0; k < per; k++) v += s[(long long)k * d];
+    dst[(row / tokens) * sb + (row % tokens) * st + h * sh + c] = from_float<T>(v);
+  }
+}
+
+template <class T, bool OUT>
+cudaError_t launch_chunks(const Run& r, cudaStream_t st) {
+  const uint32_t bytes = Plan<T>::bytes(r.slabs);
+  cudaError_t ce = cudaFuncSetAttribute(k_chunks<T, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (ce != cudaSuccess) return ce;
+  const long long grid = (long long)r.batch * r.heads * r.blocks * (OUT ? r.nseg : r.nseg - 1);
+  k_chunks<T, OUT><<<(unsigned)grid, THREADS, bytes, st>>>(r);
+  return cudaGetLastError();
+}
+
+// How a sequence is cut: one segment reads everything once, several read b
+// and c twice but fill the GPU.  Picks the least number of chunk steps on the
+// busiest SM, a state-only step counted as half a step and the two more
+// launches as two steps.
+void cut(Run& r) {
+  const int slots = 148;
+  const int chunks = (r.tokens + CH - 1) / CH;
+  const long long rows = (long long)r.batch * r.heads * r.blocks;
+  double best = 1e300;
+  for (int c = chunks;;) {
+    const int nseg = (chunks + c - 1) / c;
+    const double waves = (double)((rows * nseg + slots - 1) / slots);
+    const double cost = waves * c * (nseg > 1 ? 1.5 : 1.0) + (nseg > 1 ? 2.0 : 0.0);
+    if (cost < best) {
+      best = cost;
+      r.nseg = nseg;
+      r.chunks = c;
+    }
+    if (c == 1) break;
+    c = std::max(1, std::min(c - 1, (chunks + nseg) / (nseg + 1)));
+  }
+}
+
+long long seg_floats(const Run& r) {
+  return r.nseg > 1 ? (long long)r.batch * r.heads * r.nseg * r.slabs * 64 * r.blocks * 64 : 0;
+}
+
+template <class T>
+cudaError_t go(const Run& r, cudaStream_t st) {
+  cudaError_t ce = cudaSuccess;
+  if (r.nseg > 1) {
+    if ((ce = launch_chunks<T, false>(r, st)) != cudaSuccess) return ce;
+    const int per = r.slabs * 64 * r.blocks * 64;
+    k_scan<<<dim3((per + 255) / 256, r.batch * r.heads), 256, 0, st>>>(r);
+    if ((ce = cudaGetLastError()) != cudaSuccess) return ce;
+  }
+  return launch_chunks<T, true>(r, st);
+}
+
+cudaError_t go(const Run& r, int dtype, cudaStream_t st) {
+  return dtype == LAMA_F32 ? go<float>(r, st) : dtype == LAMA_F16 ? go<__half>(r, st) : go<__nv_bfloat16>(r, st);
+}
+
+Operand operand(const lama_rows& x, int heads, int d, int dtype) {
+  const int e = dtype_size(dtype);
+  Operand o;
+  o.p = x.data;
+  o.sb = x.batch_stride;
+  o.st = x.token_stride;
+  o.sh = x.head_stride;
+  o.per = heads / x.heads;
+  const long long bits = (long long)(uintptr_t)x.data | (x.batch_stride * e) | (x.token_stride * e) | (x.head_stride * e);
+  o.vec = (bits & 15) == 0 && d % 8 == 0;
+  return o;
+}
+
+void output(Run& r, const lama_rows& x, int d, int dtype) {
+  const Operand o = operand(x, x.heads, d, dtype);
+  r.out = x.data;
+  r.ob = o.sb;
+  r.ot = o.st;
+  r.oh = o.sh;
+  r.out_vec = o.vec;
+  r.out_f32 = 0;
+}
+
+void roles(Run& r, const Operand& a, const Operand& b, const Operand& c, int da, int dc) {
+  r.a = a;
+  r.b = b;
+  r.c = c;
+  r.da = da;
+  r.dc = dc;
+  r.slabs = (da + 63) / 64;
+  r.blocks = (dc + 63) / 64;
+  cut(r);
+}
+
+const char* check_rows(const lama_rows& x, const lama_attention* p, const char* what, char* buf, size_t n) {
+  if (!x.data) {
+    snprintf(buf, n, "%s is null", what);
+    return buf;
+  }
+  if ((uintptr_t)x.data % dtype_size(p->dtype)) {
+    snprintf(buf, n, "%s is not aligned to its elements", what);
+    return buf;
+  }
+  if (x.heads < 1 || p->heads % x.heads) {
+    snprintf(buf, n, "%s has %d heads, which do not divide the %d heads of log_decay", what, x.heads, p->heads);
+    return buf;
+  }
+  return nullptr;
+}
+
+int check(const lama_attention* p, char* err, int err_len) {
+  if (!p) return fail(err, err_len, LAMA_EINVAL, "null arguments");
+  if (!dtype_ok(p->dtype)) return fail(err, err_len, LAMA_EINVAL, "unknown element type %d", p->dtype);
+  if (p->batch < 1 || p->tokens < 1 || p->heads < 1 || p->dk < 1 || p->dv < 1)
+    return fail(err, err_len, LAMA_EINVAL, "batch, tokens, heads, dk and dv must be positive");
+  if (p->dk > 128 || p->dv > 128)
+    return fail(err, err_len, LAMA_EUNSUPPORTED, "head sizes %d and %d exceed 128", p->dk, p->dv);
+  if (p->tokens > (1 << 30) || (long long)p->batch * p->heads > 65535)
+    return fail(err, err_len, LAMA_EUNSUPPORTED, "tokens exceed 2^30 or batch * heads exceeds 65535");
+  if (!p->log_decay) return fail(err, err_len, LAMA_EINVAL, "log_decay is null");
+  char buf[160];
+  const char* m = check_rows(p->q, p, "q", buf, sizeof(buf));
+  if (!m) m = check_rows(p->k, p, "k", buf, sizeof(buf));
+  if (!m) m = check_rows(p->v, p, "v", buf, sizeof(buf));
+  if (m) return fail(err, err_len, LAMA_EINVAL, "%s", m);
+  return LAMA_OK;
+}
+
+Run common(const lama_attention* p) {
+  Run r{};
+  r.log_decay = p->log_decay;
+  r.lengths = p->lengths;
+  r.batch = p->batch;
+  r.tokens = p->tokens;
+  r.heads = p->heads;
+  return r;
+}
+
+Run forward_run(const lama_attention* p) {
+  Run r = common(p);
+  roles(r, operand(p->q, p->heads, p->dk, p->dtype), operand(p->k, p->heads, p->dk, p->dtype),
+        operand(p->v, p->heads, p->dv, p->dtype), p->dk, p->dv);
+  r.inter = r.intra = p->scale;
+  r.update = 1.f;
+  r.init = p->initial_state;
+  r.ir = r.fr = p->dv;
+  r.ic = r.fc = 1;
+  return r;
+}
+
+// The three gradient runs: 0 dq, 1 dk, 2 dv.
+Run gradient_run(const lama_attention* p, const lama_attention_grads* g, int which) {
+  Run r = common(p);
+  const Operand q = operand(p->q, p->heads, p->dk, p->dtype), k = operand(p->k, p->heads, p->dk, p->dtype),
+                v = operand(p->v, p->heads, p->dv, p->dtype), d = operand(g->grad_out, p->heads, p->dv, p->dtype);
+  if (which == 0) {
+    roles(r, d, v, k, p->dv, p->dk);
+    r.inter = r.intra = p->scale;
+    r.update = 1.f;
+    r.init = p->initial_state;
+  } else {
+    if (which == 1)
+      roles(r, v, d, q, p->dv, p->dk);
+    else
+      roles(r, k, q, d, p->dk, p->dv);
+    r.inter = 1.f;
+    r.intra = r.update = p->scale;
+    r.reverse = 1;
+    r.init = g->grad_final_state;
+  }
+  r.ir = r.fr = which == 2 ? p->dv : 1;  // states are [dk][dv]; dq and dk use them transposed
+  r.ic = r.fc = which == 2 ? 1 : p->dv;
+  return r;
+}
+
+constexpr long long ALIGN = 256;
+long long up(long long b) { return (b + ALIGN - 1) / ALIGN * ALIGN; }
+
+}  // namespace
+
+cudaError_t status_word(int** p) { return cudaGetSymbolAddress((void**)p, g_status); }
+
+}  // namespace ops
+}  // namespace lama
+
+using namespace lama::ops;
+
+extern "C" long long lama_linear_attention_workspace(const lama_attention* p, int backward, char* err, int err_len) {
+  if (err && err_len > 0) err[0] = 0;
+  const int rc = check(p, err, err_len);
+  if (rc != LAMA_OK) return rc;
+  if (!backward) return up(seg_floats(forward_run(p)) * 4);
+  lama_attention_grads g{};
+  g.grad_out = p->v;
+  g.grad_out.heads = p->heads;
+  long long seg = 0, share = 0;
+  for (int w = 0; w < 3; w++) seg = std::max(seg, seg_floats(gradient_run(p, &g, w)) * 4);
+  const int heads[3] = {p->q.heads, p->k.heads, p->v.heads}, d[3] = {p->dk, p->dk, p->dv};
+  for (int w = 0; w < 3; w++)
+    if (heads[w] != p->heads) share = std::max(share, (long long)p->batch * p->tokens * p->heads * d[w] * 4);
+  return up(seg) + up(share);
+}
+
+extern "C" int lama_linear_attention(const lama_attention* p, const lama_rows* out, float* final_state, void* workspace,
+                                     long long workspace_bytes, int device, void* stream, char* err, int err_len) {
+  const long long need = lama_linear_attention_workspace(p, 0, err, err_len);
+  if (need < 0) return (int)need;
+  if (!out) return fail(err, err_len, LAMA_EINVAL, "null output");
+  char buf[160];
+  if (const char* m = check_rows(*out, p, "out", buf, sizeof(buf))) return fail(err, err_len, LAMA_EINVAL, "%s", m);
+  if (out->heads != p->heads) return fail(err, err_len, LAMA_EINVAL, "out has %d heads, not %d", out->heads, p->heads);
+  if (workspace_bytes < need || (need && !workspace))
+    return fail(err, err_len, LAMA_EINVAL, "workspace of %lld bytes, %lld needed", workspace_bytes, need);
+  DeviceGuard dev(device);
+  cudaError_t ce = dev.status;
+  Run r = forward_run(p);
+  output(r, *out, p->dv, p->dtype);
+  r.fin = final_state;
+  r.seg = static_cast<float*>(workspace);
+  if (ce == cudaSuccess) ce = status_word(&r.status);
+  if (ce == cudaSuccess) ce = go(r, p->dtype, (cudaStream_t)stream);
+  if (ce != cudaSuccess) return fail(err, err_len, LAMA_ECUDA, "linear attention: %s", cudaGetErrorString(ce));
+  return LAMA_OK;
+}
+
+extern "C" int lama_linear_attention_backward(const lama_attention* p, const lama_attention_grads* g, void* workspace,
+                                              long long workspace_bytes, int device, void* stream, char* err,
+                                              int err_len) {
+  const long long need = lama_linear_attention_workspace(p, 1, err, err_len);
+  if (need < 0) return (int)need;
+  if (!g) return fail(err, err_len, LAMA_EINVAL, "null gradients");
+  char buf[160];
+  const lama_rows* rows[4] = {&g->grad_out, &g->grad_q, &g->grad_k, &g->grad_v};
+  const char* names[4] = {"grad_out", "grad_q", "grad_k", "grad_v"};
+  const int heads[4] = {p->heads, p->q.heads, p->k.heads, p->v.heads};
+  for (int i = 0; i < 4; i++) {
+    if (const char* m = check_rows(*rows[i], p, names[i], buf, sizeof(buf))) return fail(err, err_len, LAMA_EINVAL, "%s", m);
+    if (rows[i]->heads != heads[i])
+      return fail(err, err_len, LAMA_EINVAL, "%s has %d heads, not %d", names[i], rows[i]->heads, heads[i]);
+  }
+  if (workspace_bytes < need || (need && !workspace))
+    return fail(err, err_len, LAMA_EINVAL, "workspace of %lld bytes, %lld needed", workspace_bytes, need);
+  DeviceGuard dev(device);
+  cudaError_t ce = dev.status;
+  int* status = nullptr;
+  if (ce == cudaSuccess) ce = status_word(&status);
+  const cudaStream_t st = (cudaStream_t)stream;
+  long long seg = 0;
+  for (int w = 0; w < 3; w++) seg = std::max(seg, seg_floats(gradient_run(p, g, w)) * 4);
+  float* shared = reinterpret_cast<float*>(static_cast<char*>(workspace) + up(seg));
+  for (int w = 0; w < 3 && ce == cudaSuccess; w++) {
+    Run r = gradient_run(p, g, w);
+    const lama_rows& o = *rows[1 + w];
+    const int d = w == 2 ? p->dv : p->dk;
+    r.seg = static_cast<float*>(workspace);
+    r.status = status;
+    if (w == 2) r.fin = g->grad_initial_state;
+    if (o.heads == p->heads) {
+      output(r, o, d, p->dtype);
+      ce = go(r, p->dtype, st);
+    } else {
+      r.out = shared;
+      r.out_f32 = 1;
+      r.oh = d;
+      r.ot = (long long)p->heads * d;
+      r.ob = r.ot * p->tokens;
+      r.out_vec = d % 8 == 0;
+      ce = go(r, p->dtype, st);
+      if (ce != cudaSuccess) break;
+      const long long n = (long long)p->batch * p->tokens;
+      const int per = p->heads / o.heads;
+      const unsigned grid = (unsigned)std::min<long long>((n * o.heads * d + 255) / 256, 148 * 16);
+      auto share = [&](auto* dst) {
+        k_share<<<grid, 256, 0, st>>>(shared, dst, n, p->tokens, p->heads, per, d, o.batch_stride, o.token_stride,
+                                      o.head_stride);
+      };
+      if (p->dtype == LAMA_F32)
+        share(static_cast<float*>(o.data));
+      else if (p->dtype == LAMA_F16)
+        share(static_cast<__half*>(o.data));
+      else
+        share(static_cast<__nv_bfloat16*>(o.data));
+      ce = cudaGetLastError();
+    }
+  }
+  if (ce != cudaSuccess) return fail(err, err_len, LAMA_ECUDA, "linear attention backward: %s", cudaGetErrorString(ce));
+  return LAMA_OK;
+}
+
+extern "C" int lama_operator_status(int device, char* err, int err_len) {
+  if (err && err_len > 0) err[0] = 0;
+  DeviceGuard dev(device);
+  cudaError_t ce = dev.status;
+  int *p = nullptr, code = 0;
+  const int zero = 0;
+  if (ce == cudaSuccess) ce = status_word(&p);
+  if (ce == cudaSuccess) ce = cudaDeviceSynchronize();
+  if (ce == cudaSuccess) ce = cudaMemcpy(&code, p, sizeof(int), cudaMemcpyDeviceToHost);
+  if (ce == cudaSuccess && code) ce = cudaMemcpy(p, &zero, sizeof(int), cudaMemcpyHostToDevice);
+  if (ce != cudaSuccess) return fail(err, err_len, LAMA_ECUDA, "operator status: %s", cudaGetErrorString(ce));
+  if (code) return fail(err, err_len, LAMA_EDEVICE, "a kernel wait timed out (code %d)", code);
+  return LAMA_OK;
+}

@@ -1,0 +1,117 @@
+// What the token-mixer operators share: element types, error text, the CUDA
+// device guard and the device status word of their bounded waits.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+#include "lama_b200.h"
+
+namespace lama {
+namespace ops {
+
+inline int fail(char* err, int err_len, int code, const char* fmt, ...) {
+  if (err && err_len > 0) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(err, (size_t)err_len, fmt, ap);
+    va_end(ap);
+  }
+  return code;
+}
+
+// Makes `device` current for the duration of a call and restores the caller's.
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(int device) {
+    if ((status = cudaGetDevice(&prev_)) == cudaSuccess && prev_ != device) {
+      status = cudaSetDevice(device);
+      moved_ = status == cudaSuccess;
+    }
+    if (status != cudaSuccess) cudaGetLastError();  // not sticky: keep it from the caller's next call
+  }
+  ~DeviceGuard() {
+    if (moved_) cudaSetDevice(prev_);
+  }
+  cudaError_t status = cudaSuccess;
+
+ private:
+  int prev_ = 0;
+  bool moved_ = false;
+};
+
+// The status word of the operators' bounded waits on the current device
+// (0: no wait ran out).
+cudaError_t status_word(int** p);
+
+inline int dtype_size(int t) { return t == LAMA_F32 ? 4 : 2; }
+inline bool dtype_ok(int t) { return t == LAMA_F32 || t == LAMA_F16 || t == LAMA_BF16; }
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// N consecutive elements as floats; N * sizeof(T) is 8 or a multiple of 16
+// and p is aligned to min(16, N * sizeof(T)).
+template <class T, int N>
+__device__ __forceinline__ void load_vec(const T* p, float* v) {
+  constexpr int BYTES = N * (int)sizeof(T);
+  if constexpr (BYTES >= 16) {
+    constexpr int PER = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; i++) {
+      const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+      const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int j = 0; j < PER; j++) v[i * PER + j] = to_float(e[j]);
+    }
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int j = 0; j < N; j++) v[j] = to_float(e[j]);
+  }
+}
+template <class T, int N>
+__device__ __forceinline__ void store_vec(T* p, const float* v) {
+  constexpr int BYTES = N * (int)sizeof(T);
+  if constexpr (BYTES >= 16) {
+    constexpr int PER = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; i++) {
+      uint4 u;
+      T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+      for (int j = 0; j < PER; j++) e[j] = from_float<T>(v[i * PER + j]);
+      reinterpret_cast<uint4*>(p)[i] = u;
+    }
+  } else {
+    uint2 u;
+    T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int j = 0; j < N; j++) e[j] = from_float<T>(v[j]);
+    *reinterpret_cast<uint2*>(p) = u;
+  }
+}
+
+}  // namespace ops
+}  // namespace lama

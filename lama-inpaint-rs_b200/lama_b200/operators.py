@@ -1,0 +1,517 @@
+"""Token-mixer operators on CUDA tensors (include/lama_b200.h, no counterpart in the reference).
+
+Three operators for a block that mixes the tokens of a latent plane (or of any sequence), in
+inference and training:
+
+* `linear_attention`, `linear_attention_backward`, `linear_attention_step`: linear attention with a
+  decay for each head, over whole sequences and one token at a time;
+* `gated_residual_norm`, `gated_residual_norm_backward`: the norm after a block, its gate and
+  residual scale, the residual sum and the norm before the next block in one pass;
+* `checkpoint_store`, `checkpoint_restore`: an activation kept in 8 bits for the backward pass, which
+  `gated_residual_norm(save="int8")` also writes and its backward pass reads.
+
+Tensors are torch tensors on one CUDA device, of type float32, float16 or bfloat16; work is queued on
+torch's current stream of that device.  `linear_attention` and `gated_residual_norm` take part in
+autograd.  Wrong arguments and GPU errors raise `LamaError`; a bounded wait of a kernel that ran out
+is reported by `check_operators`.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import threading
+from dataclasses import dataclass, field
+from typing import NamedTuple
+
+import torch
+
+from .engine import AttentionArgs, AttentionGrads, LamaError, NormArgs, NormGrads, Rows, lib
+
+__all__ = ["Checkpoint8", "check_operators", "checkpoint_restore", "checkpoint_store", "gated_residual_norm",
+           "gated_residual_norm_backward", "linear_attention", "linear_attention_backward",
+           "linear_attention_step"]
+
+EINVAL = -1
+GROUP = 128  # channels that share a scale of an 8-bit checkpoint
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class _Message(threading.local):
+    def __init__(self):
+        self.buf = ctypes.create_string_buffer(256)
+
+
+_err = _Message()  # the library's message of this thread's last call
+
+
+def _refuse(msg):
+    raise LamaError(EINVAL, msg)
+
+
+def _check(rc):
+    if rc < 0:
+        raise LamaError(int(rc), _err.buf.value.decode())
+    return rc
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _tensor(t, name, like=None, dtype=None, ndim=None, shape=None):
+    if not isinstance(t, torch.Tensor):
+        _refuse(f"{name} is not a tensor")
+    if not t.is_cuda:
+        _refuse(f"{name} is not on a CUDA device")
+    if like is not None and t.device != like.device:
+        _refuse(f"{name} is on {t.device}, not on {like.device}")
+    if dtype is None and t.dtype not in _TYPES:
+        _refuse(f"{name} has type {t.dtype}; float32, float16 and bfloat16 are supported")
+    if dtype is not None and t.dtype != dtype:
+        _refuse(f"{name} has type {t.dtype}, not {dtype}")
+    if ndim is not None and t.dim() != ndim:
+        _refuse(f"{name} has {t.dim()} dimensions, not {ndim}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        _refuse(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+
+
+def check_operators(device=None) -> None:
+    """Wait for the device and raise `LamaError` if a kernel's bounded wait ran out since the last call."""
+    dev = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    _check(lib().lama_operator_status(dev, _err.buf, 256))
+
+
+# ------------------------------------------------------------------ linear attention
+
+def _unit(t):
+    """The tensor itself if its last dimension is contiguous, else a copy."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _rows(t):
+    """[B,T,n,D] (or [B,n,D]) as the library's row description."""
+    s = [0 if n == 1 else v for n, v in zip(t.shape, t.stride())]  # a lone row's stride is arbitrary
+    return Rows(t.data_ptr(), s[0], s[1] if t.dim() == 4 else 0, s[-2], t.shape[-2])
+
+
+def _attention(q, k, v, log_decay, scale, initial_state, lengths, ndim):
+    _tensor(q, "q", ndim=ndim)
+    for t, name in ((k, "k"), (v, "v")):
+        _tensor(t, name, q, q.dtype, ndim)
+        if t.shape[:-2] != q.shape[:-2]:
+            _refuse(f"{name} has shape {tuple(t.shape)}, which does not go with q's {tuple(q.shape)}")
+    if k.shape[-1] != q.shape[-1]:
+        _refuse(f"q has {q.shape[-1]} channels a head and k {k.shape[-1]}")
+    _tensor(log_decay, "log_decay", q, torch.float32, 1)
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        _refuse("log_decay has no gradient: the decays are constants of the layer")
+    h, dk, dv = log_decay.numel(), q.shape[-1], v.shape[-1]
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.shape[-2] < 1 or h % t.shape[-2]:
+            _refuse(f"{name} has {t.shape[-2]} heads, which do not divide the {h} of log_decay")
+    if not 1 <= dk <= 128 or not 1 <= dv <= 128:
+        _refuse(f"head sizes {dk} and {dv} are not in 1..128")
+    if initial_state is not None:
+        _tensor(initial_state, "initial_state", q, torch.float32, shape=(q.shape[0], h, dk, dv))
+    if lengths is not None:
+        _tensor(lengths, "lengths", q, torch.int32, shape=(q.shape[0],))
+    return h, dk, dv, (dk ** -0.5 if scale is None else float(scale))
+
+
+def _attention_args(q, k, v, log_decay, scale, initial_state, lengths, h, dk, dv):
+    return AttentionArgs(_TYPES[q.dtype], q.shape[0], q.shape[1] if q.dim() == 4 else 1, h, dk, dv, _rows(q), _rows(k),
+                         _rows(v), log_decay.data_ptr(), _ptr(initial_state), _ptr(lengths), scale)
+
+
+def _workspace(n, like):
+    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
+
+
+def _attention_forward(q, k, v, log_decay, scale, initial_state, lengths, return_state):
+    h, dk, dv, scale = _attention(q, k, v, log_decay, scale, initial_state, lengths, 4)
+    q, k, v, log_decay = _unit(q), _unit(k), _unit(v), log_decay.contiguous()
+    b, t = q.shape[:2]
+    o = torch.empty(b, t, h, dv, dtype=q.dtype, device=q.device)
+    state = torch.empty(b, h, dk, dv, dtype=torch.float32, device=q.device) if return_state else None
+    if b == 0 or t == 0:
+        if return_state:
+            state.zero_() if initial_state is None else state.copy_(initial_state)
+        return o, state
+    initial_state = None if initial_state is None else initial_state.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    a = _attention_args(q, k, v, log_decay, scale, initial_state, lengths, h, dk, dv)
+    n = _check(lib().lama_linear_attention_workspace(a, 0, _err.buf, 256))
+    w = _workspace(n, q)
+    _check(lib().lama_linear_attention(a, _rows(o), _ptr(state), _ptr(w), n, q.device.index, _stream(q), _err.buf, 256))
+    return o, state
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, scale, initial_state, lengths):
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return _attention_forward(q, k, v, log_decay, scale, initial_state, lengths, True)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_o, grad_state):
+        q, k, v, log_decay, initial_state, lengths = ctx.saved_tensors
+        if grad_o is None:
+            grad_o = q.new_zeros(*q.shape[:2], log_decay.numel(), v.shape[-1])
+        dq, dk, dv, ds = linear_attention_backward(grad_o, q, k, v, log_decay, scale=ctx.scale,
+                                                   initial_state=initial_state, lengths=lengths,
+                                                   grad_state=grad_state)
+        return dq, dk, dv, None, None, ds, None
+
+
+def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengths=None, return_state=False):
+    """Linear attention with a decay for each head over whole sequences.
+
+    S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t
+
+    q, k: [B,T,n,dk], v: [B,T,n,dv], each with its own number n of heads that divides the H heads of
+    log_decay [H] (float32, a constant of the layer; -inf is no memory): a head is shared by H/n
+    neighbours.  Any strides.  scale: 1/sqrt(dk) unless given.  initial_state: [B,H,dk,dv] float32,
+    zeros unless given.  lengths: [B] int32, the tokens of each sequence (later ones are not read, their
+    outputs are 0).  Returns o [B,T,H,dv], or (o, state after the last token) with return_state.
+    """
+    grads = torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
+                                            for t in (q, k, v, initial_state))
+    if grads:
+        o, state = _LinearAttention.apply(q, k, v, log_decay, scale, initial_state, lengths)
+    else:
+        o, state = _attention_forward(q, k, v, log_decay, scale, initial_state, lengths, return_state)
+    return (o, state) if return_state else o
+
+
+def linear_attention_backward(grad_o, q, k, v, log_decay, *, scale=None, initial_state=None, lengths=None,
+                              grad_state=None):
+    """(dq, dk, dv, d_initial_state) of `linear_attention` for the gradients grad_o [B,T,H,dv] of its output
+    and grad_state (None: zeros) of its final state; d_initial_state is None without an initial_state."""
+    h, dk, dv, scale = _attention(q, k, v, log_decay, scale, initial_state, lengths, 4)
+    b, t = q.shape[:2]
+    _tensor(grad_o, "grad_o", q, q.dtype, shape=(b, t, h, dv))
+    if grad_state is not None:
+        _tensor(grad_state, "grad_state", q, torch.float32, shape=(b, h, dk, dv))
+        grad_state = grad_state.contiguous()
+    q, k, v, grad_o, log_decay = _unit(q), _unit(k), _unit(v), _unit(grad_o), log_decay.contiguous()
+    grads = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v)]
+    ds = None if initial_state is None else torch.empty_like(initial_state, memory_format=torch.contiguous_format)
+    if b == 0 or t == 0:
+        if ds is not None:
+            ds.zero_() if grad_state is None else ds.copy_(grad_state)
+        return (*grads, ds)
+    initial_state = None if initial_state is None else initial_state.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    a = _attention_args(q, k, v, log_decay, scale, initial_state, lengths, h, dk, dv)
+    g = AttentionGrads(_rows(grad_o), *(_rows(x) for x in grads), _ptr(grad_state), _ptr(ds))
+    n = _check(lib().lama_linear_attention_workspace(a, 1, _err.buf, 256))
+    w = _workspace(n, q)
+    _check(lib().lama_linear_attention_backward(a, g, _ptr(w), n, q.device.index, _stream(q), _err.buf, 256))
+    return (*grads, ds)
+
+
+def linear_attention_step(q, k, v, log_decay, state, *, scale=None, slots=None, out_state=None):
+    """One token of `linear_attention` for each row: S <- exp(log_decay) S + k v^T, o = scale q S.
+
+    q, k: [B,n,dk], v: [B,n,dv] (heads shared as in `linear_attention`); state: [N,H,dk,dv] float32,
+    contiguous, updated in place unless out_state, a separate buffer of its shape, takes the new states.
+    slots: [B] int32, the state of each row, no slot twice (row b has slot b unless given); a slot
+    outside 0..N-1 marks an unused row, whose output is 0.  Returns o [B,H,dv].  Has no gradient.
+    """
+    h, dk, dv, scale = _attention(q, k, v, log_decay, scale, None, None, 3)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+        _refuse("a step has no gradient: call it under torch.no_grad() or use linear_attention")
+    b = q.shape[0]
+    _tensor(state, "state", q, torch.float32, 4)
+    if tuple(state.shape[1:]) != (h, dk, dv) or not state.is_contiguous():
+        _refuse(f"state is not a contiguous tensor of shape (slots, {h}, {dk}, {dv})")
+    out_state = state if out_state is None else out_state
+    _tensor(out_state, "out_state", q, torch.float32, shape=state.shape)
+    if not out_state.is_contiguous():
+        _refuse("out_state is not contiguous")
+    if slots is not None:
+        _tensor(slots, "slots", q, torch.int32, shape=(b,))
+        slots = slots.contiguous()
+    elif state.shape[0] < b:
+        _refuse(f"{state.shape[0]} states for {b} rows")
+    q, k, v, log_decay = _unit(q), _unit(k), _unit(v), log_decay.contiguous()
+    o = torch.empty(b, h, dv, dtype=q.dtype, device=q.device)
+    if b == 0:
+        return o
+    if state.shape[0] == 0:
+        return o.zero_()
+    a = _attention_args(q, k, v, log_decay, scale, None, None, h, dk, dv)
+    _check(lib().lama_linear_attention_step(a, _rows(o), state.data_ptr(), out_state.data_ptr(), state.shape[0],
+                                            _ptr(slots), q.device.index, _stream(q), _err.buf, 256))
+    return o
+
+
+# ------------------------------------------------------------------ 8-bit checkpoints
+
+@dataclass
+class Checkpoint8:
+    """An activation in 8 bits: codes [...,C] int8, scales [...,ceil(C/128)] float32, the type it had."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    dtype: torch.dtype
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.nbytes + self.scales.nbytes
+
+
+def _row_view(t):
+    """[...,C] as a matrix of rows with one stride between them (a copy where its strides do not allow that)."""
+    m = t if t.dim() == 2 else t.flatten(0, -2) if t.dim() > 1 else t[None]
+    if m.shape[-1] > 1 and m.stride(-1) != 1 or m.shape[0] > 1 and m.stride(0) < m.shape[1]:
+        m = m.contiguous()
+    return m
+
+
+def _row_stride(m):
+    return m.stride(0) if m.shape[0] > 1 else m.shape[1]
+
+
+def _empty_checkpoint(x):
+    groups = (x.shape[-1] + GROUP - 1) // GROUP
+    return Checkpoint8(torch.empty(x.shape, dtype=torch.int8, device=x.device),
+                       torch.empty(*x.shape[:-1], groups, dtype=torch.float32, device=x.device), x.dtype)
+
+
+def checkpoint_store(x) -> Checkpoint8:
+    """x [...,C] in 8 bits, a scale for each row and group of 128 channels."""
+    _tensor(x, "x")
+    if x.dim() < 1:
+        _refuse("x has no channels")
+    c = _empty_checkpoint(x)
+    if x.numel():
+        m = _row_view(x.detach())
+        _check(lib().lama_checkpoint_store(m.data_ptr(), _TYPES[x.dtype], m.shape[0], m.shape[1], _row_stride(m),
+                                           c.codes.data_ptr(), c.scales.data_ptr(), x.device.index, _stream(x),
+                                           _err.buf, 256))
+    return c
+
+
+def checkpoint_restore(ckpt: Checkpoint8, dtype=None) -> torch.Tensor:
+    """The activation a checkpoint stands for, in its own type unless `dtype` is given."""
+    if not isinstance(ckpt, Checkpoint8):
+        _refuse("not a Checkpoint8")
+    dtype = ckpt.dtype if dtype is None else dtype
+    if dtype not in _TYPES:
+        _refuse(f"type {dtype} is not supported")
+    codes, scales = ckpt.codes, ckpt.scales
+    _tensor(codes, "codes", dtype=torch.int8)
+    _tensor(scales, "scales", codes, torch.float32,
+            shape=(*codes.shape[:-1], (codes.shape[-1] + GROUP - 1) // GROUP))
+    x = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    if x.numel():
+        codes, scales, c = codes.contiguous(), scales.contiguous(), codes.shape[-1]
+        _check(lib().lama_checkpoint_restore(codes.data_ptr(), scales.data_ptr(), _TYPES[dtype], x.numel() // c, c, c,
+                                             x.data_ptr(), x.device.index, _stream(x), _err.buf, 256))
+    return x
+
+
+# ------------------------------------------------------------------ norms, gate and residual
+
+@dataclass
+class SavedNorm:
+    """What `gated_residual_norm` keeps for its backward pass."""
+    args: tuple = field(repr=False)  # post_weight, pre_weight, gate (as given), residual_scale, eps
+    y: torch.Tensor | Checkpoint8
+    u: torch.Tensor | Checkpoint8 | None
+    post_rstd: torch.Tensor | None
+    pre_rstd: torch.Tensor | None
+    shape: tuple
+    dtype: torch.dtype
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.nbytes for t in (self.y, self.u, self.post_rstd, self.pre_rstd) if t is not None)
+
+
+class NormGradients(NamedTuple):
+    x: torch.Tensor
+    y: torch.Tensor
+    post_weight: torch.Tensor | None
+    pre_weight: torch.Tensor | None
+    gate: torch.Tensor | None
+    residual_scale: torch.Tensor | None
+
+
+def _gate_rows(gate, shape):
+    """A gate that broadcasts over x's shape as (its rows as a matrix, rows of x that share one of them).
+    Its dimensions of size 1 have to be the innermost of x's row dimensions."""
+    lead = shape[:-1]
+    g = [1] * (len(lead) - (gate.dim() - 1)) + list(gate.shape[:-1])
+    if gate.dim() < 1 or gate.dim() > len(shape) or gate.shape[-1] != shape[-1]:
+        _refuse(f"a gate of shape {tuple(gate.shape)} does not broadcast over {tuple(shape)}")
+    per, whole = 1, False
+    for n, m in zip(reversed(g), reversed(lead)):
+        if n == m and (m != 1 or whole):
+            whole = True
+        elif n == 1 and not whole:
+            per *= m
+        elif n != m:
+            _refuse(f"a gate of shape {tuple(gate.shape)} does not broadcast over {tuple(shape)} one gate row to "
+                    "neighbouring rows; expand it")
+    return _row_view(gate), per
+
+
+def _norm_args(x, post_weight, pre_weight, gate, residual_scale, eps):
+    c = x.shape[-1]
+    scales = None
+    if isinstance(residual_scale, torch.Tensor):
+        _tensor(residual_scale, "residual_scale", x, shape=(c,))
+        scales, residual_scale = residual_scale.detach().float().contiguous(), 0.0
+    for w, name in ((post_weight, "post_weight"), (pre_weight, "pre_weight")):
+        if w is not None:
+            _tensor(w, name, x, shape=(c,))
+    post_weight = None if post_weight is None else post_weight.detach().float().contiguous()
+    pre_weight = None if pre_weight is None else pre_weight.detach().float().contiguous()
+    rows, per = None, 1
+    if gate is not None:
+        _tensor(gate, "gate", x, x.dtype)
+        rows, per = _gate_rows(gate.detach(), x.shape)
+    a = NormArgs(_TYPES[x.dtype], x.numel() // c, c, _ptr(rows), per, 0 if rows is None else _row_stride(rows),
+                 _ptr(post_weight), _ptr(pre_weight), _ptr(scales), float(residual_scale), float(eps))
+    return a, (post_weight, pre_weight, rows, scales)  # the tensors a points to
+
+
+def _norm_forward(x, y, post_weight, pre_weight, gate, residual_scale, eps, save):
+    _tensor(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        _refuse("x has no channels")
+    _tensor(y, "y", x, x.dtype, shape=x.shape)
+    if save not in (None, "full", "int8"):
+        _refuse(f"save is {save!r}, not None, 'full' or 'int8'")
+    if not float(eps) >= 0:
+        _refuse("eps must not be negative")
+    u = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n = None if pre_weight is None else torch.empty_like(u)
+    ry = ru = cy = cu = None
+    if save:
+        ry = None if post_weight is None else torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        ru = None if pre_weight is None else torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if save == "int8":
+        cy = _empty_checkpoint(y)
+        cu = None if pre_weight is None else _empty_checkpoint(u)
+    a, keep = (None, None) if not x.numel() else _norm_args(x, post_weight, pre_weight, gate, residual_scale, eps)
+    if a is not None:
+        mx, my = _row_view(x.detach()), _row_view(y.detach())
+        _check(lib().lama_gated_residual_norm(
+            a, mx.data_ptr(), _row_stride(mx), my.data_ptr(), _row_stride(my), u.data_ptr(), _ptr(n), _ptr(ry), _ptr(ru),
+            cy and cy.codes.data_ptr(), cy and cy.scales.data_ptr(), cu and cu.codes.data_ptr(),
+            cu and cu.scales.data_ptr(), x.device.index, _stream(x), _err.buf, 256))
+    saved = None
+    if save:
+        saved = SavedNorm((post_weight, pre_weight, gate, residual_scale, eps), cy if cy is not None else y.detach(),
+                          None if pre_weight is None else cu if cu is not None else u, ry, ru, x.shape, x.dtype)
+    return u, n, saved
+
+
+class _GatedResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, post_weight, pre_weight, gate, residual_scale, eps, int8):
+        u, n, saved = _norm_forward(x, y, post_weight, pre_weight, gate, residual_scale, eps,
+                                    "int8" if int8 else "full")
+        # everything goes through save_for_backward, so that autograd sees in-place changes and frees it in time
+        flat = []
+        for t in (saved.y, saved.u):
+            flat += [t.codes, t.scales] if isinstance(t, Checkpoint8) else [t, None]
+        scale = residual_scale if isinstance(residual_scale, torch.Tensor) else None
+        ctx.save_for_backward(*flat, saved.post_rstd, saved.pre_rstd, post_weight, pre_weight, gate, scale)
+        ctx.int8, ctx.scale, ctx.eps = int8, None if scale is not None else residual_scale, eps
+        ctx.shape, ctx.dtype = x.shape, x.dtype
+        ctx.set_materialize_grads(False)
+        return (u, n) if n is not None else u
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_u, grad_n=None):
+        y, ys, u, us, ry, ru, post_weight, pre_weight, gate, scale = ctx.saved_tensors
+        if ctx.int8:
+            y = Checkpoint8(y, ys, ctx.dtype)
+            u = None if u is None else Checkpoint8(u, us, ctx.dtype)
+        saved = SavedNorm((post_weight, pre_weight, gate, ctx.scale if scale is None else scale, ctx.eps), y, u, ry, ru,
+                          ctx.shape, ctx.dtype)
+        g = gated_residual_norm_backward(grad_u, grad_n, saved)
+        return g.x, g.y, g.post_weight, g.pre_weight, g.gate, g.residual_scale, None, None
+
+
+def gated_residual_norm(x, y, *, post_weight=None, pre_weight=None, gate=None, residual_scale=1.0, eps=1e-6, save=None):
+    """The norm after a block, its gate and residual scale, the residual sum and the next block's norm.
+
+    p = post_weight * rms_norm(y)   (p = y without post_weight)
+    u = x + residual_scale * gate * p
+    n = pre_weight * rms_norm(u)    (n = None without pre_weight)
+
+    x, y: [...,C]; weights [C]; gate: None, or a tensor of x's type that broadcasts over x with its
+    size-1 dimensions innermost ([B,1,C], [B,T,C], [C]); residual_scale: a number or [C].  Returns (u, n), or
+    (u, n, saved) with save="full" (y and u themselves are kept) or save="int8" (8-bit checkpoints of
+    them, written in the same pass): `gated_residual_norm_backward` takes `saved`.  Under autograd, "int8"
+    keeps the checkpoints in the graph and `saved` is None.
+    """
+    ts = (x, y, post_weight, pre_weight, gate, residual_scale)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts):
+        if save not in (None, "full", "int8"):
+            _refuse(f"save is {save!r}, not None, 'full' or 'int8'")
+        out = _GatedResidualNorm.apply(*ts, eps, save == "int8")
+        u, n = out if isinstance(out, tuple) else (out, None)
+        return (u, n, None) if save else (u, n)
+    u, n, saved = _norm_forward(*ts, eps, save)
+    return (u, n, saved) if save else (u, n)
+
+
+def gated_residual_norm_backward(grad_u, grad_n, saved) -> NormGradients:
+    """Gradients of `gated_residual_norm` for those of u and n (either may be None: zeros)."""
+    post_weight, pre_weight, gate, residual_scale, eps = saved.args
+    some = saved.y.codes if isinstance(saved.y, Checkpoint8) else saved.y
+    shape, dtype, dev = saved.shape, saved.dtype, some.device
+    c = shape[-1]
+    for g, name in ((grad_u, "grad_u"), (grad_n, "grad_n")):
+        if g is not None:
+            _tensor(g, name, some, dtype, shape=shape)
+
+    def vector(w):
+        return torch.zeros(c, dtype=torch.float32, device=dev) if isinstance(w, torch.Tensor) else None
+
+    dx, dy = (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
+    dpost, dpre, dscale = vector(post_weight), vector(pre_weight), vector(residual_scale)
+    dgate = None if gate is None else torch.empty(gate.shape, dtype=dtype, device=dev)
+    if dx.numel():
+        a, keep = _norm_args(dx, post_weight, pre_weight, gate, residual_scale, eps)
+        mu = None if grad_u is None else _row_view(grad_u)
+        mn = None if grad_n is None else _row_view(grad_n)
+        g = NormGrads()
+        g.grad_u, g.grad_u_stride = _ptr(mu), 0 if mu is None else _row_stride(mu)
+        g.grad_n, g.grad_n_stride = _ptr(mn), 0 if mn is None else _row_stride(mn)
+        hold = []
+        for t, name in ((saved.y, "y"), (saved.u, "u")):
+            if isinstance(t, Checkpoint8):
+                setattr(g, name + "_codes", t.codes.data_ptr())
+                setattr(g, name + "_scales", t.scales.data_ptr())
+            elif t is not None:
+                m = _row_view(t)
+                hold.append(m)
+                setattr(g, name, m.data_ptr())
+                setattr(g, name + "_stride", _row_stride(m))
+        g.post_rstd, g.pre_rstd = _ptr(saved.post_rstd), _ptr(saved.pre_rstd)
+        g.grad_x, g.grad_y, g.grad_gate = dx.data_ptr(), dy.data_ptr(), _ptr(dgate)
+        g.grad_post_weight, g.grad_pre_weight, g.grad_residual_scales = _ptr(dpost), _ptr(dpre), _ptr(dscale)
+        n = _check(lib().lama_gated_residual_norm_workspace(a, _err.buf, 256))
+        w = _workspace(n, dx)
+        _check(lib().lama_gated_residual_norm_backward(a, g, _ptr(w), n, dev.index, _stream(dx), _err.buf, 256))
+    elif dgate is not None:
+        dgate.zero_()
+
+    def like(g, w):
+        return g if g is None or g.dtype == w.dtype else g.to(w.dtype)
+
+    return NormGradients(dx, dy, like(dpost, post_weight), like(dpre, pre_weight), dgate, like(dscale, residual_scale))
