@@ -1,0 +1,548 @@
+// Linear attention over whole sequences for bf16 inputs and outputs with
+// 16-byte-aligned rows (head sizes are then multiples of 8): the recurrence of linear_attention.cu (roles (a; b, c), S = sum b c^T,
+// out = a S) as one pipeline per CTA.
+//
+// A CTA takes one segment of one (sequence, head, 64 columns of c) and walks
+// its 128-token chunks; the chunks overlap, each step by its own warps:
+//
+//   warp  12      loads a, b, c (TMA, zeros past the tokens and the head) into
+//                 a ring of stages
+//   warps  8..11  state: b decayed to the chunk's end, rounded, as an MMA
+//                 operand; U = c^T b~ back from TMEM; the state in registers
+//                 (fp32), E' = lam^n E + lam U, and E as two bf16 parts
+//   warp  13      issues the MMAs: U = c^T b~, S = a b^T, O = a E, O += P c
+//   warps  0..7   two groups that take chunks in turn: scores S from TMEM,
+//                 decay and causal mask, rounded to bf16 P in S's place (the
+//                 A operand of O += P c comes from TMEM); O's rows times
+//                 lam^i in place before that product; O to memory
+//
+// U and S need no state, so only O = a E waits for the chunk before; the
+// two groups hide the latency of each other's products.  A chunk's own tokens
+// run forward or, for the gradients of b and c, backward in time (REV: the
+// mask and every power of lam mirrored, the chunks taken last to first).
+//
+// Rounding: P and, where U only feeds the outputs of the same segment, the
+// decayed b to one bf16 part (both errors are of the size of the output's own
+// rounding and do not add up on one term), E to two.  The states that segments
+// hand on, and the final state, come from the kernel without outputs, with the
+// decayed b in three parts (24 bits): they are fp32 results.  So a final state
+// costs a pass over b and c, and outputs do not depend on asking for it.
+//
+// TMEM: two chunks' S (128 columns, P over them) and O (64), and U.
+#include "attention.cuh"
+
+namespace lama {
+namespace ops {
+
+namespace {
+
+constexpr int THREADS = 14 * 32;  // 4 warps a scheduler at most: 128 registers a thread
+
+template <int NS, bool OUT>
+struct Lay {
+  static constexpr int UP = OUT ? 1 : 3;  // parts of b~
+  static constexpr int STAGES = OUT ? (NS == 1 ? 3 : 2) : (NS == 1 ? 3 : 2);
+  static constexpr int KB = NS == 1 ? 2 : 1;  // buffers of b~ and of U
+  static constexpr int ES = NS == 1 ? 2 : 1;                                       // buffers of E
+  static constexpr uint32_t A = 0, B = OUT ? NS * TILE : 0, C = B + NS * TILE, STAGE = C + TILE;
+  static constexpr uint32_t BD = STAGES * STAGE, BD_BUF = UP * NS * TILE;
+  static constexpr uint32_t E = BD + KB * BD_BUF, E_BUF = 2 * NS * ETILE;
+  static constexpr uint32_t BYTES = E + (OUT ? ES * E_BUF : 0);
+  static constexpr uint32_t T_U = OUT ? 384 : 0;  // TMEM column of U; buffer i of S at 192 i, of O at 192 i + 128
+  static_assert(T_U + KB * 64 * NS <= 512, "TMEM columns");
+};
+
+struct Bars {
+  uint64_t full[4], empty[4], bd[2], u[2], e[2], s[2], p[2], o[2], oe[2];
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+
+// true in one lane of the (converged) warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// A from TMEM (128 lanes, two 16-bit elements a column), B from shared memory
+__device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// The roles' loops share the instruction cache: what is rare stays out of line,
+// and what repeats is a loop (unrolled throughout, the kernel was 143 KB of
+// code and took 5.8 us a chunk).
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t phase, int* err, int code) {
+  return mbar_wait(bar, phase, err, code);
+}
+
+template <int NS, bool OUT, bool REV>
+__global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run r,
+                                                        const __grid_constant__ Maps maps, int segs) {
+  using L = Lay<NS, OUT>;
+  constexpr int UP = L::UP;
+  using T = __nv_bfloat16;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(16) float pw[CH + 4];
+  __shared__ __align__(16) float rv[32];  // lam^{31-j}
+  __shared__ Bars bars;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  int id = blockIdx.x;
+  const int slot = id % segs;  // in the order of the recurrence
+  id /= segs;
+  const int blk = id % r.blocks;
+  id /= r.blocks;
+  const int head = id % r.heads, batch = id / r.heads;
+  const float g = r.log_decay[head];
+  int len = r.tokens;
+  if (r.lengths) len = min(max(r.lengths[batch], 0), r.tokens);
+  const int seg_tokens = r.chunks * CH;
+  const int seg = REV ? r.nseg - 1 - slot : slot;
+  const int p0 = seg * seg_tokens;
+  const int mine = min(max(len - p0, 0), seg_tokens);  // tokens of this segment
+  const int live = (mine + CH - 1) / CH;
+  // the c-th chunk of the recurrence starts at token p0 + at(c) and has num(c) tokens
+  auto at = [&](int c) { return (REV ? live - 1 - c : c) * CH; };
+  auto num = [&](int c) { return min(CH, mine - at(c)); };
+
+  if (warp == 0) tmem_alloc(smem_u32(&tmem_slot), 512);
+  if (tid == 32) {
+    failed = 0;
+    for (int i = 0; i < 4; i++) {
+      mbar_init(smem_u32(&bars.full[i]), 1);
+      mbar_init(smem_u32(&bars.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(smem_u32(&bars.bd[i]), 4);
+      mbar_init(smem_u32(&bars.u[i]), 1);
+      mbar_init(smem_u32(&bars.e[i]), 4);
+      mbar_init(smem_u32(&bars.s[i]), 1);
+      mbar_init(smem_u32(&bars.p[i]), 4);
+      mbar_init(smem_u32(&bars.o[i]), 1);
+      mbar_init(smem_u32(&bars.oe[i]), 4);
+    }
+    fence_mbar_init();
+  }
+  for (int i = tid; i <= CH; i += THREADS) pw[i] = power(g, i);
+  for (int i = tid; i < 32; i += THREADS) rv[i] = power(g, 31 - i);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  // barrier i of a set of n for the c-th chunk: its phase ends once every n chunks
+  auto wait = [&](uint64_t* set, int n, int c, int code) {
+    const uint32_t bar = smem_u32(&set[c % n]), ph = (uint32_t)(c / n) & 1;
+    return mbar_try_wait(bar, ph) || wait_long(bar, ph, &failed, code);
+  };
+  auto arrive = [&](uint64_t* set, int n, int c) {  // once a warp, after all its lanes
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&set[c % n]));
+  };
+
+  if (warp == 12) {
+    // ------------------------------------------------------------ loads
+    if (elect_one()) {
+      bool ok = true;
+#pragma unroll 1
+      for (int c = 0; c < live && ok; c++) {
+        const uint32_t st = smem + (c % L::STAGES) * L::STAGE, bar = smem_u32(&bars.full[c % L::STAGES]);
+        if (c >= L::STAGES && !(ok = wait(bars.empty, L::STAGES, c - L::STAGES, 11))) break;
+        mbar_arrive_expect_tx(bar, L::STAGE);  // boxes count in full, past the tensor's end too
+        auto tile = [&](uint32_t dst, const CUtensorMap* map, const Operand& o, int d0) {
+          tma_load_4d(dst, map, d0, p0 + at(c), (head / o.per) * o.hs, batch * o.bs, bar);
+        };
+#pragma unroll 1
+        for (int s = 0; s < NS; s++) {
+          if (OUT) tile(st + L::A + s * TILE, &maps.a, r.a, s * 64);
+          tile(st + L::B + s * TILE, &maps.b, r.b, s * 64);
+        }
+        tile(st + L::C, &maps.c, r.c, blk * 64);
+      }
+      // the copies in flight end before the CTA does
+      for (int c = max(0, live - L::STAGES); !ok && c < live; c++)
+        mbar_wait_drain(smem_u32(&bars.full[c % L::STAGES]), (uint32_t)(c / L::STAGES) & 1);
+    }
+  } else if (warp >= 8 && warp < 12) {
+    // ------------------------------------------------------------ state
+    const int t = tid - 8 * 32;            // TMEM lane: column t % 64 of c, half t / 64 of the rows of b
+    const int ec = blk * 64 + (t & 63), half = t >> 6;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    constexpr int W = 32 * NS;             // state elements of a thread
+    const long long bh = (long long)batch * r.heads + head;
+    const float lam = pw[1];
+    float E[W];
+    {
+      const float* src = nullptr;
+      long long step = 0;
+      int rows = 0;  // of this thread's state rows, how many are read
+      float f = 1.f;
+      if (OUT && r.staged) {
+        src = r.seg + ((bh * r.nseg + slot) * (NS * 64) + half * W) * (r.blocks * 64) + ec;
+        step = r.blocks * 64;
+        rows = W;
+      } else if (OUT && r.init && ec < r.dc) {
+        src = r.init + bh * r.da * r.dc + half * W * r.ir + ec * r.ic;
+        step = r.ir;
+        rows = r.da - half * W;
+        if (!REV) f = lam;
+      }
+#pragma unroll
+      for (int i = 0; i < W; i++, src += step) E[i] = i < rows ? f * *src : 0.f;
+    }
+    bool ok = true;
+    auto take = [&](int c) {  // E: the state after chunk c, and unless it is the last one decayed to the next
+      if (!wait(bars.u, L::KB, c, 12)) return false;
+      tc_fence_after();
+      const float d = pw[num(c) - 1], f = c + 1 < live ? lam : 1.f;
+      const float fe = f * d, fu = f * r.update;
+#pragma unroll
+      for (int i = 0; i < W; i += 32) {
+        float u[32];
+        tmem_ld32(tmem + L::T_U + (c % L::KB) * (64 * NS) + lane_base + half * W + i, u);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j++) E[i + j] = fe * E[i + j] + fu * u[j];
+      }
+      tc_fence_before();
+      return true;
+    };
+    for (int c = 0; c < live && ok; c++) {
+      if (!(ok = __all_sync(~0u, wait(bars.full, L::STAGES, c, 13)))) break;
+      if (L::KB == 1 && c > 0 && !(ok = __all_sync(~0u, take(c - 1)))) break;
+      const uint32_t src = smem + (c % L::STAGES) * L::STAGE + L::B, dst = smem + L::BD + (c % L::KB) * L::BD_BUF;
+      const int n = num(c), ck = t & 7;
+      if (r.lengths && n < CH) {  // the box holds tokens past the sequence's end
+        const uint32_t stage = smem + (c % L::STAGES) * L::STAGE;
+        for (uint32_t i = t; i < L::STAGE / 16; i += 128)
+          if ((int)((i >> 3) & 127) >= n) sts16(stage + i * 16, make_uint4(0, 0, 0, 0));
+      }
+#pragma unroll 1
+      for (int s = 0; s < NS; s++)
+#pragma unroll(UP == 1 ? 4 : 2)
+        for (int i = 0; i < 8; i++) {
+          const int j = (t >> 3) + 16 * i;
+          const uint32_t off = swz(j, ck);
+          uint4 x = lds16(src + s * TILE + off);
+          if (j >= n) x = make_uint4(0, 0, 0, 0);
+          const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&x);
+          const float w = pw[REV ? j : max(n - 1 - j, 0)];
+          float v[8];
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            v[2 * q] = __low2float(e[q]) * w;
+            v[2 * q + 1] = __high2float(e[q]) * w;
+          }
+          uint4 parts[UP];
+          split8<UP>(v, parts);
+#pragma unroll
+          for (int p = 0; p < UP; p++) sts16(dst + (p * NS + s) * TILE + off, parts[p]);
+        }
+      fence_async_smem();
+      arrive(bars.bd, L::KB, c);
+      if (L::KB == 2 && c > 0 && !(ok = __all_sync(~0u, take(c - 1)))) break;
+      if (OUT) {
+        // E's buffer is free once the products of chunk c - ES are done
+        if (c >= L::ES && !(ok = __all_sync(~0u, wait(bars.s, 2, c - L::ES, 14)))) break;
+        const uint32_t eb = smem + L::E + (c % L::ES) * L::E_BUF;
+#pragma unroll
+        for (int i = 0; i < W; i += 8) {
+          uint4 parts[2];
+          split8<2>(E + i, parts);
+          const int er = half * W + i;
+#pragma unroll
+          for (int p = 0; p < 2; p++) sts16(eb + (p * NS + (er >> 6)) * ETILE + swz(t & 63, (er & 63) >> 3), parts[p]);
+        }
+        fence_async_smem();
+        arrive(bars.e, L::ES, c);
+      }
+    }
+    if (ok && live) ok = take(live - 1);
+    if (ok && !OUT) {
+      float* dst = r.seg + ((bh * r.nseg + slot) * (NS * 64) + half * W) * (r.blocks * 64) + ec;
+#pragma unroll
+      for (int i = 0; i < W; i++, dst += r.blocks * 64) *dst = E[i];
+    }
+  } else if (warp == 13) {
+    // ------------------------------------------------------------ MMAs
+    // The whole warp walks the loop and one elected lane issues: in a branch
+    // on the lane number the compiler takes 88 clocks an MMA, elected 51 (what
+    // 128 x 64 x 16 from shared memory takes).
+    const bool leader = elect_one();
+    constexpr uint32_t ID_U = idesc_bf16_f32(64 * NS) | A_MN | B_MN, ID_S = idesc_bf16_f32(128),
+                       ID_E = idesc_bf16_f32(64), ID_P = idesc_bf16_f32(64) | B_MN;
+    bool ok = true;
+    auto ready = [&](uint64_t* set, int n, int c, int code) {
+      ok = __all_sync(~0u, wait(set, n, c, code));
+      tc_fence_after();
+      return ok;
+    };
+    auto second = [&](int c) {  // O += P c of chunk c; its stage is free afterwards
+      if (!ready(bars.p, 2, c, 15)) return;
+      if (leader) {
+        const uint32_t t = tmem + (c & 1) * 192;
+        const uint64_t dc = desc_mn(smem + (c % L::STAGES) * L::STAGE + L::C, 0);
+#pragma unroll 4
+        for (int k = 0; k < 8; k++) mma_ta(t + 128, t + 8 * k, dc + ((2048 * k) >> 4), ID_P, 1);
+        mma_commit(smem_u32(&bars.o[c & 1]));
+        mma_commit(smem_u32(&bars.empty[c % L::STAGES]));
+      }
+      __syncwarp();
+    };
+#pragma unroll 1
+    for (int c = 0; c < live; c++) {
+      const uint32_t st = smem + (c % L::STAGES) * L::STAGE;
+      if (!ready(bars.bd, L::KB, c, 16)) break;  // b~ is made from a full stage
+      if (leader) {
+        const uint32_t tu = tmem + L::T_U + (c % L::KB) * (64 * NS);
+        const uint64_t dc = desc_mn(st + L::C, 0);  // 64 columns, read twice to fill the MMA's 128 rows
+#pragma unroll 1
+        for (int p = UP - 1; p >= 0; p--) {
+          const uint64_t db = desc_mn(smem + L::BD + (c % L::KB) * L::BD_BUF + p * NS * TILE, TILE);
+#pragma unroll 4
+          for (int k = 0; k < 8; k++)
+            mma_bf16(tu, dc + ((2048 * k) >> 4), db + ((2048 * k) >> 4), ID_U, p < UP - 1 || k > 0);
+        }
+        mma_commit(smem_u32(&bars.u[c % L::KB]));
+        if (!OUT) mma_commit(smem_u32(&bars.empty[c % L::STAGES]));
+      }
+      __syncwarp();
+      if (!OUT) continue;
+      // S and O of this chunk: the group has read O of chunk c - 2, and P c of that chunk was issued before
+      if (c >= 2 && !ready(bars.oe, 2, c - 2, 17)) break;
+      const uint32_t t = tmem + (c & 1) * 192;
+      if (leader) {
+#pragma unroll 1
+        for (int s = 0; s < NS; s++) {
+          const uint64_t da = smem_desc(st + L::A + s * TILE, 1024, 2), db = smem_desc(st + L::B + s * TILE, 1024, 2);
+#pragma unroll
+          for (int k = 0; k < 4; k++) mma_bf16(t, da + 2 * k, db + 2 * k, ID_S, s > 0 || k > 0);
+        }
+      }
+      __syncwarp();
+      if (!ready(bars.e, L::ES, c, 18)) break;
+      if (leader) {
+#pragma unroll 1
+        for (int i = 2 * NS - 1; i >= 0; i--) {  // the small part of E first
+          const uint64_t da = smem_desc(st + L::A + (i % NS) * TILE, 1024, 2),
+                         de = smem_desc(smem + L::E + (c % L::ES) * L::E_BUF + i * ETILE, 1024, 2);
+#pragma unroll
+          for (int k = 0; k < 4; k++) mma_bf16(t + 128, da + 2 * k, de + 2 * k, ID_E, i < 2 * NS - 1 || k > 0);
+        }
+        mma_commit(smem_u32(&bars.s[c & 1]));
+      }
+      __syncwarp();
+      if (c > 0) second(c - 1);
+      if (!ok) break;
+    }
+    if (OUT && ok && live) second(live - 1);
+    // leave only when every product issued has completed
+    __shared__ uint64_t drain;
+    if (leader) {
+      mbar_init(smem_u32(&drain), 1);
+      fence_mbar_init();
+      mma_commit(smem_u32(&drain));
+      mbar_wait_drain(smem_u32(&drain), 0);
+    }
+  } else if (OUT && warp < 8) {
+    // ------------------------------------------------------------ scores and outputs
+    const int grp = warp >> 2, rb = warp & 3, row = rb * 32 + lane;
+    const uint32_t t = tmem + grp * 192 + ((uint32_t)(rb * 32) << 16);
+    const long long hb = batch * r.ob + head * r.oh + blk * 64;
+    const int width = min(64, r.dc - blk * 64);
+    bool ok = true;
+    for (int c = grp; c < live; c += 2) {
+      if (!(ok = __all_sync(~0u, wait(bars.s, 2, c, 19)))) break;
+      tc_fence_after();
+      const int n = num(c);
+#pragma unroll 1
+      for (int b = 0; b < 4; b++) {
+        uint32_t w[16];
+        if (REV ? b < rb : b > rb) {
+#pragma unroll
+          for (int i = 0; i < 16; i++) w[i] = 0;
+        } else {
+          float v[32];
+          tmem_ld32(t + b * 32, v);
+          tmem_wait_ld();
+          if (b == rb) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              const int d = REV ? j - lane : lane - j;
+              v[j] = d >= 0 ? v[j] * (r.intra * pw[max(d, 0)]) : 0.f;
+            }
+          } else {
+            const float base = r.intra * pw[REV ? b * 32 - row : row - b * 32 - 31];
+            const float4* f = reinterpret_cast<const float4*>(REV ? pw : rv);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              const float4 x = f[j];
+              v[4 * j] *= base * x.x;
+              v[4 * j + 1] *= base * x.y;
+              v[4 * j + 2] *= base * x.z;
+              v[4 * j + 3] *= base * x.w;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 16; i++) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+        }
+        tmem_st16(t + b * 16, w);  // over columns already read
+      }
+      const int dist = REV ? n - 1 - row : row;
+      const float di = dist >= 0 ? r.inter * pw[dist] : 0.f;
+#pragma unroll 1
+      for (int h = 0; h < 2; h++) {
+        float v[32];
+        tmem_ld32(t + 128 + h * 32, v);
+        tmem_wait_ld();
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) w[i] = __float_as_uint(v[i] * di);
+        tmem_st16(t + 128 + h * 32, w);
+        tmem_st16(t + 144 + h * 32, w + 16);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      arrive(bars.p, 2, c);
+      if (!(ok = __all_sync(~0u, wait(bars.o, 2, c, 20)))) break;
+      tc_fence_after();
+      const int tok = p0 + at(c) + row;
+      const long long dst = hb + (long long)tok * r.ot;
+#pragma unroll 1
+      for (int h = 0; h < 2; h++) {
+        float v[32];
+        tmem_ld32(t + 128 + h * 32, v);
+        tmem_wait_ld();
+        if (h == 1) {
+          tc_fence_before();
+          arrive(bars.oe, 2, c);
+        }
+        if (tok < r.tokens) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            const int col = h * 32 + i;
+            if (col >= width) break;
+            if (row >= n)
+#pragma unroll
+              for (int j = 0; j < 8; j++) v[i + j] = 0.f;
+            if (r.out_f32)
+              store_vec<float, 8>(static_cast<float*>(r.out) + dst + col, v + i);
+            else
+              store_vec<T, 8>(static_cast<T*>(r.out) + dst + col, v + i);
+          }
+        }
+      }
+    }
+    // tokens past the sequence's end
+    const int end = min(p0 + seg_tokens, r.tokens);
+    for (int i = tid; i < (end - p0 - live * CH) * 64; i += 256) {
+      const int c = i & 63;
+      if (c >= width) continue;
+      const long long dst = hb + (long long)(p0 + live * CH + (i >> 6)) * r.ot + c;
+      if (r.out_f32)
+        static_cast<float*>(r.out)[dst] = 0.f;
+      else
+        static_cast<T*>(r.out)[dst] = from_float<T>(0.f);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (tid == 0 && failed) atomicCAS(r.status, 0, failed);
+  if (warp == 0) {
+    tmem_relinquish();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int NS, bool OUT, bool REV>
+cudaError_t launch(const Run& r, const Maps& maps, int segs, cudaStream_t st) {
+  constexpr int bytes = Lay<NS, OUT>::BYTES + 1024;
+  static_assert(bytes + 2048 <= 227 * 1024, "shared memory");
+  const cudaError_t ce =
+      cudaFuncSetAttribute(k_pipe<NS, OUT, REV>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (ce != cudaSuccess) return ce;
+  const long long grid = (long long)r.batch * r.heads * r.blocks * segs;
+  k_pipe<NS, OUT, REV><<<(unsigned)grid, THREADS, bytes, st>>>(r, maps, segs);
+  return cudaGetLastError();
+}
+
+template <int NS, bool REV>
+cudaError_t launch(const Run& r, const Maps& m, bool states, cudaStream_t st) {
+  if (states)  // the last segment's state is needed only where the final state is
+    return launch<NS, false, REV>(r, m, r.fin ? r.nseg : r.nseg - 1, st);
+  return launch<NS, true, REV>(r, m, r.nseg, st);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess) {
+      cudaGetLastError();
+      p = nullptr;
+    }
+    return (PFN_cuTensorMapEncodeTiled_v12000)p;
+  }();
+  return fn;
+}
+
+// [batch][heads][tokens][d] in boxes of 128 tokens x 64 columns.  A dimension
+// with stride 0 has one element (its coordinate is multiplied by hs or bs = 0).
+bool encode(CUtensorMap* m, Operand& o, const Run& r, int d) {
+  const cuuint64_t heads = (cuuint64_t)(r.heads / o.per);
+  o.hs = o.sh != 0, o.bs = o.sb != 0;
+  if (!encode_fn() || o.st <= 0 || o.sh < 0 || o.sb < 0) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)r.tokens, o.hs ? heads : 1, o.bs ? (cuuint64_t)r.batch : 1};
+  const cuuint64_t row = (cuuint64_t)o.st * 2;
+  const cuuint64_t strides[3] = {row, o.hs ? (cuuint64_t)o.sh * 2 : row, o.bs ? (cuuint64_t)o.sb * 2 : row};
+  for (cuuint64_t s : strides)
+    if (s >> 40) return false;
+  const cuuint32_t box[4] = {64, CH, 1, 1}, one[4] = {1, 1, 1, 1};
+  return encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(o.p), dims, strides, box, one,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+bool encode_maps(Run& r, Maps& m) {
+  return encode(&m.a, r.a, r, r.da) && encode(&m.b, r.b, r, r.da) && encode(&m.c, r.c, r, r.dc);
+}
+
+cudaError_t launch_pipe(const Run& r, const Maps& m, bool states, cudaStream_t st) {
+  if (r.slabs == 1) return r.reverse ? launch<1, true>(r, m, states, st) : launch<1, false>(r, m, states, st);
+  return r.reverse ? launch<2, true>(r, m, states, st) : launch<2, false>(r, m, states, st);
+}
+
+}  // namespace ops
+}  // namespace lama

@@ -33,9 +33,9 @@
 // have, the entering state to two (three for fp32 inputs).  For bf16 inputs the
 // scores' one rounding is of the size of the output's own.
 #include <algorithm>
+#include <type_traits>
 
-#include "operators.cuh"
-#include "ptx.cuh"
+#include "attention.cuh"
 
 namespace lama {
 namespace ops {
@@ -44,47 +44,7 @@ namespace {
 
 __device__ int g_status;
 
-constexpr int CH = 128;         // tokens of a chunk (the MMA's M)
 constexpr int THREADS = 256;
-constexpr uint32_t TILE = 128 * 128;  // bytes of 128 rows x 64 bf16, 128-byte swizzle
-constexpr uint32_t ETILE = 64 * 128;  // 64 rows x 64 bf16
-
-// One operand: element (token, d) of the head's row at
-// p + batch * sb + token * st + head * sh + d.
-struct Operand {
-  const void* p;
-  long long sb, st, sh;
-  int per;  // heads of the run that share one head of the operand
-  int vec;  // rows are 16-byte aligned and a multiple of 16 bytes long
-};
-
-struct Run {
-  Operand a, b, c;
-  void* out;  // element (token, d) of head h at out + batch * ob + token * ot + h * oh + d
-  long long ob, ot, oh;
-  int out_f32;  // out is fp32 whatever the inputs are
-  int out_vec;
-  const float* log_decay;
-  const int* lengths;
-  const float* init;  // [batch][heads] of [da][dc], element (r, c) at r * ir + c * ic
-  float* fin;
-  long long ir, ic, fr, fc;
-  float* seg;  // [batch*heads][nseg][slabs*64][blocks*64]: states of the segments
-  int* status;
-  float inter, intra, update;  // scales of a E, of the scores, of b c^T
-  int batch, tokens, heads, da, dc;
-  int reverse;     // walk backwards in time; the initial state is not decayed, the final one is
-  int nseg, chunks;  // segments of a sequence, chunks of a segment
-  int blocks;      // 64-column blocks of c
-  int slabs;       // 64-column slabs of a and b
-};
-
-__device__ __forceinline__ float power(float g, int n) { return n == 0 ? 1.f : expf(g * (float)n); }
-
-__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t lbo) {
-  // MN-major, 128-byte swizzle: 64-element blocks `lbo` bytes apart, groups of 8 k-rows 1024 apart
-  return smem_desc(saddr, 1024, 2) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16);
-}
 
 template <class T>
 struct Parts {
@@ -98,38 +58,6 @@ template <>
 struct Parts<float> {
   static constexpr int N = 3;
 };
-
-// v[0..7] into N bf16 parts of 16 bytes each (part p holds what parts 0..p-1 left over)
-template <int N>
-__device__ __forceinline__ void split8(const float* v, uint4* out) {
-  float r[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) r[i] = v[i];
-#pragma unroll
-  for (int p = 0; p < N; p++) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(r[2 * i], r[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      if (p + 1 < N) {
-        r[2 * i] -= __low2float(h);
-        r[2 * i + 1] -= __high2float(h);
-      }
-    }
-    out[p] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
-__device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-__device__ __forceinline__ uint4 lds16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t swz(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
 
 // 64 columns from d0 of the chunk's rows, as parts, zeros past the sequence
 // and past the head's size.  Row r of the chunk is token first + r * step.
@@ -189,8 +117,6 @@ __device__ __forceinline__ void mma_parts(uint32_t d, uint64_t a, uint64_t b, ui
       }
     }
 }
-
-constexpr uint32_t A_MN = 1u << 15, B_MN = 1u << 16;
 
 template <class T>
 struct Plan {
@@ -260,7 +186,7 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
       float v = 0.f;
       const int er = s * 64 + srow, ec = blk * 64 + scol + i;
       if (OUT && s < r.slabs) {
-        if (r.nseg > 1) {
+        if (r.staged) {
           v = r.seg[(((long long)(batch * r.heads + head) * r.nseg + seg) * (r.slabs * 64) + er) * ld + ec];
         } else if (r.init && er < r.da && ec < r.dc) {
           v = r.init[(long long)(batch * r.heads + head) * r.da * r.dc + er * r.ir + ec * r.ic];
@@ -436,24 +362,12 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
       if (row < n) {
         const long long at = batch * r.ob + (first + (long long)row * step) * r.ot + head * r.oh;
         const int c0 = blk * 64 + col0;
-        if (r.out_f32) {
-          float* dst = static_cast<float*>(r.out) + at + c0;
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            if (r.out_vec && c0 + i + 8 <= r.dc)
-              store_vec<float, 8>(dst + i, x + i);
-            else
-              for (int j = 0; j < 8; j++)
-                if (c0 + i + j < r.dc) dst[i + j] = x[i + j];
-        } else {
-          T* dst = static_cast<T*>(r.out) + at + c0;
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            if (r.out_vec && c0 + i + 8 <= r.dc)
-              store_vec<T, 8>(dst + i, x + i);
-            else
-              for (int j = 0; j < 8; j++)
-                if (c0 + i + j < r.dc) dst[i + j] = from_float<T>(x[i + j]);
+        for (int i = 0; i < 32; i += 8) {
+          if (r.out_f32)
+            store_row(static_cast<float*>(r.out) + at + c0 + i, x + i, r.dc - c0 - i, r.out_vec);
+          else
+            store_row(static_cast<T*>(r.out) + at + c0 + i, x + i, r.dc - c0 - i, r.out_vec);
         }
       }
     }
@@ -500,7 +414,9 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
   }
 }
 
-// seg[s]: the state segment s adds -> the state that enters it.
+// seg[s]: the state segment s adds -> the state that enters it (segments in
+// the order of the recurrence).  The pipelined kernel leaves the final state
+// to this kernel.
 __global__ void k_scan(const __grid_constant__ Run r) {
   const int rows = r.slabs * 64, cols = r.blocks * 64;
   const long long per = (long long)rows * cols;
@@ -508,23 +424,31 @@ __global__ void k_scan(const __grid_constant__ Run r) {
   if (i >= per) return;
   const int bh = blockIdx.y, head = bh % r.heads, batch = bh / r.heads;
   const int er = (int)(i / cols), ec = (int)(i % cols);
+  const bool inside = er < r.da && ec < r.dc;
   const float g = r.log_decay[head];
   int len = r.tokens;
   if (r.lengths) len = min(max(r.lengths[batch], 0), r.tokens);
   const float lam = power(g, 1);
-  float e = 0.f;
-  if (r.init && er < r.da && ec < r.dc) {
-    e = r.init[(long long)bh * r.da * r.dc + er * r.ir + ec * r.ic];
+  const long long base = (long long)bh * r.da * r.dc;
+  float e = 0.f, after = 0.f;  // the state that enters a segment, and the one after the last token
+  if (r.init && inside) {
+    e = after = r.init[base + er * r.ir + ec * r.ic];
     if (!r.reverse) e *= lam;
   }
   float* p = r.seg + (long long)bh * r.nseg * per + i;
   const int seg_tokens = r.chunks * CH;
   for (int s = 0; s < r.nseg; s++) {
-    const int n = min(max(len - s * seg_tokens, 0), seg_tokens);
-    const float x = s + 1 < r.nseg ? p[s * per] : 0.f;
+    const int seg = r.pipe && r.reverse ? r.nseg - 1 - s : s;
+    const int n = min(max(len - seg * seg_tokens, 0), seg_tokens);
+    const float x = r.pipe && r.fin || s + 1 < r.nseg ? p[s * per] : 0.f;
     p[s * per] = e;
-    if (n > 0) e = lam * x + power(g, n) * e;
+    if (n > 0) {
+      after = x + power(g, n - 1) * e;
+      e = lam * after;
+      if (r.reverse) after = e;
+    }
   }
+  if (r.pipe && r.fin && inside) r.fin[base + er * r.fr + ec * r.fc] = after;
 }
 
 // Sum over the heads that share one head of the operand: src fp32
@@ -577,25 +501,36 @@ void cut(Run& r) {
     if (c == 1) break;
     c = std::max(1, std::min(c - 1, (chunks + nseg) / (nseg + 1)));
   }
+  r.staged = r.nseg > 1;
 }
 
-long long seg_floats(const Run& r) {
-  return r.nseg > 1 ? (long long)r.batch * r.heads * r.nseg * r.slabs * 64 * r.blocks * 64 : 0;
+// Room for the segments' states of a run, whatever its alignment turns out to
+// be and whether or not the final state is asked for.
+long long seg_bytes(const lama_attention* p, int da, int dc) {
+  Run r{};
+  r.batch = p->batch, r.heads = p->heads, r.tokens = p->tokens;
+  r.slabs = (da + 63) / 64, r.blocks = (dc + 63) / 64;
+  cut(r);
+  if (!r.staged && p->dtype != LAMA_BF16) return 0;
+  return (long long)r.batch * r.heads * r.nseg * r.slabs * 64 * r.blocks * 64 * 4;
 }
 
 template <class T>
-cudaError_t go(const Run& r, cudaStream_t st) {
+cudaError_t go(Run& r, cudaStream_t st) {
   cudaError_t ce = cudaSuccess;
-  if (r.nseg > 1) {
-    if ((ce = launch_chunks<T, false>(r, st)) != cudaSuccess) return ce;
+  Maps maps;
+  r.pipe = std::is_same_v<T, __nv_bfloat16> && r.a.vec && r.b.vec && r.c.vec && r.out_vec && encode_maps(r, maps);
+  if (r.pipe && r.fin) r.staged = 1;
+  if (r.staged) {
+    if ((ce = r.pipe ? launch_pipe(r, maps, true, st) : launch_chunks<T, false>(r, st)) != cudaSuccess) return ce;
     const int per = r.slabs * 64 * r.blocks * 64;
     k_scan<<<dim3((per + 255) / 256, r.batch * r.heads), 256, 0, st>>>(r);
     if ((ce = cudaGetLastError()) != cudaSuccess) return ce;
   }
-  return launch_chunks<T, true>(r, st);
+  return r.pipe ? launch_pipe(r, maps, false, st) : launch_chunks<T, true>(r, st);
 }
 
-cudaError_t go(const Run& r, int dtype, cudaStream_t st) {
+cudaError_t go(Run& r, int dtype, cudaStream_t st) {
   return dtype == LAMA_F32 ? go<float>(r, st) : dtype == LAMA_F16 ? go<__half>(r, st) : go<__nv_bfloat16>(r, st);
 }
 
@@ -677,10 +612,11 @@ Run common(const lama_attention* p) {
   return r;
 }
 
-Run forward_run(const lama_attention* p) {
+Run forward_run(const lama_attention* p, float* final_state) {
   Run r = common(p);
   roles(r, operand(p->q, p->heads, p->dk, p->dtype), operand(p->k, p->heads, p->dk, p->dtype),
         operand(p->v, p->heads, p->dv, p->dtype), p->dk, p->dv);
+  r.fin = final_state;
   r.inter = r.intra = p->scale;
   r.update = 1.f;
   r.init = p->initial_state;
@@ -700,10 +636,12 @@ Run gradient_run(const lama_attention* p, const lama_attention_grads* g, int whi
     r.update = 1.f;
     r.init = p->initial_state;
   } else {
-    if (which == 1)
+    if (which == 1) {
       roles(r, v, d, q, p->dv, p->dk);
-    else
+    } else {
       roles(r, k, q, d, p->dk, p->dv);
+      r.fin = g->grad_initial_state;
+    }
     r.inter = 1.f;
     r.intra = r.update = p->scale;
     r.reverse = 1;
@@ -730,12 +668,9 @@ extern "C" long long lama_linear_attention_workspace(const lama_attention* p, in
   if (err && err_len > 0) err[0] = 0;
   const int rc = check(p, err, err_len);
   if (rc != LAMA_OK) return rc;
-  if (!backward) return up(seg_floats(forward_run(p)) * 4);
-  lama_attention_grads g{};
-  g.grad_out = p->v;
-  g.grad_out.heads = p->heads;
-  long long seg = 0, share = 0;
-  for (int w = 0; w < 3; w++) seg = std::max(seg, seg_floats(gradient_run(p, &g, w)) * 4);
+  if (!backward) return up(seg_bytes(p, p->dk, p->dv));
+  const long long seg = std::max(seg_bytes(p, p->dk, p->dv), seg_bytes(p, p->dv, p->dk));
+  long long share = 0;
   const int heads[3] = {p->q.heads, p->k.heads, p->v.heads}, d[3] = {p->dk, p->dk, p->dv};
   for (int w = 0; w < 3; w++)
     if (heads[w] != p->heads) share = std::max(share, (long long)p->batch * p->tokens * p->heads * d[w] * 4);
@@ -754,9 +689,8 @@ extern "C" int lama_linear_attention(const lama_attention* p, const lama_rows* o
     return fail(err, err_len, LAMA_EINVAL, "workspace of %lld bytes, %lld needed", workspace_bytes, need);
   DeviceGuard dev(device);
   cudaError_t ce = dev.status;
-  Run r = forward_run(p);
+  Run r = forward_run(p, final_state);
   output(r, *out, p->dv, p->dtype);
-  r.fin = final_state;
   r.seg = static_cast<float*>(workspace);
   if (ce == cudaSuccess) ce = status_word(&r.status);
   if (ce == cudaSuccess) ce = go(r, p->dtype, (cudaStream_t)stream);
@@ -786,8 +720,7 @@ extern "C" int lama_linear_attention_backward(const lama_attention* p, const lam
   int* status = nullptr;
   if (ce == cudaSuccess) ce = status_word(&status);
   const cudaStream_t st = (cudaStream_t)stream;
-  long long seg = 0;
-  for (int w = 0; w < 3; w++) seg = std::max(seg, seg_floats(gradient_run(p, g, w)) * 4);
+  const long long seg = std::max(seg_bytes(p, p->dk, p->dv), seg_bytes(p, p->dv, p->dk));
   float* shared = reinterpret_cast<float*>(static_cast<char*>(workspace) + up(seg));
   for (int w = 0; w < 3 && ce == cudaSuccess; w++) {
     Run r = gradient_run(p, g, w);
@@ -795,7 +728,6 @@ extern "C" int lama_linear_attention_backward(const lama_attention* p, const lam
     const int d = w == 2 ? p->dv : p->dk;
     r.seg = static_cast<float*>(workspace);
     r.status = status;
-    if (w == 2) r.fin = g->grad_initial_state;
     if (o.heads == p->heads) {
       output(r, o, d, p->dtype);
       ce = go(r, p->dtype, st);

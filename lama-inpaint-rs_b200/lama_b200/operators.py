@@ -88,8 +88,17 @@ def check_operators(device=None) -> None:
 # ------------------------------------------------------------------ linear attention
 
 def _unit(t):
-    """The tensor itself if its last dimension is contiguous, else a copy."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """The tensor itself where the kernels take its strides at full speed, else a contiguous copy: rows have
+    to be contiguous, and bfloat16 rows of a multiple of 8 channels on 16-byte boundaries (the copy then
+    goes through the same kernel as a contiguous tensor, to the same bits)."""
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        return t.contiguous()
+    if t.dtype == torch.bfloat16 and t.shape[-1] % 8 == 0:
+        if t.dim() == 4 and t.shape[1] > 1 and t.stride(1) == 0:
+            return t.contiguous()
+        if t.data_ptr() % 16 or any(s % 8 and n > 1 for n, s in zip(t.shape[:-1], t.stride())):
+            return t.clone(memory_format=torch.contiguous_format)
+    return t
 
 
 def _rows(t):
