@@ -104,7 +104,7 @@ constexpr uint32_t A_MN = 1u << 15, B_MN = 1u << 16;
 // cannot address the operands.  `states`: only the states that the segments
 // add, into r.seg.
 struct Maps {
-  CUtensorMap a, b, c;
+  CUtensorMap a, b, c, o;
 };
 bool encode_maps(Run& r, Maps& m);
 cudaError_t launch_pipe(const Run& r, const Maps& m, bool states, cudaStream_t st);

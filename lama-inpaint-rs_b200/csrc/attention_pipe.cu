@@ -41,19 +41,21 @@ constexpr int THREADS = 14 * 32;  // 4 warps a scheduler at most: 128 registers 
 template <int NS, bool OUT>
 struct Lay {
   static constexpr int UP = OUT ? 1 : 3;  // parts of b~
-  static constexpr int STAGES = OUT ? (NS == 1 ? 3 : 2) : (NS == 1 ? 3 : 2);
-  static constexpr int KB = NS == 1 ? 2 : 1;  // buffers of b~ and of U
-  static constexpr int ES = NS == 1 ? 2 : 1;                                       // buffers of E
-  static constexpr uint32_t A = 0, B = OUT ? NS * TILE : 0, C = B + NS * TILE, STAGE = C + TILE;
-  static constexpr uint32_t BD = STAGES * STAGE, BD_BUF = UP * NS * TILE;
+  // stages of (a, b), free once S and a E are made, and of c, free after P c;
+  // buffers of b~ and of U, and of E
+  static constexpr int AS = OUT ? (NS == 1 ? 3 : 2) : (NS == 1 ? 4 : 2), CS = OUT ? (NS == 1 ? 4 : 2) : (NS == 1 ? 4 : 3);
+  static constexpr int KB = NS == 1 ? 2 : 1, ES = NS == 1 ? 2 : 1;
+  static constexpr uint32_t B = OUT ? NS * TILE : 0, AB = B + NS * TILE;  // a stage's b, its size
+  static constexpr uint32_t C = AS * AB, BD = C + CS * TILE, BD_BUF = UP * NS * TILE;
   static constexpr uint32_t E = BD + KB * BD_BUF, E_BUF = 2 * NS * ETILE;
   static constexpr uint32_t BYTES = E + (OUT ? ES * E_BUF : 0);
+  static constexpr int CONV = OUT ? 4 : 8;  // warps that make b~
   static constexpr uint32_t T_U = OUT ? 384 : 0;  // TMEM column of U; buffer i of S at 192 i, of O at 192 i + 128
   static_assert(T_U + KB * 64 * NS <= 512, "TMEM columns");
 };
 
 struct Bars {
-  uint64_t full[4], empty[4], bd[2], u[2], e[2], s[2], p[2], o[2], oe[2];
+  uint64_t full[4], empty[4], cfull[4], cempty[4], bd[2], u[2], e[2], s[2], p[2], o[2], oe[2];
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int c0, int c1, int c2, int c3, uint32_t bar) {
@@ -73,6 +75,17 @@ __device__ __forceinline__ bool elect_one() {
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(p));
   return p != 0;
+}
+
+// (x, y) *= (a, b), one instruction
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 p, q;\n\t"
+      "mov.b64 p, {%0, %1};\n\t"
+      "mov.b64 q, {%2, %3};\n\t"
+      "mul.rn.f32x2 p, p, q;\n\t"
+      "mov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
 }
 
 // A from TMEM (128 lanes, two 16-bit elements a column), B from shared memory
@@ -106,9 +119,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
                                                         const __grid_constant__ Maps maps, int segs) {
   using L = Lay<NS, OUT>;
   constexpr int UP = L::UP;
+  // Results leave through the stage that held c (one TMA store a chunk; per-row
+  // stores kept the load/store unit busy: 70 -> 59 us at 128 x 4096 tokens of
+  // 64).  With two slabs c has two stages only, and holding them longer costs
+  // more (195 -> 213 us): there the rows are stored directly.
+  constexpr bool STAGED_OUT = NS == 1;
   using T = __nv_bfloat16;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(16) float pw[CH + 4];
+  __shared__ float pi[CH];  // intra lam^i
   __shared__ __align__(16) float rv[32];  // lam^{31-j}
   __shared__ Bars bars;
   __shared__ uint32_t tmem_slot;
@@ -140,9 +159,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
     for (int i = 0; i < 4; i++) {
       mbar_init(smem_u32(&bars.full[i]), 1);
       mbar_init(smem_u32(&bars.empty[i]), 1);
+      mbar_init(smem_u32(&bars.cfull[i]), 1);
+      mbar_init(smem_u32(&bars.cempty[i]), 1);
     }
     for (int i = 0; i < 2; i++) {
-      mbar_init(smem_u32(&bars.bd[i]), 4);
+      mbar_init(smem_u32(&bars.bd[i]), L::CONV);
       mbar_init(smem_u32(&bars.u[i]), 1);
       mbar_init(smem_u32(&bars.e[i]), 4);
       mbar_init(smem_u32(&bars.s[i]), 1);
@@ -152,7 +173,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
     }
     fence_mbar_init();
   }
-  for (int i = tid; i <= CH; i += THREADS) pw[i] = power(g, i);
+  for (int i = tid; i <= CH; i += THREADS) {
+    pw[i] = power(g, i);
+    if (i < CH) pi[i] = r.intra * pw[i];
+  }
   for (int i = tid; i < 32; i += THREADS) rv[i] = power(g, 31 - i);
   tc_fence_before();
   __syncthreads();
@@ -169,28 +193,85 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
     if (lane == 0) mbar_arrive(smem_u32(&set[c % n]));
   };
 
+  auto wait_stage = [&](int c) {  // b, and c where its rows may have to be cleared
+    return wait(bars.full, L::AS, c, 13) && (!r.lengths || wait(bars.cfull, L::CS, c, 22));
+  };
+  // b~ of chunk c by the CONV warps, t their thread: row j times lam to the chunk's end, UP parts
+  auto make_bd = [&](int c, int t) {
+    constexpr int TH = L::CONV * 32;
+    const uint32_t ab = smem + (c % L::AS) * L::AB, ct = smem + L::C + (c % L::CS) * TILE;
+    const uint32_t src = ab + L::B, dst = smem + L::BD + (c % L::KB) * L::BD_BUF;
+    const int n = num(c), ck = t & 7;
+    if (r.lengths && n < CH) {  // the boxes hold tokens past the sequence's end
+#pragma unroll 1
+      for (uint32_t i = t; i < (L::AB + TILE) / 16; i += TH)
+        if ((int)((i >> 3) & 127) >= n) sts16(i < L::AB / 16 ? ab + i * 16 : ct + (i - L::AB / 16) * 16, make_uint4(0, 0, 0, 0));
+    }
+    // a batch's loads go out before its first use: loads and stores of shared memory stay in program order
+    constexpr int BATCH = UP == 1 ? 8 : 4;
+#pragma unroll 1
+    for (int i0 = 0; i0 < NS * CH * 8 / TH; i0 += BATCH) {
+      uint4 x[BATCH];
+      float w[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; i++) {
+        const int k = (i0 + i) * (TH / 8) + (t >> 3), j = k & (CH - 1);  // the slabs' rows one after another
+        x[i] = lds16(src + (k >> 7) * TILE + swz(j, ck));
+        w[i] = pw[REV ? j : max(n - 1 - j, 0)];
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; i++) {
+        const int k = (i0 + i) * (TH / 8) + (t >> 3), j = k & (CH - 1);
+        if (j >= n) x[i] = make_uint4(0, 0, 0, 0);
+        const uint32_t* e = reinterpret_cast<const uint32_t*>(&x[i]);
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          v[2 * q] = __uint_as_float(e[q] << 16);  // bf16 is the upper half of an fp32
+          v[2 * q + 1] = __uint_as_float(e[q] & 0xffff0000u);
+          mul2(v[2 * q], v[2 * q + 1], w[i], w[i]);
+        }
+        uint4 parts[UP];
+        split8<UP>(v, parts);
+#pragma unroll
+        for (int p = 0; p < UP; p++) sts16(dst + (p * NS + (k >> 7)) * TILE + swz(j, ck), parts[p]);
+      }
+    }
+    fence_async_smem();
+    arrive(bars.bd, L::KB, c);
+  };
+
   if (warp == 12) {
     // ------------------------------------------------------------ loads
     if (elect_one()) {
       bool ok = true;
+      int issued = 0, cissued = 0;
 #pragma unroll 1
-      for (int c = 0; c < live && ok; c++) {
-        const uint32_t st = smem + (c % L::STAGES) * L::STAGE, bar = smem_u32(&bars.full[c % L::STAGES]);
-        if (c >= L::STAGES && !(ok = wait(bars.empty, L::STAGES, c - L::STAGES, 11))) break;
-        mbar_arrive_expect_tx(bar, L::STAGE);  // boxes count in full, past the tensor's end too
-        auto tile = [&](uint32_t dst, const CUtensorMap* map, const Operand& o, int d0) {
+      for (int c = 0; c < live; c++) {
+        auto tile = [&](uint32_t dst, const CUtensorMap* map, const Operand& o, int d0, uint32_t bar) {
           tma_load_4d(dst, map, d0, p0 + at(c), (head / o.per) * o.hs, batch * o.bs, bar);
         };
+        // boxes count in full, past the tensor's end too
+        if (c >= L::AS && !(ok = wait(bars.empty, L::AS, c - L::AS, 11))) break;
+        const uint32_t ab = smem + (c % L::AS) * L::AB, bar = smem_u32(&bars.full[c % L::AS]);
+        mbar_arrive_expect_tx(bar, L::AB);
 #pragma unroll 1
         for (int s = 0; s < NS; s++) {
-          if (OUT) tile(st + L::A + s * TILE, &maps.a, r.a, s * 64);
-          tile(st + L::B + s * TILE, &maps.b, r.b, s * 64);
+          if (OUT) tile(ab + s * TILE, &maps.a, r.a, s * 64, bar);
+          tile(ab + L::B + s * TILE, &maps.b, r.b, s * 64, bar);
         }
-        tile(st + L::C, &maps.c, r.c, blk * 64);
+        issued = c + 1;
+        if (c >= L::CS && !(ok = wait(bars.cempty, L::CS, c - L::CS, 21))) break;
+        const uint32_t cbar = smem_u32(&bars.cfull[c % L::CS]);
+        mbar_arrive_expect_tx(cbar, TILE);
+        tile(smem + L::C + (c % L::CS) * TILE, &maps.c, r.c, blk * 64, cbar);
+        cissued = c + 1;
       }
-      // the copies in flight end before the CTA does
-      for (int c = max(0, live - L::STAGES); !ok && c < live; c++)
-        mbar_wait_drain(smem_u32(&bars.full[c % L::STAGES]), (uint32_t)(c / L::STAGES) & 1);
+      // after a wait that ran out, the copies in flight end before the CTA does
+      for (int c = max(0, issued - L::AS); !ok && c < issued; c++)
+        mbar_wait_drain(smem_u32(&bars.full[c % L::AS]), (uint32_t)(c / L::AS) & 1);
+      for (int c = max(0, cissued - L::CS); !ok && c < cissued; c++)
+        mbar_wait_drain(smem_u32(&bars.cfull[c % L::CS]), (uint32_t)(c / L::CS) & 1);
     }
   } else if (warp >= 8 && warp < 12) {
     // ------------------------------------------------------------ state
@@ -231,44 +312,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
         tmem_ld32(tmem + L::T_U + (c % L::KB) * (64 * NS) + lane_base + half * W + i, u);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; j++) E[i + j] = fe * E[i + j] + fu * u[j];
+        for (int j = 0; j < 32; j += 2) {
+          mul2(u[j], u[j + 1], fu, fu);
+          mul2(E[i + j], E[i + j + 1], fe, fe);
+          E[i + j] += u[j];
+          E[i + j + 1] += u[j + 1];
+        }
       }
       tc_fence_before();
+      if (!OUT) arrive(bars.e, L::KB, c);  // U's buffer is free
       return true;
     };
     for (int c = 0; c < live && ok; c++) {
-      if (!(ok = __all_sync(~0u, wait(bars.full, L::STAGES, c, 13)))) break;
+      if (OUT && !(ok = __all_sync(~0u, wait_stage(c)))) break;
       if (L::KB == 1 && c > 0 && !(ok = __all_sync(~0u, take(c - 1)))) break;
-      const uint32_t src = smem + (c % L::STAGES) * L::STAGE + L::B, dst = smem + L::BD + (c % L::KB) * L::BD_BUF;
-      const int n = num(c), ck = t & 7;
-      if (r.lengths && n < CH) {  // the box holds tokens past the sequence's end
-        const uint32_t stage = smem + (c % L::STAGES) * L::STAGE;
-        for (uint32_t i = t; i < L::STAGE / 16; i += 128)
-          if ((int)((i >> 3) & 127) >= n) sts16(stage + i * 16, make_uint4(0, 0, 0, 0));
-      }
-#pragma unroll 1
-      for (int s = 0; s < NS; s++)
-#pragma unroll(UP == 1 ? 4 : 2)
-        for (int i = 0; i < 8; i++) {
-          const int j = (t >> 3) + 16 * i;
-          const uint32_t off = swz(j, ck);
-          uint4 x = lds16(src + s * TILE + off);
-          if (j >= n) x = make_uint4(0, 0, 0, 0);
-          const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&x);
-          const float w = pw[REV ? j : max(n - 1 - j, 0)];
-          float v[8];
-#pragma unroll
-          for (int q = 0; q < 4; q++) {
-            v[2 * q] = __low2float(e[q]) * w;
-            v[2 * q + 1] = __high2float(e[q]) * w;
-          }
-          uint4 parts[UP];
-          split8<UP>(v, parts);
-#pragma unroll
-          for (int p = 0; p < UP; p++) sts16(dst + (p * NS + s) * TILE + off, parts[p]);
-        }
-      fence_async_smem();
-      arrive(bars.bd, L::KB, c);
+      if (OUT) make_bd(c, t);
       if (L::KB == 2 && c > 0 && !(ok = __all_sync(~0u, take(c - 1)))) break;
       if (OUT) {
         // E's buffer is free once the products of chunk c - ES are done
@@ -306,25 +364,27 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
       tc_fence_after();
       return ok;
     };
-    auto second = [&](int c) {  // O += P c of chunk c; its stage is free afterwards
+    auto second = [&](int c) {  // O += P c of chunk c
       if (!ready(bars.p, 2, c, 15)) return;
       if (leader) {
         const uint32_t t = tmem + (c & 1) * 192;
-        const uint64_t dc = desc_mn(smem + (c % L::STAGES) * L::STAGE + L::C, 0);
+        const uint64_t dc = desc_mn(smem + L::C + (c % L::CS) * TILE, 0);
 #pragma unroll 4
         for (int k = 0; k < 8; k++) mma_ta(t + 128, t + 8 * k, dc + ((2048 * k) >> 4), ID_P, 1);
         mma_commit(smem_u32(&bars.o[c & 1]));
-        mma_commit(smem_u32(&bars.empty[c % L::STAGES]));
+        if (!STAGED_OUT) mma_commit(smem_u32(&bars.cempty[c % L::CS]));
       }
       __syncwarp();
     };
 #pragma unroll 1
     for (int c = 0; c < live; c++) {
-      const uint32_t st = smem + (c % L::STAGES) * L::STAGE;
+      const uint32_t st = smem + (c % L::AS) * L::AB;
+      if (!ready(bars.cfull, L::CS, c, 23)) break;
       if (!ready(bars.bd, L::KB, c, 16)) break;  // b~ is made from a full stage
+      if (!OUT && c >= L::KB && !ready(bars.e, L::KB, c - L::KB, 25)) break;
       if (leader) {
         const uint32_t tu = tmem + L::T_U + (c % L::KB) * (64 * NS);
-        const uint64_t dc = desc_mn(st + L::C, 0);  // 64 columns, read twice to fill the MMA's 128 rows
+        const uint64_t dc = desc_mn(smem + L::C + (c % L::CS) * TILE, 0);  // 64 columns, read twice to fill the MMA's 128 rows
 #pragma unroll 1
         for (int p = UP - 1; p >= 0; p--) {
           const uint64_t db = desc_mn(smem + L::BD + (c % L::KB) * L::BD_BUF + p * NS * TILE, TILE);
@@ -333,7 +393,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
             mma_bf16(tu, dc + ((2048 * k) >> 4), db + ((2048 * k) >> 4), ID_U, p < UP - 1 || k > 0);
         }
         mma_commit(smem_u32(&bars.u[c % L::KB]));
-        if (!OUT) mma_commit(smem_u32(&bars.empty[c % L::STAGES]));
+        if (!OUT) {
+          mma_commit(smem_u32(&bars.empty[c % L::AS]));
+          mma_commit(smem_u32(&bars.cempty[c % L::CS]));
+        }
       }
       __syncwarp();
       if (!OUT) continue;
@@ -343,7 +406,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
       if (leader) {
 #pragma unroll 1
         for (int s = 0; s < NS; s++) {
-          const uint64_t da = smem_desc(st + L::A + s * TILE, 1024, 2), db = smem_desc(st + L::B + s * TILE, 1024, 2);
+          const uint64_t da = smem_desc(st + s * TILE, 1024, 2), db = smem_desc(st + L::B + s * TILE, 1024, 2);
 #pragma unroll
           for (int k = 0; k < 4; k++) mma_bf16(t, da + 2 * k, db + 2 * k, ID_S, s > 0 || k > 0);
         }
@@ -353,12 +416,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
       if (leader) {
 #pragma unroll 1
         for (int i = 2 * NS - 1; i >= 0; i--) {  // the small part of E first
-          const uint64_t da = smem_desc(st + L::A + (i % NS) * TILE, 1024, 2),
+          const uint64_t da = smem_desc(st + (i % NS) * TILE, 1024, 2),
                          de = smem_desc(smem + L::E + (c % L::ES) * L::E_BUF + i * ETILE, 1024, 2);
 #pragma unroll
           for (int k = 0; k < 4; k++) mma_bf16(t + 128, da + 2 * k, de + 2 * k, ID_E, i < 2 * NS - 1 || k > 0);
         }
         mma_commit(smem_u32(&bars.s[c & 1]));
+        mma_commit(smem_u32(&bars.empty[c % L::AS]));
       }
       __syncwarp();
       if (c > 0) second(c - 1);
@@ -373,6 +437,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
       mma_commit(smem_u32(&drain));
       mbar_wait_drain(smem_u32(&drain), 0);
     }
+  } else if (!OUT && warp < 8) {
+    // ------------------------------------------------------------ b~ of the kernel without outputs
+#pragma unroll 1
+    for (int c = 0; c < live; c++) {
+      if (!__all_sync(~0u, wait_stage(c))) break;
+      if (c >= L::KB && !__all_sync(~0u, wait(bars.u, L::KB, c - L::KB, 24))) break;
+      make_bd(c, tid);
+    }
   } else if (OUT && warp < 8) {
     // ------------------------------------------------------------ scores and outputs
     const int grp = warp >> 2, rb = warp & 3, row = rb * 32 + lane;
@@ -385,37 +457,47 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
       tc_fence_after();
       const int n = num(c);
 #pragma unroll 1
-      for (int b = 0; b < 4; b++) {
-        uint32_t w[16];
-        if (REV ? b < rb : b > rb) {
-#pragma unroll
-          for (int i = 0; i < 16; i++) w[i] = 0;
-        } else {
-          float v[32];
-          tmem_ld32(t + b * 32, v);
+      for (int h = 0; h < 2; h++) {
+        float v[64];
+        const bool some = REV ? 2 * h + 1 >= rb : 2 * h <= rb;
+        if (some) {
+          tmem_ld32(t + h * 64, v);
+          tmem_ld32(t + h * 64 + 32, v + 32);
           tmem_wait_ld();
+        }
+        uint32_t w[32];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const int b = 2 * h + k;
+          float* x = v + k * 32;
+          if (REV ? b < rb : b > rb) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) w[k * 16 + i] = 0;
+            continue;
+          }
           if (b == rb) {
 #pragma unroll
             for (int j = 0; j < 32; j++) {
               const int d = REV ? j - lane : lane - j;
-              v[j] = d >= 0 ? v[j] * (r.intra * pw[max(d, 0)]) : 0.f;
+              x[j] = d >= 0 ? x[j] * pi[max(d, 0)] : 0.f;
             }
           } else {
-            const float base = r.intra * pw[REV ? b * 32 - row : row - b * 32 - 31];
+            const float base = pi[REV ? b * 32 - row : row - b * 32 - 31];
             const float4* f = reinterpret_cast<const float4*>(REV ? pw : rv);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-              const float4 x = f[j];
-              v[4 * j] *= base * x.x;
-              v[4 * j + 1] *= base * x.y;
-              v[4 * j + 2] *= base * x.z;
-              v[4 * j + 3] *= base * x.w;
+              float4 y = f[j];
+              mul2(y.x, y.y, base, base);
+              mul2(y.z, y.w, base, base);
+              mul2(x[4 * j], x[4 * j + 1], y.x, y.y);
+              mul2(x[4 * j + 2], x[4 * j + 3], y.z, y.w);
             }
           }
 #pragma unroll
-          for (int i = 0; i < 16; i++) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+          for (int i = 0; i < 16; i++) w[k * 16 + i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
         }
-        tmem_st16(t + b * 16, w);  // over columns already read
+        tmem_st16(t + h * 32, w);  // over columns already read
+        tmem_st16(t + h * 32 + 16, w + 16);
       }
       const int dist = REV ? n - 1 - row : row;
       const float di = dist >= 0 ? r.inter * pw[dist] : 0.f;
@@ -426,7 +508,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
         tmem_wait_ld();
         uint32_t w[32];
 #pragma unroll
-        for (int i = 0; i < 32; i++) w[i] = __float_as_uint(v[i] * di);
+        for (int i = 0; i < 32; i += 2) {
+          mul2(v[i], v[i + 1], di, di);
+          w[i] = __float_as_uint(v[i]);
+          w[i + 1] = __float_as_uint(v[i + 1]);
+        }
         tmem_st16(t + 128 + h * 32, w);
         tmem_st16(t + 144 + h * 32, w + 16);
       }
@@ -436,7 +522,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
       if (!(ok = __all_sync(~0u, wait(bars.o, 2, c, 20)))) break;
       tc_fence_after();
       const int tok = p0 + at(c) + row;
-      const long long dst = hb + (long long)tok * r.ot;
+      // the tile of c has been read: the results take its place on their way out
+      const uint32_t ct = smem + L::C + (c % L::CS) * TILE;
 #pragma unroll 1
       for (int h = 0; h < 2; h++) {
         float v[32];
@@ -446,22 +533,44 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
           tc_fence_before();
           arrive(bars.oe, 2, c);
         }
-        if (tok < r.tokens) {
+        if (row >= n)
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            const int col = h * 32 + i;
-            if (col >= width) break;
-            if (row >= n)
+          for (int i = 0; i < 32; i++) v[i] = 0.f;
+        if (r.out_f32 || !STAGED_OUT) {
+          if (tok < r.tokens) {
+            const long long dst = hb + (long long)tok * r.ot + h * 32;
 #pragma unroll
-              for (int j = 0; j < 8; j++) v[i + j] = 0.f;
-            if (r.out_f32)
-              store_vec<float, 8>(static_cast<float*>(r.out) + dst + col, v + i);
-            else
-              store_vec<T, 8>(static_cast<T*>(r.out) + dst + col, v + i);
+            for (int i = 0; i < 32; i += 8) {
+              if (h * 32 + i >= width) break;
+              if (r.out_f32)
+                store_vec<float, 8>(static_cast<float*>(r.out) + dst + i, v + i);
+              else
+                store_vec<T, 8>(static_cast<T*>(r.out) + dst + i, v + i);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            uint4 x;
+            split8<1>(v + i * 8, &x);
+            sts16(ct + swz(row, h * 4 + i), x);
           }
         }
       }
+      if (!STAGED_OUT) continue;
+      if (!r.out_f32) fence_async_smem();
+      named_sync(1 + grp, 128);
+      if (rb == (REV ? 3 : 0) && lane == 0) {  // the warp with the fewest scores
+        if (!r.out_f32) {
+          tma_store_4d(&maps.o, ct, blk * 64, p0 + at(c), head, batch);
+          bulk_commit();
+          bulk_wait_read0();
+        }
+        mbar_arrive(smem_u32(&bars.cempty[c % L::CS]));
+      }
+      __syncwarp();
     }
+    bulk_wait0();
     // tokens past the sequence's end
     const int end = min(p0 + seg_tokens, r.tokens);
     for (int i = tid; i < (end - p0 - live * CH) * 64; i += 256) {
@@ -536,7 +645,11 @@ bool encode(CUtensorMap* m, Operand& o, const Run& r, int d) {
 }  // namespace
 
 bool encode_maps(Run& r, Maps& m) {
-  return encode(&m.a, r.a, r, r.da) && encode(&m.b, r.b, r, r.da) && encode(&m.c, r.c, r, r.dc);
+  if (!encode(&m.a, r.a, r, r.da) || !encode(&m.b, r.b, r, r.da) || !encode(&m.c, r.c, r, r.dc)) return false;
+  if (r.out_f32) return true;
+  Operand o{r.out, r.ob, r.ot, r.oh, 1, 1, 0, 0};
+  // a row of results has one place: no dimension may fold onto itself
+  return (r.oh != 0 || r.heads == 1) && (r.ob != 0 || r.batch == 1) && encode(&m.o, o, r, r.dc);
 }
 
 cudaError_t launch_pipe(const Run& r, const Maps& m, bool states, cudaStream_t st) {

@@ -437,15 +437,23 @@ __global__ void k_scan(const __grid_constant__ Run r) {
   }
   float* p = r.seg + (long long)bh * r.nseg * per + i;
   const int seg_tokens = r.chunks * CH;
-  for (int s = 0; s < r.nseg; s++) {
-    const int seg = r.pipe && r.reverse ? r.nseg - 1 - s : s;
-    const int n = min(max(len - seg * seg_tokens, 0), seg_tokens);
-    const float x = r.pipe && r.fin || s + 1 < r.nseg ? p[s * per] : 0.f;
-    p[s * per] = e;
-    if (n > 0) {
-      after = x + power(g, n - 1) * e;
-      e = lam * after;
-      if (r.reverse) after = e;
+  const int made = r.pipe && r.fin ? r.nseg : r.nseg - 1;  // segments whose states are there
+  for (int s0 = 0; s0 < r.nseg; s0 += 8) {
+    float x[8];  // loaded ahead: the stores below go to the same array
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = s0 + k < made ? p[(s0 + k) * per] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int s = s0 + k;
+      if (s >= r.nseg) break;
+      const int seg = r.pipe && r.reverse ? r.nseg - 1 - s : s;
+      const int n = min(max(len - seg * seg_tokens, 0), seg_tokens);
+      p[s * per] = e;
+      if (n > 0) {
+        after = x[k] + power(g, n - 1) * e;
+        e = lam * after;
+        if (r.reverse) after = e;
+      }
     }
   }
   if (r.pipe && r.fin && inside) r.fin[base + er * r.fr + ec * r.fc] = after;
@@ -481,9 +489,10 @@ cudaError_t launch_chunks(const Run& r, cudaStream_t st) {
 }
 
 // How a sequence is cut: one segment reads everything once, several read b
-// and c twice but fill the GPU.  Picks the least number of chunk steps on the
-// busiest SM, a state-only step counted as half a step and the two more
-// launches as two steps.
+// and c twice but fill the GPU.  Takes the least time on the busiest SM,
+// counted in chunk steps: a CTA costs 4 beside its chunks (set-up, the first
+// loads, the last products), the pass that makes the states about 0.6 a
+// chunk and, with the scan, two launches of about 3 each.
 void cut(Run& r) {
   const int slots = 148;
   const int chunks = (r.tokens + CH - 1) / CH;
@@ -492,7 +501,7 @@ void cut(Run& r) {
   for (int c = chunks;;) {
     const int nseg = (chunks + c - 1) / c;
     const double waves = (double)((rows * nseg + slots - 1) / slots);
-    const double cost = waves * c * (nseg > 1 ? 1.5 : 1.0) + (nseg > 1 ? 2.0 : 0.0);
+    const double cost = nseg == 1 ? waves * (c + 4) : waves * (1.6 * c + 8) + 6 + 0.05 * nseg;
     if (cost < best) {
       best = cost;
       r.nseg = nseg;
