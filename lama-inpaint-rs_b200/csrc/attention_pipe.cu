@@ -77,17 +77,6 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// (x, y) *= (a, b), one instruction
-__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {
-  asm("{\n\t.reg .b64 p, q;\n\t"
-      "mov.b64 p, {%0, %1};\n\t"
-      "mov.b64 q, {%2, %3};\n\t"
-      "mul.rn.f32x2 p, p, q;\n\t"
-      "mov.b64 {%0, %1}, p;\n\t}"
-      : "+f"(x), "+f"(y)
-      : "f"(a), "f"(b));
-}
-
 // A from TMEM (128 lanes, two 16-bit elements a column), B from shared memory
 __device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(

@@ -20,6 +20,9 @@ constexpr int GROUP8 = 128;
 
 // Codes (packed, 8 bytes) of this lane's 8 values and the group's scale; every
 // lane of the half-warp takes part.  Channels past the row's end hold zeros.
+// Integers up to 127 are rounded (half to even) and read off by adding
+// 1.5 * 2^23, whose last place is 1: the conversion instructions run at a
+// sixteenth of the rate.
 __device__ __forceinline__ uint2 encode8(const float* v, float& scale) {
   uint32_t a = 0;
 #pragma unroll
@@ -27,27 +30,66 @@ __device__ __forceinline__ uint2 encode8(const float* v, float& scale) {
 #pragma unroll
   for (int m = 1; m < 16; m <<= 1) a = max(a, __shfl_xor_sync(~0u, a, m));
   const float amax = __uint_as_float(a);
-  uint32_t w[2] = {0, 0};
+  float inv = 0.f;
+  scale = 0.f;
   if (a >= 0x7f800000u) {
     scale = __uint_as_float(0x7fffffffu);
-  } else if (amax < 1.2621774483536189e-29f) {  // 2^-96
-    scale = 0.f;
-  } else {
-    const float inv = __fdiv_rn(127.f, amax);
+  } else if (amax >= 1.2621774483536189e-29f) {  // 2^-96
+    inv = __fdiv_rn(127.f, amax);
     scale = __fdiv_rn(amax, 127.f);
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      w[i >> 2] |= ((uint32_t)__float2int_rn(__fmul_rn(v[i], inv)) & 255u) << ((i & 3) * 8);
   }
+  constexpr float MAGIC = 12582912.f;
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = __fadd_rn(__fmul_rn(v[i + j], inv), MAGIC);  // mul2 and add2 may become one fma
+    const uint32_t lo = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x0040);
+    w[i >> 2] = __byte_perm(lo, hi, 0x5410);
+  }
+  if (inv == 0.f) w[0] = w[1] = 0;  // zeros, or a group that restores to NaN
   return make_uint2(w[0], w[1]);
 }
 
+// The 8 codes times `scale`, rounded once: a byte c + 128 below the exponent
+// of 2^23 is the number 2^23 + 128 + c.
 __device__ __forceinline__ void decode8(uint2 c, float scale, float* v) {
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const uint32_t w = i < 4 ? c.x : c.y;
-    v[i] = __fmul_rn((float)(int)(int8_t)((w >> ((i & 3) * 8)) & 255u), scale);
+  for (int i = 0; i < 8; i += 4) {
+    const uint32_t w = (i ? c.y : c.x) ^ 0x80808080u;
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[i + j] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + j));
+    add2(v[i], v[i + 1], -8388736.f, -8388736.f);
+    add2(v[i + 2], v[i + 3], -8388736.f, -8388736.f);
+    mul2(v[i], v[i + 1], scale, scale);
+    mul2(v[i + 2], v[i + 3], scale, scale);
   }
+}
+
+// 8 elements of a row as they are in memory.
+template <class T>
+struct alignas(16) Raw8 {
+  T e[8];
+  __device__ __forceinline__ void to(float* v) const {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = to_float(e[i]);
+  }
+};
+template <class T, bool VEC>  // VEC: p is 16-byte aligned, and n is 8 or not positive
+__device__ __forceinline__ Raw8<T> load_raw(const T* p, int n) {
+  Raw8<T> r;
+  if (VEC) {
+    if (n > 0)
+      r = *reinterpret_cast<const Raw8<T>*>(p);
+    else
+      memset(&r, 0, sizeof(r));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) r.e[i] = i < n ? p[i] : from_float<T>(0.f);
+  }
+  return r;
 }
 
 // 8 elements from p (or n < 8 where the row ends); `vec`: p is 16-byte (fp32:

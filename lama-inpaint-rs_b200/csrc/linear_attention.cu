@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
   __shared__ float pw[CH + 1];
   __shared__ uint64_t bar_mem;
   __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
   const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t bar = smem_u32(&bar_mem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
   if (tid == 0) {
     mbar_init(bar, 1);
     fence_mbar_init();
+    failed = 0;
   }
   for (int i = tid; i <= CH; i += THREADS) pw[i] = power(g, i);
   tc_fence_before();
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
                             idesc_bf16_f32(64) | B_MN, 4, 32, 2048, TILE, ETILE, 4, 0, s > 0);
           mma_commit(bar);
         }
-        ok = mbar_wait(bar, phase, r.status, 1);
+        ok = mbar_wait(bar, phase, &failed, 1);
         phase ^= 1;
         ok = __syncthreads_and(ok);
         if (!ok) break;
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
                          2048, 2048, TILE, TILE, 8, 0, false);
         mma_commit(bar);
       }
-      ok = mbar_wait(bar, phase, r.status, 2);
+      ok = mbar_wait(bar, phase, &failed, 2);
       phase ^= 1;
       ok = __syncthreads_and(ok);
       if (!ok) break;
@@ -345,7 +347,7 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
                           32, 2048, 2 * TILE, TILE, 4, TILE, false);
         mma_commit(bar);
       }
-      ok = mbar_wait(bar, phase, r.status, 3);
+      ok = mbar_wait(bar, phase, &failed, 3);
       phase ^= 1;
       ok = __syncthreads_and(ok);
       if (!ok) break;
@@ -404,7 +406,10 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
           r.seg[(((long long)(batch * r.heads + head) * r.nseg + seg) * (r.slabs * 64) + s * 64 + srow) * ld + blk * 64 +
                 scol + i] = E[s][i];
   }
-  if (!ok) mbar_wait_drain(bar, phase ^ 1);  // the products still in flight
+  if (!ok) {
+    mbar_wait_drain(bar, phase ^ 1);  // the products still in flight
+    if (tid == 0) atomicCAS(r.status, 0, failed);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -113,5 +113,36 @@ __device__ __forceinline__ void store_vec(T* p, const float* v) {
   }
 }
 
+// Pairs of fp32 in one instruction: (x, y) *= (a, b); (x, y) += (a, b);
+// (x, y) = (a, b) * (c, d) + (x, y).  Each element is rounded as by itself.
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 p, q;\n\t"
+      "mov.b64 p, {%0, %1};\n\t"
+      "mov.b64 q, {%2, %3};\n\t"
+      "mul.rn.f32x2 p, p, q;\n\t"
+      "mov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 p, q;\n\t"
+      "mov.b64 p, {%0, %1};\n\t"
+      "mov.b64 q, {%2, %3};\n\t"
+      "add.rn.f32x2 p, p, q;\n\t"
+      "mov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float c, float d) {
+  asm("{\n\t.reg .b64 p, q, r;\n\t"
+      "mov.b64 p, {%0, %1};\n\t"
+      "mov.b64 q, {%2, %3};\n\t"
+      "mov.b64 r, {%4, %5};\n\t"
+      "fma.rn.f32x2 p, q, r, p;\n\t"
+      "mov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+}
+
 }  // namespace ops
 }  // namespace lama

@@ -489,7 +489,7 @@ def gated_residual_norm_backward(grad_u, grad_n, saved) -> NormGradients:
             _tensor(g, name, some, dtype, shape=shape)
 
     def vector(w):
-        return torch.zeros(c, dtype=torch.float32, device=dev) if isinstance(w, torch.Tensor) else None
+        return torch.empty(c, dtype=torch.float32, device=dev) if isinstance(w, torch.Tensor) else None
 
     dx, dy = (torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
     dpost, dpre, dscale = vector(post_weight), vector(pre_weight), vector(residual_scale)
@@ -517,8 +517,10 @@ def gated_residual_norm_backward(grad_u, grad_n, saved) -> NormGradients:
         n = _check(lib().lama_gated_residual_norm_workspace(a, _err.buf, 256))
         w = _workspace(n, dx)
         _check(lib().lama_gated_residual_norm_backward(a, g, _ptr(w), n, dev.index, _stream(dx), _err.buf, 256))
-    elif dgate is not None:
-        dgate.zero_()
+    else:
+        for t in (dgate, dpost, dpre, dscale):
+            if t is not None:
+                t.zero_()
 
     def like(g, w):
         return g if g is None or g.dtype == w.dtype else g.to(w.dtype)
