@@ -586,8 +586,8 @@ template <int NS, bool OUT, bool REV>
 cudaError_t launch(const Run& r, const Maps& maps, int segs, cudaStream_t st) {
   constexpr int bytes = Lay<NS, OUT>::BYTES + 1024;
   static_assert(bytes + 2048 <= 227 * 1024, "shared memory");
-  const cudaError_t ce =
-      cudaFuncSetAttribute(k_pipe<NS, OUT, REV>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static SmemLimit limit;
+  const cudaError_t ce = limit.reach(k_pipe<NS, OUT, REV>, bytes);
   if (ce != cudaSuccess) return ce;
   const long long grid = (long long)r.batch * r.heads * r.blocks * segs;
   k_pipe<NS, OUT, REV><<<(unsigned)grid, THREADS, bytes, st>>>(r, maps, segs);

@@ -486,7 +486,8 @@ __global__ void k_share(const float* src, T* dst, long long rows, int tokens, in
 template <class T, bool OUT>
 cudaError_t launch_chunks(const Run& r, cudaStream_t st) {
   const uint32_t bytes = Plan<T>::bytes(r.slabs);
-  cudaError_t ce = cudaFuncSetAttribute(k_chunks<T, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  static SmemLimit limit;
+  const cudaError_t ce = limit.reach(k_chunks<T, OUT>, (int)bytes);
   if (ce != cudaSuccess) return ce;
   const long long grid = (long long)r.batch * r.heads * r.blocks * (OUT ? r.nseg : r.nseg - 1);
   k_chunks<T, OUT><<<(unsigned)grid, THREADS, bytes, st>>>(r);
@@ -671,7 +672,16 @@ long long up(long long b) { return (b + ALIGN - 1) / ALIGN * ALIGN; }
 
 }  // namespace
 
-cudaError_t status_word(int** p) { return cudaGetSymbolAddress((void**)p, g_status); }
+cudaError_t status_word(int** p) {
+  static std::atomic<int*> known[MAX_DEVICES] = {};
+  int dev = 0;
+  cudaError_t ce = cudaGetDevice(&dev);
+  if (ce != cudaSuccess) return ce;
+  if (dev < MAX_DEVICES && (*p = known[dev].load(std::memory_order_acquire))) return cudaSuccess;
+  ce = cudaGetSymbolAddress((void**)p, g_status);
+  if (ce == cudaSuccess && dev < MAX_DEVICES) known[dev].store(*p, std::memory_order_release);
+  return ce;
+}
 
 }  // namespace ops
 }  // namespace lama

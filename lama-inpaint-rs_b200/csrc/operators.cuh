@@ -6,9 +6,11 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <mutex>
 
 #include "lama_b200.h"
 
@@ -48,6 +50,26 @@ class DeviceGuard {
 // The status word of the operators' bounded waits on the current device
 // (0: no wait ran out).
 cudaError_t status_word(int** p);
+
+// Sets a kernel's dynamic shared-memory limit once per device (`done`: one per
+// kernel; the limit only ever has to be at least `bytes`).
+constexpr int MAX_DEVICES = 64;
+struct SmemLimit {
+  std::atomic<int> set[MAX_DEVICES] = {};
+  template <class K>
+  cudaError_t reach(K* kernel, int bytes) {
+    int dev = 0;
+    cudaError_t ce = cudaGetDevice(&dev);
+    if (ce != cudaSuccess) return ce;
+    if (dev < MAX_DEVICES && set[dev].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+    std::lock_guard<std::mutex> lock(mutex);  // two threads' limits: the larger stays
+    if (dev < MAX_DEVICES && set[dev].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+    ce = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (ce == cudaSuccess && dev < MAX_DEVICES) set[dev].store(bytes, std::memory_order_release);
+    return ce;
+  }
+  std::mutex mutex;
+};
 
 inline int dtype_size(int t) { return t == LAMA_F32 ? 4 : 2; }
 inline bool dtype_ok(int t) { return t == LAMA_F32 || t == LAMA_F16 || t == LAMA_BF16; }

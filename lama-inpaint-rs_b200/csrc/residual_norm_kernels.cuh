@@ -612,13 +612,14 @@ cudaError_t by_width(int c, F&& f) {
 }
 constexpr int STATIC_SMEM = 12 * 1024;  // the kernels' static arrays, at most
 
-template <class P>
-cudaError_t start(void (*kernel)(P), unsigned grid, int threads, size_t smem, cudaStream_t st, const P& p) {
+template <auto KERNEL, class P>
+cudaError_t start(unsigned grid, int threads, size_t smem, cudaStream_t st, const P& p) {
+  static SmemLimit limit;
   if (smem > 48 * 1024 - STATIC_SMEM) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = limit.reach(KERNEL, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  kernel<<<grid, threads, smem, st>>>(p);
+  KERNEL<<<grid, threads, smem, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -641,13 +642,13 @@ cudaError_t run_forward(const Fwd& f, cudaStream_t st) {
     size_t smem = 2 * sizeof(float) * (size_t)f.c;
     const size_t row = (size_t)f.c * sizeof(T) * (f.gate && f.per == 1 ? 3 : 2);
     if (f.vec && ring_fits<W>(f.c, row, smem))
-      return f.cy ? start(k_norm<T, W, NI, true, RING>, grid, TH, smem, st, f)
-                  : start(k_norm<T, W, NI, false, RING>, grid, TH, smem, st, f);
+      return f.cy ? start<k_norm<T, W, NI, true, RING>>(grid, TH, smem, st, f)
+                  : start<k_norm<T, W, NI, false, RING>>(grid, TH, smem, st, f);
     if (f.vec)
-      return f.cy ? start(k_norm<T, W, NI, true, VECTOR>, grid, TH, smem, st, f)
-                  : start(k_norm<T, W, NI, false, VECTOR>, grid, TH, smem, st, f);
-    return f.cy ? start(k_norm<T, W, NI, true, SCALAR>, grid, TH, smem, st, f)
-                : start(k_norm<T, W, NI, false, SCALAR>, grid, TH, smem, st, f);
+      return f.cy ? start<k_norm<T, W, NI, true, VECTOR>>(grid, TH, smem, st, f)
+                  : start<k_norm<T, W, NI, false, VECTOR>>(grid, TH, smem, st, f);
+    return f.cy ? start<k_norm<T, W, NI, true, SCALAR>>(grid, TH, smem, st, f)
+                : start<k_norm<T, W, NI, false, SCALAR>>(grid, TH, smem, st, f);
   });
 }
 
@@ -662,13 +663,13 @@ cudaError_t run_backward(const Bwd& b, cudaStream_t st) {
     const size_t row = kept * (pre ? 2 : 1) + full * ((b.gu != nullptr) + pre + (b.gate && b.per == 1)) +
                        (8 + (codes ? 8 * (size_t)b.groups : 0) + 15) / 16 * 16;
     if (b.vec && (!codes || ((uintptr_t)b.cy | (uintptr_t)b.cu | b.c) % 16 == 0) && ring_fits<W>(b.c, row, smem))
-      return codes ? start(k_norm_grad<T, W, NI, true, RING>, grid, TH, smem, st, b)
-                   : start(k_norm_grad<T, W, NI, false, RING>, grid, TH, smem, st, b);
+      return codes ? start<k_norm_grad<T, W, NI, true, RING>>(grid, TH, smem, st, b)
+                   : start<k_norm_grad<T, W, NI, false, RING>>(grid, TH, smem, st, b);
     if (b.vec)
-      return codes ? start(k_norm_grad<T, W, NI, true, VECTOR>, grid, TH, smem, st, b)
-                   : start(k_norm_grad<T, W, NI, false, VECTOR>, grid, TH, smem, st, b);
-    return codes ? start(k_norm_grad<T, W, NI, true, SCALAR>, grid, TH, smem, st, b)
-                 : start(k_norm_grad<T, W, NI, false, SCALAR>, grid, TH, smem, st, b);
+      return codes ? start<k_norm_grad<T, W, NI, true, VECTOR>>(grid, TH, smem, st, b)
+                   : start<k_norm_grad<T, W, NI, false, VECTOR>>(grid, TH, smem, st, b);
+    return codes ? start<k_norm_grad<T, W, NI, true, SCALAR>>(grid, TH, smem, st, b)
+                 : start<k_norm_grad<T, W, NI, false, SCALAR>>(grid, TH, smem, st, b);
   });
   if (e != cudaSuccess) return e;
   k_norm_sums<T><<<(b.c + 31) / 32, 1024, 0, st>>>(b);

@@ -48,38 +48,6 @@ class OpTime(ctypes.Structure):
                 ("end_ms", ctypes.c_float)]
 
 
-class Rows(ctypes.Structure):  # lama_rows
-    _fields_ = [("data", _vp), ("batch_stride", ctypes.c_longlong), ("token_stride", ctypes.c_longlong),
-                ("head_stride", ctypes.c_longlong), ("heads", ctypes.c_int)]
-
-
-class AttentionArgs(ctypes.Structure):  # lama_attention
-    _fields_ = [("dtype", ctypes.c_int), ("batch", ctypes.c_int), ("tokens", ctypes.c_int), ("heads", ctypes.c_int),
-                ("dk", ctypes.c_int), ("dv", ctypes.c_int), ("q", Rows), ("k", Rows), ("v", Rows), ("log_decay", _vp),
-                ("initial_state", _vp), ("lengths", _vp), ("scale", ctypes.c_float)]
-
-
-class AttentionGrads(ctypes.Structure):  # lama_attention_grads
-    _fields_ = [("grad_out", Rows), ("grad_q", Rows), ("grad_k", Rows), ("grad_v", Rows), ("grad_final_state", _vp),
-                ("grad_initial_state", _vp)]
-
-
-class NormArgs(ctypes.Structure):  # lama_norm
-    _fields_ = [("dtype", ctypes.c_int), ("rows", ctypes.c_longlong), ("channels", ctypes.c_int), ("gate", _vp),
-                ("gate_rows", ctypes.c_longlong), ("gate_stride", ctypes.c_longlong), ("post_weight", _vp),
-                ("pre_weight", _vp), ("residual_scales", _vp), ("residual_scale", ctypes.c_float),
-                ("eps", ctypes.c_float)]
-
-
-class NormGrads(ctypes.Structure):  # lama_norm_grads
-    _fields_ = [("grad_u", _vp), ("grad_n", _vp), ("y", _vp), ("u", _vp), ("grad_u_stride", ctypes.c_longlong),
-                ("grad_n_stride", ctypes.c_longlong), ("y_stride", ctypes.c_longlong),
-                ("u_stride", ctypes.c_longlong), ("y_codes", _vp), ("u_codes", _vp), ("y_scales", _vp),
-                ("u_scales", _vp), ("post_rstd", _vp), ("pre_rstd", _vp), ("grad_x", _vp), ("grad_y", _vp),
-                ("grad_gate", _vp), ("grad_post_weight", _vp), ("grad_pre_weight", _vp),
-                ("grad_residual_scales", _vp)]
-
-
 _lib = None
 
 # Every symbol include/lama_b200.h declares: (name, restype, argtypes).
@@ -123,22 +91,23 @@ SIGNATURES = [
     ("lama_mask_depth", ctypes.c_int, [_u8p, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
     ("lama_section_rects", ctypes.c_int, [_u8p, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_int),
                                           ctypes.c_int]),
-    ("lama_linear_attention_workspace", ctypes.c_longlong, [ctypes.POINTER(AttentionArgs), ctypes.c_int,
+    # the operators' structures are passed as packed bytes (operators.py)
+    ("lama_linear_attention_workspace", ctypes.c_longlong, [ctypes.c_char_p, ctypes.c_int,
                                                             ctypes.c_char_p, ctypes.c_int]),
-    ("lama_linear_attention", ctypes.c_int, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(Rows), _vp, _vp,
+    ("lama_linear_attention", ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, _vp, _vp,
                                              ctypes.c_longlong, ctypes.c_int, _vp, ctypes.c_char_p, ctypes.c_int]),
-    ("lama_linear_attention_backward", ctypes.c_int, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(AttentionGrads),
+    ("lama_linear_attention_backward", ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p,
                                                       _vp, ctypes.c_longlong, ctypes.c_int, _vp, ctypes.c_char_p,
                                                       ctypes.c_int]),
-    ("lama_linear_attention_step", ctypes.c_int, [ctypes.POINTER(AttentionArgs), ctypes.POINTER(Rows), _vp, _vp,
+    ("lama_linear_attention_step", ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, _vp, _vp,
                                                   ctypes.c_int, _vp, ctypes.c_int, _vp, ctypes.c_char_p,
                                                   ctypes.c_int]),
-    ("lama_gated_residual_norm", ctypes.c_int, [ctypes.POINTER(NormArgs), _vp, ctypes.c_longlong, _vp,
+    ("lama_gated_residual_norm", ctypes.c_int, [ctypes.c_char_p, _vp, ctypes.c_longlong, _vp,
                                                 ctypes.c_longlong, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                                 ctypes.c_int, _vp, ctypes.c_char_p, ctypes.c_int]),
-    ("lama_gated_residual_norm_workspace", ctypes.c_longlong, [ctypes.POINTER(NormArgs), ctypes.c_char_p,
+    ("lama_gated_residual_norm_workspace", ctypes.c_longlong, [ctypes.c_char_p, ctypes.c_char_p,
                                                                ctypes.c_int]),
-    ("lama_gated_residual_norm_backward", ctypes.c_int, [ctypes.POINTER(NormArgs), ctypes.POINTER(NormGrads), _vp,
+    ("lama_gated_residual_norm_backward", ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, _vp,
                                                          ctypes.c_longlong, ctypes.c_int, _vp, ctypes.c_char_p,
                                                          ctypes.c_int]),
     ("lama_checkpoint_store", ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_longlong,
