@@ -66,17 +66,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int c
       : "memory");
 }
 
-// true in one lane of the (converged) warp
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(p));
-  return p != 0;
-}
-
 // A from TMEM (128 lanes, two 16-bit elements a column), B from shared memory
 __device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(

@@ -61,60 +61,66 @@ struct Parts<float> {
 
 // 64 columns from d0 of the chunk's rows, as parts, zeros past the sequence
 // and past the head's size.  Row r of the chunk is token first + r * step.
+// Loops here and below stay loops: unrolled, the kernel is 150 KB of code that is
+// fetched again for every chunk.
 template <class T>
-__device__ void load_tile(uint32_t dst, const Operand& o, int batch, int head, long long first, int step, int n, int d0,
-                          int d) {
+__device__ __noinline__ void load_tile(uint32_t dst, const T* base, long long stride, int n, int left, bool vec) {
   constexpr int NP = Parts<T>::N;
-  const T* base = static_cast<const T*>(o.p) + batch * o.sb + (head / o.per) * o.sh + first * o.st;
+  if (vec) {
+#pragma unroll 2
+    for (int it = 0; it < CH * 8 / THREADS; it++) {
+      const int c = it * THREADS + (int)threadIdx.x, row = c >> 3, ck = c & 7;
+      uint4 parts[NP];
 #pragma unroll
-  for (int it = 0; it < CH * 8 / THREADS; it++) {
-    const int c = it * THREADS + (int)threadIdx.x, row = c >> 3, ck = c & 7;
-    const int col = d0 + ck * 8;
-    uint4 parts[NP];
-#pragma unroll
-    for (int p = 0; p < NP; p++) parts[p] = make_uint4(0, 0, 0, 0);
-    if (row < n && col < d) {
-      const T* src = base + (long long)row * step * o.st + col;
-      if (o.vec && NP == 1) {
-        parts[0] = *reinterpret_cast<const uint4*>(src);
-      } else {
+      for (int p = 0; p < NP; p++) parts[p] = make_uint4(0, 0, 0, 0);
+      if (row < n && ck * 8 < left) {
         float v[8];
-        if (o.vec) {
-          load_vec<T, 8>(src, v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; i++) v[i] = col + i < d ? to_float(src[i]) : 0.f;
-        }
+        load_vec<T, 8>(base + row * stride + ck * 8, v);
         split8<NP>(v, parts);
       }
-    }
 #pragma unroll
-    for (int p = 0; p < NP; p++) sts16(dst + p * TILE + swz(row, ck), parts[p]);
+      for (int p = 0; p < NP; p++) sts16(dst + p * TILE + swz(row, ck), parts[p]);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < CH * 64; i += THREADS) {
+      const int row = i >> 6, col = i & 63;
+      float v = row < n && col < left ? to_float(base[row * stride + col]) : 0.f;
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+        const __nv_bfloat16 h = __float2bfloat16_rn(v);
+        asm volatile("st.shared.b16 [%0], %1;" ::"r"(dst + p * TILE + swz(row, col >> 3) + (col & 7) * 2),
+                     "h"(__bfloat16_as_ushort(h))
+                     : "memory");
+        v -= __bfloat162float(h);
+      }
+    }
   }
 }
 
 // D (+)= A B over K, the pairs of parts (x, y) with x + y < max(NA, NB), the
 // smallest first: the tensor core truncates each sum to fp32, so what is
 // added while the accumulator is still small loses less (fp32 inputs measured
-// 2e-6 off with the largest pair first).
-// `ka`, `kb`: byte steps of a 16-wide K step; after `kwrap` steps A moves on by `awrap` bytes instead.
+// 2e-6 off with the largest pair first).  K in `blocks` of four 16-wide steps,
+// `ka` and `kb` bytes apart, the blocks `ba` and `bb`.
 template <int NA, int NB>
-__device__ __forceinline__ void mma_parts(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int steps, uint32_t ka,
-                                          uint32_t kb, uint32_t pa, uint32_t pb, int kwrap, uint32_t awrap,
+__device__ __forceinline__ void mma_parts(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int blocks, uint32_t ka,
+                                          uint32_t ba, uint32_t pa, uint32_t kb, uint32_t bb, uint32_t pb,
                                           bool accumulate) {
   constexpr int LIM = NA > NB ? NA : NB;
   uint32_t acc = accumulate;
-#pragma unroll
+#pragma unroll 1
   for (int z = LIM - 1; z >= 0; z--)
+#pragma unroll 1
+    for (int x = max(0, z - NB + 1); x < NA && x <= z; x++) {
+      uint64_t ax = a + ((x * pa) >> 4), by = b + (((z - x) * pb) >> 4);
+#pragma unroll 1
+      for (int k = 0; k < blocks; k++, ax += ba >> 4, by += bb >> 4)
 #pragma unroll
-    for (int x = 0; x < NA; x++) {
-      const int y = z - x;
-      if (y < 0 || y >= NB) continue;
-      for (int s = 0; s < steps; s++) {
-        const uint32_t ao = x * pa + (s % kwrap) * ka + (s / kwrap) * awrap, bo = y * pb + s * kb;
-        mma_bf16(d, a + (ao >> 4), b + (bo >> 4), idesc, acc);
-        acc = 1;
-      }
+        for (int s = 0; s < 4; s++) {
+          mma_bf16(d, ax + ((s * ka) >> 4), by + ((s * kb) >> 4), idesc, acc);
+          acc = 1;
+        }
     }
 }
 
@@ -130,7 +136,7 @@ struct Plan {
   static constexpr uint32_t P = NP == 3 ? A : BD;
   static constexpr uint32_t W = NP == 3 ? 0 : (2 * NP > 3 ? 2 * NP : 3) * TILE;
   static constexpr uint32_t E = 3 * NP * TILE + W;
-  static constexpr uint32_t bytes(int slabs) { return E + EP * ETILE * slabs + 1024; }
+  static constexpr uint32_t bytes() { return E + EP * ETILE + 1024; }
 };
 
 template <class T, bool OUT>
@@ -178,77 +184,93 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
   const int srow = row & 63;                         // state row of a slab
   const int scol = ((warp >> 2) * 2 + (row >> 6)) * 16;  // its 16 columns
 
+  // the carried state: 16 columns of row srow of each slab
   float E[MAXS][16];
   const int ld = r.blocks * 64;
   const float lam = pw[1];
+  const long long bh = (long long)batch * r.heads + head;
 #pragma unroll
-  for (int s = 0; s < MAXS; s++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      float v = 0.f;
-      const int er = s * 64 + srow, ec = blk * 64 + scol + i;
-      if (OUT && s < r.slabs) {
-        if (r.staged) {
-          v = r.seg[(((long long)(batch * r.heads + head) * r.nseg + seg) * (r.slabs * 64) + er) * ld + ec];
-        } else if (r.init && er < r.da && ec < r.dc) {
-          v = r.init[(long long)(batch * r.heads + head) * r.da * r.dc + er * r.ir + ec * r.ic];
-          if (!r.reverse) v *= lam;
-        }
+  for (int s = 0; s < MAXS; s++) {
+    const int er = s * 64 + srow, ec = blk * 64 + scol;
+    const float* src = nullptr;
+    long long step = 1;
+    int cols = 0;
+    float f = 1.f;
+    if (OUT && s < r.slabs) {
+      if (r.staged) {
+        src = r.seg + ((bh * r.nseg + seg) * (r.slabs * 64) + er) * ld + ec;
+        cols = 16;
+      } else if (r.init && er < r.da) {
+        src = r.init + bh * r.da * r.dc + er * r.ir + ec * r.ic;
+        step = r.ic;
+        cols = r.dc - ec;
+        if (!r.reverse) f = lam;
       }
-      E[s][i] = v;
     }
+#pragma unroll
+    for (int i = 0; i < 16; i++, src += step) E[s][i] = i < cols ? f * *src : 0.f;
+  }
 
   uint32_t phase = 0;
   bool ok = true;
   int done = 0;  // tokens of this segment so far
   const int step = r.reverse ? -1 : 1;
+  auto wait = [&](int code) {
+    ok = __syncthreads_and(mbar_wait(bar, phase, &failed, code));
+    phase ^= 1;
+    tc_fence_after();
+    return ok;
+  };
+#pragma unroll 1
   for (int ch = 0; ok && ch < r.chunks; ch++) {
     const int pos = p0 + ch * CH;
     const int n = min(CH, len - pos);
     if (n <= 0) break;
     const bool last = pos + n == len;
     const long long first = r.reverse ? (long long)len - 1 - pos : pos;
-    load_tile<T>(smem + PL::C, r.c, batch, head, first, step, n, blk * 64, r.dc);
-    if (OUT) {
+    auto load = [&](uint32_t dst, const Operand& o, int d0, int d) {
+      const T* base = static_cast<const T*>(o.p) + batch * o.sb + (head / o.per) * o.sh + first * o.st + d0;
+      load_tile<T>(dst, base, step * o.st, n, d - d0, o.vec);
+    };
+    load(smem + PL::C, r.c, blk * 64, r.dc);
+#pragma unroll 1
+    for (int s = 0; s < r.slabs; s++) {
+      float e[16];
 #pragma unroll
-      for (int s = 0; s < MAXS; s++) {
-        if (s >= r.slabs) break;
+      for (int i = 0; i < 16; i++) e[i] = s ? E[1][i] : E[0][i];
+      if (OUT) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           uint4 parts[EP];
-          split8<EP>(&E[s][h * 8], parts);
+          split8<EP>(e + h * 8, parts);
 #pragma unroll
-          for (int p = 0; p < EP; p++) sts16(smem + PL::E + (s * EP + p) * ETILE + swz(srow, (scol >> 3) + h), parts[p]);
+          for (int p = 0; p < EP; p++) sts16(smem + PL::E + p * ETILE + swz(srow, (scol >> 3) + h), parts[p]);
         }
+        load(smem + PL::A, r.a, s * 64, r.da);
       }
-    }
-#pragma unroll
-    for (int s = 0; s < MAXS; s++) {
-      if (s >= r.slabs) break;
-      if (OUT) load_tile<T>(smem + PL::A, r.a, batch, head, first, step, n, s * 64, r.da);
-      load_tile<T>(smem + PL::B, r.b, batch, head, first, step, n, s * 64, r.da);
+      load(smem + PL::B, r.b, s * 64, r.da);
+      // scores and a E before b's place may be taken by the decayed b
+      auto scores = [&] {
+        tc_fence_after();
+        mma_parts<NP, NP>(t_p, smem_desc(smem + PL::A, 1024, 2), smem_desc(smem + PL::B, 1024, 2), idesc_bf16_f32(128),
+                          1, 32, 0, TILE, 32, 0, TILE, s > 0);
+        mma_parts<NP, EP>(t_o, smem_desc(smem + PL::A, 1024, 2), desc_mn(smem + PL::E, 0), idesc_bf16_f32(64) | B_MN, 1,
+                          32, 0, TILE, 2048, 0, ETILE, s > 0);
+      };
       if (OUT && NP == 3) {
-        // scores and a E first: the decayed b takes b's place
         fence_async_smem();
         __syncthreads();
-        if (tid == 0) {
-          tc_fence_after();
-          mma_parts<NP, NP>(t_p, smem_desc(smem + PL::A, 1024, 2), smem_desc(smem + PL::B, 1024, 2), idesc_bf16_f32(128),
-                            4, 32, 32, TILE, TILE, 4, 0, s > 0);
-          mma_parts<NP, EP>(t_o, smem_desc(smem + PL::A, 1024, 2), desc_mn(smem + PL::E + s * EP * ETILE, 0),
-                            idesc_bf16_f32(64) | B_MN, 4, 32, 2048, TILE, ETILE, 4, 0, s > 0);
+        if (warp == 0 && elect_one()) {
+          scores();
           mma_commit(bar);
         }
-        ok = mbar_wait(bar, phase, &failed, 1);
-        phase ^= 1;
-        ok = __syncthreads_and(ok);
-        if (!ok) break;
-        tc_fence_after();
+        __syncwarp();
+        if (!wait(1)) break;
       } else {
         __syncthreads();
       }
       // decayed b: row j times lam^{n-1-j}, three parts
-#pragma unroll
+#pragma unroll 2
       for (int it = 0; it < CH * 8 / THREADS; it++) {
         const int c = it * THREADS + tid, j = c >> 3, ck = c & 7;
         float v[8];
@@ -257,11 +279,11 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
 #pragma unroll
         for (int p = 0; p < NP; p++) {
           const uint4 u = lds16(smem + PL::B + p * TILE + swz(j, ck));
-          const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&u);
+          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&u);
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            v[2 * i] += __low2float(e[i]);
-            v[2 * i + 1] += __high2float(e[i]);
+            v[2 * i] += __low2float(x[i]);
+            v[2 * i + 1] += __high2float(x[i]);
           }
         }
         const float w = j < n ? pw[n - 1 - j] : 0.f;
@@ -274,51 +296,46 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
       }
       fence_async_smem();
       __syncthreads();
-      if (tid == 0) {
+      if (warp == 0 && elect_one()) {
         tc_fence_after();
-        if (OUT && NP != 3) {
-          mma_parts<NP, NP>(t_p, smem_desc(smem + PL::A, 1024, 2), smem_desc(smem + PL::B, 1024, 2), idesc_bf16_f32(128),
-                            4, 32, 32, TILE, TILE, 4, 0, s > 0);
-          mma_parts<NP, EP>(t_o, smem_desc(smem + PL::A, 1024, 2), desc_mn(smem + PL::E + s * EP * ETILE, 0),
-                            idesc_bf16_f32(64) | B_MN, 4, 32, 2048, TILE, ETILE, 4, 0, s > 0);
-        }
+        if (OUT && NP != 3) scores();
         // both 64-row halves of the MMA's 128 rows read the slab's 64 columns
-        mma_parts<3, NP>(t_u, desc_mn(smem + PL::BD, 0), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | A_MN | B_MN, 8,
-                         2048, 2048, TILE, TILE, 8, 0, false);
+        mma_parts<3, NP>(t_u, desc_mn(smem + PL::BD, 0), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | A_MN | B_MN, 2,
+                         2048, 8192, TILE, 2048, 8192, TILE, false);
         mma_commit(bar);
       }
-      ok = mbar_wait(bar, phase, &failed, 2);
-      phase ^= 1;
-      ok = __syncthreads_and(ok);
-      if (!ok) break;
-      tc_fence_after();
+      __syncwarp();
+      if (!wait(2)) break;
       float u[16];
       tmem_ld16(t_u + lane_base + scol, u);
       tmem_wait_ld();
       const float dn1 = pw[n - 1];
 #pragma unroll
-      for (int i = 0; i < 16; i++) E[s][i] = dn1 * E[s][i] + r.update * u[i];  // the state after the chunk
+      for (int i = 0; i < 16; i++) e[i] = dn1 * e[i] + r.update * u[i];  // the state after the chunk
       if (OUT && last && r.fin) {
+        const int er = s * 64 + srow, ec = blk * 64 + scol;
+        float* dst = r.fin + bh * r.da * r.dc + er * r.fr + ec * r.fc;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const int er = s * 64 + srow, ec = blk * 64 + scol + i;
-          if (er < r.da && ec < r.dc)
-            r.fin[(long long)(batch * r.heads + head) * r.da * r.dc + er * r.fr + ec * r.fc] =
-                r.reverse ? lam * E[s][i] : E[s][i];
-        }
+        for (int i = 0; i < 16; i++, dst += r.fc)
+          if (er < r.da && ec + i < r.dc) *dst = r.reverse ? lam * e[i] : e[i];
       }
-      if (OUT || ch + 1 < r.chunks)
+      const float f = OUT || ch + 1 < r.chunks ? lam : 1.f;
 #pragma unroll
-        for (int i = 0; i < 16; i++) E[s][i] *= lam;
+      for (int i = 0; i < 16; i++) {
+        e[i] *= f;
+        if (s)
+          E[1][i] = e[i];
+        else
+          E[0][i] = e[i];
+      }
       tc_fence_before();
-      if (s + 1 < r.slabs) __syncthreads();  // the next slab's tiles and accumulator
+      __syncthreads();  // the next slab's tiles and accumulator
     }
     if (!ok) break;
     done = pos + n - p0;
     if (OUT) {
       // scores: decay and causal mask, rounded to NP parts
-      __syncthreads();
-#pragma unroll
+#pragma unroll 1
       for (int h = 0; h < 2; h++) {
         const int col0 = (warp >> 2) * 64 + h * 32;
         float v[32];
@@ -341,45 +358,43 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
       tc_fence_before();
       fence_async_smem();
       __syncthreads();
-      if (tid == 0) {
+      if (warp == 0 && elect_one()) {
         tc_fence_after();
-        mma_parts<NP, NP>(t_p, smem_desc(smem + PL::P, 1024, 2), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | B_MN, 8,
-                          32, 2048, 2 * TILE, TILE, 4, TILE, false);
+        mma_parts<NP, NP>(t_p, smem_desc(smem + PL::P, 1024, 2), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | B_MN, 2,
+                          32, TILE, 2 * TILE, 2048, 8192, TILE, false);
         mma_commit(bar);
       }
-      ok = mbar_wait(bar, phase, &failed, 3);
-      phase ^= 1;
-      ok = __syncthreads_and(ok);
-      if (!ok) break;
-      tc_fence_after();
-      const int col0 = (warp >> 2) * 32;
-      float x[32], y[32];
-      tmem_ld32(t_o + lane_base + col0, x);
-      tmem_ld32(t_p + lane_base + col0, y);
-      tmem_wait_ld();
-      tc_fence_before();
+      __syncwarp();
+      if (!wait(3)) break;
       const float di = pw[row] * r.inter;
+      const long long at = batch * r.ob + (first + (long long)row * step) * r.ot + head * r.oh + blk * 64;
+#pragma unroll 1
+      for (int h = 0; h < 2; h++) {
+        const int col0 = (warp >> 2) * 32 + h * 16, left = r.dc - blk * 64 - col0;
+        float x[16], y[16];
+        tmem_ld16(t_o + lane_base + col0, x);
+        tmem_ld16(t_p + lane_base + col0, y);
+        tmem_wait_ld();
+        if (row >= n) continue;
 #pragma unroll
-      for (int i = 0; i < 32; i++) x[i] = di * x[i] + r.intra * y[i];
-      if (row < n) {
-        const long long at = batch * r.ob + (first + (long long)row * step) * r.ot + head * r.oh;
-        const int c0 = blk * 64 + col0;
+        for (int i = 0; i < 16; i++) x[i] = di * x[i] + r.intra * y[i];
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
+        for (int i = 0; i < 16; i += 8)
           if (r.out_f32)
-            store_row(static_cast<float*>(r.out) + at + c0 + i, x + i, r.dc - c0 - i, r.out_vec);
+            store_row(static_cast<float*>(r.out) + at + col0 + i, x + i, left - i, r.out_vec);
           else
-            store_row(static_cast<T*>(r.out) + at + c0 + i, x + i, r.dc - c0 - i, r.out_vec);
-        }
+            store_row(static_cast<T*>(r.out) + at + col0 + i, x + i, left - i, r.out_vec);
       }
+      tc_fence_before();
+      __syncthreads();  // the next chunk's tiles
     }
-    __syncthreads();  // the next chunk's tiles
   }
 
   if (ok && OUT) {
     // tokens past the sequence's end
     const int end = min(p0 + seg_tokens, r.tokens);
     const int width = min(64, r.dc - blk * 64);
+#pragma unroll 1
     for (int i = tid; i < (end - p0 - done) * 64; i += THREADS) {
       const int t = p0 + done + (i >> 6), c = i & 63;
       if (c >= width) continue;
@@ -390,21 +405,22 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
         static_cast<T*>(r.out)[at] = from_float<T>(0.f);
     }
     if (len == 0 && seg == 0 && r.fin) {
+#pragma unroll 1
       for (int i = tid; i < r.da * 64; i += THREADS) {
         const int er = i >> 6, ec = blk * 64 + (i & 63);
-        const long long base = (long long)(batch * r.heads + head) * r.da * r.dc;
+        const long long base = bh * r.da * r.dc;
         if (ec < r.dc) r.fin[base + er * r.fr + ec * r.fc] = r.init ? r.init[base + er * r.ir + ec * r.ic] : 0.f;
       }
     }
   }
   if (ok && !OUT) {
 #pragma unroll
-    for (int s = 0; s < MAXS; s++)
+    for (int s = 0; s < MAXS; s++) {
+      if (s >= r.slabs) break;
+      float* dst = r.seg + ((bh * r.nseg + seg) * (r.slabs * 64) + s * 64 + srow) * ld + blk * 64 + scol;
 #pragma unroll
-      for (int i = 0; i < 16; i++)
-        if (s < r.slabs)
-          r.seg[(((long long)(batch * r.heads + head) * r.nseg + seg) * (r.slabs * 64) + s * 64 + srow) * ld + blk * 64 +
-                scol + i] = E[s][i];
+      for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(E[s][i], E[s][i + 1], E[s][i + 2], E[s][i + 3]);
+    }
   }
   if (!ok) {
     mbar_wait_drain(bar, phase ^ 1);  // the products still in flight
@@ -485,7 +501,7 @@ __global__ void k_share(const float* src, T* dst, long long rows, int tokens, in
 
 template <class T, bool OUT>
 cudaError_t launch_chunks(const Run& r, cudaStream_t st) {
-  const uint32_t bytes = Plan<T>::bytes(r.slabs);
+  const uint32_t bytes = Plan<T>::bytes();
   static SmemLimit limit;
   const cudaError_t ce = limit.reach(k_chunks<T, OUT>, (int)bytes);
   if (ce != cudaSuccess) return ce;
@@ -496,10 +512,12 @@ cudaError_t launch_chunks(const Run& r, cudaStream_t st) {
 
 // How a sequence is cut: one segment reads everything once, several read b
 // and c twice but fill the GPU.  Takes the least time on the busiest SM,
-// counted in chunk steps: a CTA costs 4 beside its chunks (set-up, the first
-// loads, the last products), the pass that makes the states about 0.6 a
-// chunk and, with the scan, two launches of about 3 each.
-void cut(Run& r) {
+// counted in chunk steps.  Pipelined (bf16): a CTA costs 4 beside its chunks
+// (set-up, the first loads, the last products), the pass that makes the
+// states 0.6 a chunk and, with the scan, two launches of 3 each.  The other
+// kernel's steps are several times longer and do not overlap.
+void cut(Run& r, bool pipe) {
+  const double cta = pipe ? 4 : 1, pass = pipe ? 6 : 1;
   const int slots = 148;
   const int chunks = (r.tokens + CH - 1) / CH;
   const long long rows = (long long)r.batch * r.heads * r.blocks;
@@ -507,7 +525,7 @@ void cut(Run& r) {
   for (int c = chunks;;) {
     const int nseg = (chunks + c - 1) / c;
     const double waves = (double)((rows * nseg + slots - 1) / slots);
-    const double cost = nseg == 1 ? waves * (c + 4) : waves * (1.6 * c + 8) + 6 + 0.05 * nseg;
+    const double cost = nseg == 1 ? waves * (c + cta) : waves * (1.6 * c + 2 * cta) + pass + 0.05 * nseg;
     if (cost < best) {
       best = cost;
       r.nseg = nseg;
@@ -525,7 +543,7 @@ long long seg_bytes(const lama_attention* p, int da, int dc) {
   Run r{};
   r.batch = p->batch, r.heads = p->heads, r.tokens = p->tokens;
   r.slabs = (da + 63) / 64, r.blocks = (dc + 63) / 64;
-  cut(r);
+  cut(r, p->dtype == LAMA_BF16);
   if (!r.staged && p->dtype != LAMA_BF16) return 0;
   return (long long)r.batch * r.heads * r.nseg * r.slabs * 64 * r.blocks * 64 * 4;
 }
@@ -572,7 +590,7 @@ void output(Run& r, const lama_rows& x, int d, int dtype) {
   r.out_f32 = 0;
 }
 
-void roles(Run& r, const Operand& a, const Operand& b, const Operand& c, int da, int dc) {
+void roles(Run& r, const Operand& a, const Operand& b, const Operand& c, int da, int dc, int dtype) {
   r.a = a;
   r.b = b;
   r.c = c;
@@ -580,7 +598,7 @@ void roles(Run& r, const Operand& a, const Operand& b, const Operand& c, int da,
   r.dc = dc;
   r.slabs = (da + 63) / 64;
   r.blocks = (dc + 63) / 64;
-  cut(r);
+  cut(r, dtype == LAMA_BF16);
 }
 
 const char* check_rows(const lama_rows& x, const lama_attention* p, const char* what, char* buf, size_t n) {
@@ -630,7 +648,7 @@ Run common(const lama_attention* p) {
 Run forward_run(const lama_attention* p, float* final_state) {
   Run r = common(p);
   roles(r, operand(p->q, p->heads, p->dk, p->dtype), operand(p->k, p->heads, p->dk, p->dtype),
-        operand(p->v, p->heads, p->dv, p->dtype), p->dk, p->dv);
+        operand(p->v, p->heads, p->dv, p->dtype), p->dk, p->dv, p->dtype);
   r.fin = final_state;
   r.inter = r.intra = p->scale;
   r.update = 1.f;
@@ -646,15 +664,15 @@ Run gradient_run(const lama_attention* p, const lama_attention_grads* g, int whi
   const Operand q = operand(p->q, p->heads, p->dk, p->dtype), k = operand(p->k, p->heads, p->dk, p->dtype),
                 v = operand(p->v, p->heads, p->dv, p->dtype), d = operand(g->grad_out, p->heads, p->dv, p->dtype);
   if (which == 0) {
-    roles(r, d, v, k, p->dv, p->dk);
+    roles(r, d, v, k, p->dv, p->dk, p->dtype);
     r.inter = r.intra = p->scale;
     r.update = 1.f;
     r.init = p->initial_state;
   } else {
     if (which == 1) {
-      roles(r, v, d, q, p->dv, p->dk);
+      roles(r, v, d, q, p->dv, p->dk, p->dtype);
     } else {
-      roles(r, k, q, d, p->dk, p->dv);
+      roles(r, k, q, d, p->dk, p->dv, p->dtype);
       r.fin = g->grad_initial_state;
     }
     r.inter = 1.f;
