@@ -68,30 +68,6 @@ __device__ __forceinline__ void decode8(uint2 c, float scale, float* v) {
   }
 }
 
-// 8 elements of a row as they are in memory.
-template <class T>
-struct alignas(16) Raw8 {
-  T e[8];
-  __device__ __forceinline__ void to(float* v) const {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = to_float(e[i]);
-  }
-};
-template <class T, bool VEC>  // VEC: p is 16-byte aligned, and n is 8 or not positive
-__device__ __forceinline__ Raw8<T> load_raw(const T* p, int n) {
-  Raw8<T> r;
-  if (VEC) {
-    if (n > 0)
-      r = *reinterpret_cast<const Raw8<T>*>(p);
-    else
-      memset(&r, 0, sizeof(r));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) r.e[i] = i < n ? p[i] : from_float<T>(0.f);
-  }
-  return r;
-}
-
 // 8 elements from p (or n < 8 where the row ends); `vec`: p is 16-byte (fp32:
 // two 16-byte words) aligned and n is 8.
 template <class T>

@@ -63,37 +63,45 @@ struct Parts<float> {
 // and past the head's size.  Row r of the chunk is token first + r * step.
 // Loops here and below stay loops: unrolled, the kernel is 150 KB of code that is
 // fetched again for every chunk.
+// Aligned rows are fetched into registers a tile ahead (Fetch), so that their
+// latency passes during the products of the tile before; other rows are read
+// element by element when their place is free.
 template <class T>
-__device__ __noinline__ void load_tile(uint32_t dst, const T* base, long long stride, int n, int left, bool vec) {
-  constexpr int NP = Parts<T>::N;
-  if (vec) {
-#pragma unroll 2
+struct Fetch {
+  Raw8<T> r[CH * 8 / THREADS];
+  __device__ __forceinline__ void load(const T* base, long long stride, int n, int left) {
+#pragma unroll
     for (int it = 0; it < CH * 8 / THREADS; it++) {
       const int c = it * THREADS + (int)threadIdx.x, row = c >> 3, ck = c & 7;
-      uint4 parts[NP];
-#pragma unroll
-      for (int p = 0; p < NP; p++) parts[p] = make_uint4(0, 0, 0, 0);
-      if (row < n && ck * 8 < left) {
-        float v[8];
-        load_vec<T, 8>(base + row * stride + ck * 8, v);
-        split8<NP>(v, parts);
-      }
-#pragma unroll
-      for (int p = 0; p < NP; p++) sts16(dst + p * TILE + swz(row, ck), parts[p]);
+      r[it] = load_raw<T, true>(base + row * stride + ck * 8, row < n ? left - ck * 8 : 0);
     }
-  } else {
-#pragma unroll 1
-    for (int i = threadIdx.x; i < CH * 64; i += THREADS) {
-      const int row = i >> 6, col = i & 63;
-      float v = row < n && col < left ? to_float(base[row * stride + col]) : 0.f;
+  }
+  __device__ __forceinline__ void store(uint32_t dst) const {
 #pragma unroll
-      for (int p = 0; p < NP; p++) {
-        const __nv_bfloat16 h = __float2bfloat16_rn(v);
-        asm volatile("st.shared.b16 [%0], %1;" ::"r"(dst + p * TILE + swz(row, col >> 3) + (col & 7) * 2),
-                     "h"(__bfloat16_as_ushort(h))
-                     : "memory");
-        v -= __bfloat162float(h);
-      }
+    for (int it = 0; it < CH * 8 / THREADS; it++) {
+      const int c = it * THREADS + (int)threadIdx.x, row = c >> 3, ck = c & 7;
+      float v[8];
+      uint4 parts[Parts<T>::N];
+      r[it].to(v);
+      split8<Parts<T>::N>(v, parts);
+#pragma unroll
+      for (int p = 0; p < Parts<T>::N; p++) sts16(dst + p * TILE + swz(row, ck), parts[p]);
+    }
+  }
+};
+template <class T>
+__device__ __noinline__ void load_elements(uint32_t dst, const T* base, long long stride, int n, int left) {
+#pragma unroll 1
+  for (int i = threadIdx.x; i < CH * 64; i += THREADS) {
+    const int row = i >> 6, col = i & 63;
+    float v = row < n && col < left ? to_float(base[row * stride + col]) : 0.f;
+#pragma unroll
+    for (int p = 0; p < Parts<T>::N; p++) {
+      const __nv_bfloat16 h = __float2bfloat16_rn(v);
+      asm volatile("st.shared.b16 [%0], %1;" ::"r"(dst + p * TILE + swz(row, col >> 3) + (col & 7) * 2),
+                   "h"(__bfloat16_as_ushort(h))
+                   : "memory");
+      v -= __bfloat162float(h);
     }
   }
 }
@@ -221,18 +229,31 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
     tc_fence_after();
     return ok;
   };
+  auto first_of = [&](int pos) { return r.reverse ? (long long)len - 1 - pos : (long long)pos; };
+  auto at_tile = [&](const Operand& o, long long first, int d0) {
+    return static_cast<const T*>(o.p) + batch * o.sb + (head / o.per) * o.sh + first * o.st + d0;
+  };
+  Fetch<T> fa, fb, fc;
+  auto fetch = [&](int pos, int s) {  // the tiles of the chunk at pos and slab s
+    const int n = min(CH, len - pos);
+    if (n <= 0) return;
+    const long long first = first_of(pos);
+    if (OUT && r.a.vec) fa.load(at_tile(r.a, first, s * 64), step * r.a.st, n, r.da - s * 64);
+    if (r.b.vec) fb.load(at_tile(r.b, first, s * 64), step * r.b.st, n, r.da - s * 64);
+    if (s == 0 && r.c.vec) fc.load(at_tile(r.c, first, blk * 64), step * r.c.st, n, r.dc - blk * 64);
+  };
+  fetch(p0, 0);
 #pragma unroll 1
   for (int ch = 0; ok && ch < r.chunks; ch++) {
     const int pos = p0 + ch * CH;
     const int n = min(CH, len - pos);
     if (n <= 0) break;
     const bool last = pos + n == len;
-    const long long first = r.reverse ? (long long)len - 1 - pos : pos;
-    auto load = [&](uint32_t dst, const Operand& o, int d0, int d) {
-      const T* base = static_cast<const T*>(o.p) + batch * o.sb + (head / o.per) * o.sh + first * o.st + d0;
-      load_tile<T>(dst, base, step * o.st, n, d - d0, o.vec);
-    };
-    load(smem + PL::C, r.c, blk * 64, r.dc);
+    const long long first = first_of(pos);
+    if (r.c.vec)
+      fc.store(smem + PL::C);
+    else
+      load_elements<T>(smem + PL::C, at_tile(r.c, first, blk * 64), step * r.c.st, n, r.dc - blk * 64);
 #pragma unroll 1
     for (int s = 0; s < r.slabs; s++) {
       float e[16];
@@ -246,9 +267,19 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
 #pragma unroll
           for (int p = 0; p < EP; p++) sts16(smem + PL::E + p * ETILE + swz(srow, (scol >> 3) + h), parts[p]);
         }
-        load(smem + PL::A, r.a, s * 64, r.da);
+        if (r.a.vec)
+          fa.store(smem + PL::A);
+        else
+          load_elements<T>(smem + PL::A, at_tile(r.a, first, s * 64), step * r.a.st, n, r.da - s * 64);
       }
-      load(smem + PL::B, r.b, s * 64, r.da);
+      if (r.b.vec)
+        fb.store(smem + PL::B);
+      else
+        load_elements<T>(smem + PL::B, at_tile(r.b, first, s * 64), step * r.b.st, n, r.da - s * 64);
+      if (s + 1 < r.slabs)
+        fetch(pos, s + 1);
+      else if (ch + 1 < r.chunks)
+        fetch(pos + CH, 0);
       // scores and a E before b's place may be taken by the decayed b
       auto scores = [&] {
         tc_fence_after();

@@ -135,6 +135,30 @@ __device__ __forceinline__ void store_vec(T* p, const float* v) {
   }
 }
 
+// 8 elements of a row as they are in memory.
+template <class T>
+struct alignas(16) Raw8 {
+  T e[8];
+  __device__ __forceinline__ void to(float* v) const {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = to_float(e[i]);
+  }
+};
+template <class T, bool VEC>  // VEC: p is 16-byte aligned, and n is 8 or not positive
+__device__ __forceinline__ Raw8<T> load_raw(const T* p, int n) {
+  Raw8<T> r;
+  if (VEC) {
+    if (n > 0)
+      r = *reinterpret_cast<const Raw8<T>*>(p);
+    else
+      memset(&r, 0, sizeof(r));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) r.e[i] = i < n ? p[i] : from_float<T>(0.f);
+  }
+  return r;
+}
+
 // Pairs of fp32 in one instruction: (x, y) *= (a, b); (x, y) += (a, b);
 // (x, y) = (a, b) * (c, d) + (x, y).  Each element is rounded as by itself.
 __device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {
