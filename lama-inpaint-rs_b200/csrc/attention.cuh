@@ -118,7 +118,7 @@ struct Maps {
   CUtensorMap a, b, c, o;
 };
 bool encode_maps(Run& r, Maps& m);
-cudaError_t launch_pipe(const Run& r, const Maps& m, bool states, cudaStream_t st);
+cudaError_t launch_pipe(const Run& r, const Maps& m, int dtype, bool states, cudaStream_t st);
 
 }  // namespace ops
 }  // namespace lama

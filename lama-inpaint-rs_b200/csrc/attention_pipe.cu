@@ -1,4 +1,4 @@
-// Linear attention over whole sequences for bf16 inputs and outputs with
+// Linear attention over whole sequences for 16-bit inputs and outputs with
 // 16-byte-aligned rows (head sizes are then multiples of 8): the recurrence of linear_attention.cu (roles (a; b, c), S = sum b c^T,
 // out = a S) as one pipeline per CTA.
 //
@@ -21,14 +21,21 @@
 // run forward or, for the gradients of b and c, backward in time (REV: the
 // mask and every power of lam mirrored, the chunks taken last to first).
 //
-// Rounding: P and, where U only feeds the outputs of the same segment, the
+// Rounding (bf16; fp16 below): P and, where U only feeds the outputs of the same segment, the
 // decayed b to one bf16 part (both errors are of the size of the output's own
 // rounding and do not add up on one term), E to two.  The states that segments
 // hand on, and the final state, come from the kernel without outputs, with the
 // decayed b in three parts (24 bits): they are fp32 results.  So a final state
 // costs a pass over b and c, and outputs do not depend on asking for it.
 //
+// fp16 has 3 more bits and a narrow range, so what the kernel rounds to it is
+// scaled by powers of two first: the rows of P by the row's largest score, the
+// columns of E by the column's largest entry, b~ by 2^8 where that fits; two
+// parts of b~ (22 bits) make the states.
+//
 // TMEM: two chunks' S (128 columns, P over them) and O (64), and U.
+#include <type_traits>
+
 #include "attention.cuh"
 
 namespace lama {
@@ -38,9 +45,9 @@ namespace {
 
 constexpr int THREADS = 14 * 32;  // 4 warps a scheduler at most: 128 registers a thread
 
-template <int NS, bool OUT>
+template <class T, int NS, bool OUT>
 struct Lay {
-  static constexpr int UP = OUT ? 1 : 3;  // parts of b~
+  static constexpr int UP = OUT ? 1 : std::is_same_v<T, __half> ? 2 : 3;  // parts of b~
   // stages of (a, b), free once S and a E are made, and of c, free after P c;
   // buffers of b~ and of U, and of E
   static constexpr int AS = OUT ? (NS == 1 ? 3 : 2) : (NS == 1 ? 4 : 2), CS = OUT ? (NS == 1 ? 4 : 2) : (NS == 1 ? 4 : 3);
@@ -64,6 +71,53 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int c
       " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
       "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(a, b);
+  }
+}
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+  if constexpr (std::is_same_v<T, __half>)
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+  else
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));  // bf16: the upper half of an fp32
+}
+template <class T>
+__device__ __forceinline__ void unpack8(uint4 x, float* v) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float2 f = unpack2<T>(w[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+// v[0..7] into N parts of type T
+template <int N, class T>
+__device__ __forceinline__ void split8(const float* v, uint4* out) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) r[i] = v[i];
+#pragma unroll
+  for (int p = 0; p < N; p++) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      w[i] = pack2<T>(r[2 * i], r[2 * i + 1]);
+      if (p + 1 < N) {
+        const float2 h = unpack2<T>(w[i]);
+        r[2 * i] -= h.x;
+        r[2 * i + 1] -= h.y;
+      }
+    }
+    out[p] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // A from TMEM (128 lanes, two 16-bit elements a column), B from shared memory
@@ -92,20 +146,25 @@ __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t phase, int* err, i
   return mbar_wait(bar, phase, err, code);
 }
 
-template <int NS, bool OUT, bool REV>
+template <class T, int NS, bool OUT, bool REV>
 __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run r,
                                                         const __grid_constant__ Maps maps, int segs) {
-  using L = Lay<NS, OUT>;
+  using L = Lay<T, NS, OUT>;
   constexpr int UP = L::UP;
+  constexpr bool HALF = std::is_same_v<T, __half>;
   // Results leave through the stage that held c (one TMA store a chunk; per-row
   // stores kept the load/store unit busy: 70 -> 59 us at 128 x 4096 tokens of
   // 64).  With two slabs c has two stages only, and holding them longer costs
   // more (195 -> 213 us): there the rows are stored directly.
   constexpr bool STAGED_OUT = NS == 1;
-  using T = __nv_bfloat16;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(16) float pw[CH + 4];
-  __shared__ float pi[CH];  // intra lam^i
+  // fp16: factors 2^e of the columns of E (bf16, chunk c in row c % 4: a group is done with its chunk
+  // before E of the fourth next is made), exponents on their way between threads, 1 / the scale of b~
+  // (chunk c in entry c % 4: b~ is made at most three chunks ahead of the states)
+  __shared__ __align__(16) uint16_t ef[HALF && OUT ? 4 : 1][64];
+  __shared__ uint8_t ex[HALF && OUT ? 128 : 1];
+  __shared__ float bs[HALF ? 4 : 1];
   __shared__ __align__(16) float rv[32];  // lam^{31-j}
   __shared__ Bars bars;
   __shared__ uint32_t tmem_slot;
@@ -151,10 +210,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
     }
     fence_mbar_init();
   }
-  for (int i = tid; i <= CH; i += THREADS) {
-    pw[i] = power(g, i);
-    if (i < CH) pi[i] = r.intra * pw[i];
-  }
+  for (int i = tid; i <= CH; i += THREADS) pw[i] = power(g, i);
   for (int i = tid; i < 32; i += THREADS) rv[i] = power(g, 31 - i);
   tc_fence_before();
   __syncthreads();
@@ -186,9 +242,25 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
         if ((int)((i >> 3) & 127) >= n) sts16(i < L::AB / 16 ? ab + i * 16 : ct + (i - L::AB / 16) * 16, make_uint4(0, 0, 0, 0));
     }
     // a batch's loads go out before its first use: loads and stores of shared memory stay in program order
-    constexpr int BATCH = UP == 1 ? 8 : 4;
+    constexpr int BATCH = UP == 1 ? 8 : 4, ALL = NS * CH * 8 / TH;
+    float up = 1.f;
+    if (HALF) {
+      // b~ = b lam^m may leave fp16's normal numbers at the lower end: where no |b| reaches 2^8, it is made 2^8 times as large
+      uint32_t top = 0;
+#pragma unroll 8
+      for (int i = 0; i < ALL; i++) {
+        const int k = i * (TH / 8) + (t >> 3);
+        uint4 x = lds16(src + (k >> 7) * TILE + swz(k & (CH - 1), ck));
+        if ((k & (CH - 1)) >= n) x = make_uint4(0, 0, 0, 0);
+        top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                                     __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+      }
+      const uint32_t most = max(top & 0xffffu, top >> 16);
+      if (named_sync_and(3, TH, most < 0x5c00u)) up = 256.f;  // 0x5c00: 2^8
+      if (t == 0) bs[c & 3] = 1.f / up;
+    }
 #pragma unroll 1
-    for (int i0 = 0; i0 < NS * CH * 8 / TH; i0 += BATCH) {
+    for (int i0 = 0; i0 < ALL; i0 += BATCH) {
       uint4 x[BATCH];
       float w[BATCH];
 #pragma unroll
@@ -196,21 +268,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
         const int k = (i0 + i) * (TH / 8) + (t >> 3), j = k & (CH - 1);  // the slabs' rows one after another
         x[i] = lds16(src + (k >> 7) * TILE + swz(j, ck));
         w[i] = pw[REV ? j : max(n - 1 - j, 0)];
+        if (HALF) w[i] *= up;
       }
 #pragma unroll
       for (int i = 0; i < BATCH; i++) {
         const int k = (i0 + i) * (TH / 8) + (t >> 3), j = k & (CH - 1);
         if (j >= n) x[i] = make_uint4(0, 0, 0, 0);
-        const uint32_t* e = reinterpret_cast<const uint32_t*>(&x[i]);
         float v[8];
+        unpack8<T>(x[i], v);
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          v[2 * q] = __uint_as_float(e[q] << 16);  // bf16 is the upper half of an fp32
-          v[2 * q + 1] = __uint_as_float(e[q] & 0xffff0000u);
-          mul2(v[2 * q], v[2 * q + 1], w[i], w[i]);
-        }
+        for (int q = 0; q < 8; q += 2) mul2(v[q], v[q + 1], w[i], w[i]);
         uint4 parts[UP];
-        split8<UP>(v, parts);
+        split8<UP, T>(v, parts);
 #pragma unroll
         for (int p = 0; p < UP; p++) sts16(dst + (p * NS + (k >> 7)) * TILE + swz(j, ck), parts[p]);
       }
@@ -283,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
       if (!wait(bars.u, L::KB, c, 12)) return false;
       tc_fence_after();
       const float d = pw[num(c) - 1], f = c + 1 < live ? lam : 1.f;
-      const float fe = f * d, fu = f * r.update;
+      const float fe = f * d, fu = f * r.update * (HALF ? bs[c & 3] : 1.f);
 #pragma unroll
       for (int i = 0; i < W; i += 32) {
         float u[32];
@@ -310,10 +379,29 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
         // E's buffer is free once the products of chunk c - ES are done
         if (c >= L::ES && !(ok = __all_sync(~0u, wait(bars.s, 2, c - L::ES, 14)))) break;
         const uint32_t eb = smem + L::E + (c % L::ES) * L::E_BUF;
+        float fe = 1.f;
+        if (HALF) {
+          // E in fp16's range: the row's largest magnitude (the other half's thread has a say) to 2^14..2^15
+          float m = 0.f;
+#pragma unroll
+          for (int i = 0; i < W; i++) m = fmaxf(m, fabsf(E[i]));
+          ex[t] = (uint8_t)(__float_as_uint(m) >> 23);
+          named_sync(4, 128);
+          const int e = max((int)max(ex[t], ex[t ^ 64]), 28);  // below 2^-99 as zero
+          fe = __uint_as_float((uint32_t)(268 - min(e, 254)) << 23);   // 2^(14 - (e - 127))
+          if (half == 0) ef[c & 3][t] = (uint16_t)((uint32_t)(min(e, 254) - 14) << 7);  // 1 / fe, as bf16
+          named_sync(4, 128);
+        }
 #pragma unroll
         for (int i = 0; i < W; i += 8) {
           uint4 parts[2];
-          split8<2>(E + i, parts);
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) x[j] = E[i + j];
+          if (HALF)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) mul2(x[j], x[j + 1], fe, fe);
+          split8<2, T>(x, parts);
           const int er = half * W + i;
 #pragma unroll
           for (int p = 0; p < 2; p++) sts16(eb + (p * NS + (er >> 6)) * ETILE + swz(t & 63, (er & 63) >> 3), parts[p]);
@@ -334,8 +422,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
     // on the lane number the compiler takes 88 clocks an MMA, elected 51 (what
     // 128 x 64 x 16 from shared memory takes).
     const bool leader = elect_one();
-    constexpr uint32_t ID_U = idesc_bf16_f32(64 * NS) | A_MN | B_MN, ID_S = idesc_bf16_f32(128),
-                       ID_E = idesc_bf16_f32(64), ID_P = idesc_bf16_f32(64) | B_MN;
+    constexpr uint32_t F = HALF ? (1u << 7) | (1u << 10) : 0;  // the format fields: 1 bf16, 0 fp16
+    constexpr uint32_t ID_U = (idesc_bf16_f32(64 * NS) ^ F) | A_MN | B_MN, ID_S = idesc_bf16_f32(128) ^ F,
+                       ID_E = idesc_bf16_f32(64) ^ F, ID_P = (idesc_bf16_f32(64) ^ F) | B_MN;
     bool ok = true;
     auto ready = [&](uint64_t* set, int n, int c, int code) {
       ok = __all_sync(~0u, wait(set, n, c, code));
@@ -434,6 +523,26 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
       if (!(ok = __all_sync(~0u, wait(bars.s, 2, c, 19)))) break;
       tc_fence_after();
       const int n = num(c);
+      float rowf = r.intra, back = 1.f;  // factors of the row's scores, and of its results
+      if (HALF) {
+        // P in fp16's range: the row's largest score (masked ones included, an
+        // upper bound does: fp16 keeps its precision over 2^28) to at most 2^14
+        float m = 0.f;
+#pragma unroll 1
+        for (int h = 0; h < 2; h++) {
+          if (!(REV ? 2 * h + 1 >= rb : 2 * h <= rb)) continue;
+          float v[64];
+          tmem_ld32(t + h * 64, v);
+          tmem_ld32(t + h * 64 + 32, v + 32);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 64; i++) m = fmaxf(m, fabsf(v[i]));
+        }
+        const int e = (int)(__float_as_uint(m * fabsf(r.intra)) >> 23);
+        const int shift = min(max(e - 127 - 13, -24), 40);
+        rowf *= __uint_as_float((uint32_t)(127 - shift) << 23);
+        back = __uint_as_float((uint32_t)(127 + shift) << 23);
+      }
 #pragma unroll 1
       for (int h = 0; h < 2; h++) {
         float v[64];
@@ -457,10 +566,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
 #pragma unroll
             for (int j = 0; j < 32; j++) {
               const int d = REV ? j - lane : lane - j;
-              x[j] = d >= 0 ? x[j] * pi[max(d, 0)] : 0.f;
+              x[j] = d >= 0 ? x[j] * (rowf * pw[max(d, 0)]) : 0.f;
             }
           } else {
-            const float base = pi[REV ? b * 32 - row : row - b * 32 - 31];
+            const float base = rowf * pw[REV ? b * 32 - row : row - b * 32 - 31];
             const float4* f = reinterpret_cast<const float4*>(REV ? pw : rv);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -472,13 +581,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
             }
           }
 #pragma unroll
-          for (int i = 0; i < 16; i++) w[k * 16 + i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+          for (int i = 0; i < 16; i++) w[k * 16 + i] = pack2<T>(x[2 * i], x[2 * i + 1]);
         }
         tmem_st16(t + h * 32, w);  // over columns already read
         tmem_st16(t + h * 32 + 16, w + 16);
       }
       const int dist = REV ? n - 1 - row : row;
-      const float di = dist >= 0 ? r.inter * pw[dist] : 0.f;
+      float di = dist >= 0 ? r.inter * pw[dist] : 0.f;
+      if (HALF) di *= 1.f / back;
 #pragma unroll 1
       for (int h = 0; h < 2; h++) {
         float v[32];
@@ -488,6 +598,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           mul2(v[i], v[i + 1], di, di);
+          if (HALF) {
+            const uint32_t f = *reinterpret_cast<const uint32_t*>(&ef[c & 3][h * 32 + i]);
+            mul2(v[i], v[i + 1], __uint_as_float(f << 16), __uint_as_float(f & 0xffff0000u));
+          }
           w[i] = __float_as_uint(v[i]);
           w[i + 1] = __float_as_uint(v[i + 1]);
         }
@@ -511,6 +625,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
           tc_fence_before();
           arrive(bars.oe, 2, c);
         }
+        if (HALF)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) mul2(v[i], v[i + 1], back, back);
         if (row >= n)
 #pragma unroll
           for (int i = 0; i < 32; i++) v[i] = 0.f;
@@ -530,7 +647,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             uint4 x;
-            split8<1>(v + i * 8, &x);
+            split8<1, T>(v + i * 8, &x);
             sts16(ct + swz(row, h * 4 + i), x);
           }
         }
@@ -571,23 +688,28 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
   }
 }
 
-template <int NS, bool OUT, bool REV>
+template <class T, int NS, bool OUT, bool REV>
 cudaError_t launch(const Run& r, const Maps& maps, int segs, cudaStream_t st) {
-  constexpr int bytes = Lay<NS, OUT>::BYTES + 1024;
+  constexpr int bytes = Lay<T, NS, OUT>::BYTES + 1024;
   static_assert(bytes + 2048 <= 227 * 1024, "shared memory");
   static SmemLimit limit;
-  const cudaError_t ce = limit.reach(k_pipe<NS, OUT, REV>, bytes);
+  const cudaError_t ce = limit.reach(k_pipe<T, NS, OUT, REV>, bytes);
   if (ce != cudaSuccess) return ce;
   const long long grid = (long long)r.batch * r.heads * r.blocks * segs;
-  k_pipe<NS, OUT, REV><<<(unsigned)grid, THREADS, bytes, st>>>(r, maps, segs);
+  k_pipe<T, NS, OUT, REV><<<(unsigned)grid, THREADS, bytes, st>>>(r, maps, segs);
   return cudaGetLastError();
 }
 
-template <int NS, bool REV>
+template <class T, int NS, bool REV>
 cudaError_t launch(const Run& r, const Maps& m, bool states, cudaStream_t st) {
   if (states)  // the last segment's state is needed only where the final state is
-    return launch<NS, false, REV>(r, m, r.fin ? r.nseg : r.nseg - 1, st);
-  return launch<NS, true, REV>(r, m, r.nseg, st);
+    return launch<T, NS, false, REV>(r, m, r.fin ? r.nseg : r.nseg - 1, st);
+  return launch<T, NS, true, REV>(r, m, r.nseg, st);
+}
+template <class T>
+cudaError_t launch(const Run& r, const Maps& m, bool states, cudaStream_t st) {
+  if (r.slabs == 1) return r.reverse ? launch<T, 1, true>(r, m, states, st) : launch<T, 1, false>(r, m, states, st);
+  return r.reverse ? launch<T, 2, true>(r, m, states, st) : launch<T, 2, false>(r, m, states, st);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -630,9 +752,8 @@ bool encode_maps(Run& r, Maps& m) {
   return (r.oh != 0 || r.heads == 1) && (r.ob != 0 || r.batch == 1) && encode(&m.o, o, r, r.dc);
 }
 
-cudaError_t launch_pipe(const Run& r, const Maps& m, bool states, cudaStream_t st) {
-  if (r.slabs == 1) return r.reverse ? launch<1, true>(r, m, states, st) : launch<1, false>(r, m, states, st);
-  return r.reverse ? launch<2, true>(r, m, states, st) : launch<2, false>(r, m, states, st);
+cudaError_t launch_pipe(const Run& r, const Maps& m, int dtype, bool states, cudaStream_t st) {
+  return dtype == LAMA_F16 ? launch<__half>(r, m, states, st) : launch<__nv_bfloat16>(r, m, states, st);
 }
 
 }  // namespace ops

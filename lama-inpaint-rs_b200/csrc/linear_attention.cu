@@ -543,7 +543,7 @@ cudaError_t launch_chunks(const Run& r, cudaStream_t st) {
 
 // How a sequence is cut: one segment reads everything once, several read b
 // and c twice but fill the GPU.  Takes the least time on the busiest SM,
-// counted in chunk steps.  Pipelined (bf16): a CTA costs 4 beside its chunks
+// counted in chunk steps.  Pipelined (16-bit types): a CTA costs 4 beside its chunks
 // (set-up, the first loads, the last products), the pass that makes the
 // states 0.6 a chunk and, with the scan, two launches of 3 each.  The other
 // kernel's steps are several times longer and do not overlap.
@@ -574,28 +574,30 @@ long long seg_bytes(const lama_attention* p, int da, int dc) {
   Run r{};
   r.batch = p->batch, r.heads = p->heads, r.tokens = p->tokens;
   r.slabs = (da + 63) / 64, r.blocks = (dc + 63) / 64;
-  cut(r, p->dtype == LAMA_BF16);
-  if (!r.staged && p->dtype != LAMA_BF16) return 0;
+  cut(r, p->dtype != LAMA_F32);
+  if (!r.staged && p->dtype == LAMA_F32) return 0;
   return (long long)r.batch * r.heads * r.nseg * r.slabs * 64 * r.blocks * 64 * 4;
 }
 
 template <class T>
-cudaError_t go(Run& r, cudaStream_t st) {
+cudaError_t go(Run& r, int dtype, cudaStream_t st) {
   cudaError_t ce = cudaSuccess;
   Maps maps;
-  r.pipe = std::is_same_v<T, __nv_bfloat16> && r.a.vec && r.b.vec && r.c.vec && r.out_vec && encode_maps(r, maps);
+  r.pipe = dtype != LAMA_F32 && r.a.vec && r.b.vec && r.c.vec && r.out_vec && encode_maps(r, maps);
   if (r.pipe && r.fin) r.staged = 1;
   if (r.staged) {
-    if ((ce = r.pipe ? launch_pipe(r, maps, true, st) : launch_chunks<T, false>(r, st)) != cudaSuccess) return ce;
+    if ((ce = r.pipe ? launch_pipe(r, maps, dtype, true, st) : launch_chunks<T, false>(r, st)) != cudaSuccess) return ce;
     const int per = r.slabs * 64 * r.blocks * 64;
     k_scan<<<dim3((per + 255) / 256, r.batch * r.heads), 256, 0, st>>>(r);
     if ((ce = cudaGetLastError()) != cudaSuccess) return ce;
   }
-  return r.pipe ? launch_pipe(r, maps, false, st) : launch_chunks<T, true>(r, st);
+  return r.pipe ? launch_pipe(r, maps, dtype, false, st) : launch_chunks<T, true>(r, st);
 }
 
-cudaError_t go(Run& r, int dtype, cudaStream_t st) {
-  return dtype == LAMA_F32 ? go<float>(r, st) : dtype == LAMA_F16 ? go<__half>(r, st) : go<__nv_bfloat16>(r, st);
+cudaError_t run(Run& r, int dtype, cudaStream_t st) {
+  return dtype == LAMA_F32   ? go<float>(r, dtype, st)
+         : dtype == LAMA_F16 ? go<__half>(r, dtype, st)
+                             : go<__nv_bfloat16>(r, dtype, st);
 }
 
 Operand operand(const lama_rows& x, int heads, int d, int dtype) {
@@ -629,7 +631,7 @@ void roles(Run& r, const Operand& a, const Operand& b, const Operand& c, int da,
   r.dc = dc;
   r.slabs = (da + 63) / 64;
   r.blocks = (dc + 63) / 64;
-  cut(r, dtype == LAMA_BF16);
+  cut(r, dtype != LAMA_F32);
 }
 
 const char* check_rows(const lama_rows& x, const lama_attention* p, const char* what, char* buf, size_t n) {
@@ -766,7 +768,7 @@ extern "C" int lama_linear_attention(const lama_attention* p, const lama_rows* o
   output(r, *out, p->dv, p->dtype);
   r.seg = static_cast<float*>(workspace);
   if (ce == cudaSuccess) ce = status_word(&r.status);
-  if (ce == cudaSuccess) ce = go(r, p->dtype, (cudaStream_t)stream);
+  if (ce == cudaSuccess) ce = run(r, p->dtype, (cudaStream_t)stream);
   if (ce != cudaSuccess) return fail(err, err_len, LAMA_ECUDA, "linear attention: %s", cudaGetErrorString(ce));
   return LAMA_OK;
 }
@@ -803,7 +805,7 @@ extern "C" int lama_linear_attention_backward(const lama_attention* p, const lam
     r.status = status;
     if (o.heads == p->heads) {
       output(r, o, d, p->dtype);
-      ce = go(r, p->dtype, st);
+      ce = run(r, p->dtype, st);
     } else {
       r.out = shared;
       r.out_f32 = 1;
@@ -811,7 +813,7 @@ extern "C" int lama_linear_attention_backward(const lama_attention* p, const lam
       r.ot = (long long)p->heads * d;
       r.ob = r.ot * p->tokens;
       r.out_vec = d % 8 == 0;
-      ce = go(r, p->dtype, st);
+      ce = run(r, p->dtype, st);
       if (ce != cudaSuccess) break;
       const long long n = (long long)p->batch * p->tokens;
       const int per = p->heads / o.heads;

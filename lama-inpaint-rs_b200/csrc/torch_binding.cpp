@@ -172,14 +172,14 @@ double number(PyObject* o, const char* name) {
 // ------------------------------------------------------------------ linear attention
 
 // The tensor itself where the kernels take its strides at full speed, else a
-// contiguous copy: rows have to be contiguous, and bfloat16 rows of a multiple
+// contiguous copy: rows have to be contiguous, and 16-bit rows of a multiple
 // of 8 channels on 16-byte boundaries (the copy then goes through the same
 // kernel as a contiguous tensor, to the same bits).
 Tensor unit(const Tensor& t, bool whole) {
   const auto n = t.sizes(), s = t.strides();
   const size_t d = n.size() - 1;
   if (s[d] != 1 && n[d] != 1) return t.contiguous();
-  if (whole && t.scalar_type() == at::kBFloat16 && n[d] % 8 == 0) {
+  if (whole && t.scalar_type() != at::kFloat && n[d] % 8 == 0) {
     if (n[1] > 1 && s[1] == 0) return t.contiguous();
     bool fits = ((uintptr_t)t.data_ptr() & 15) == 0;
     for (size_t i = 0; i < d; i++) fits = fits && (s[i] % 8 == 0 || n[i] <= 1);
