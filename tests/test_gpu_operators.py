@@ -595,3 +595,88 @@ def test_norm_of_zeros_and_of_nothing(F):
     u, n, saved = F.gated_residual_norm(e, e, post_weight=w, pre_weight=w, save="full")
     g = F.gated_residual_norm_backward(e, e, saved)
     assert g.x.shape == (0, 64) and not g.pre_weight.any()
+
+
+# ------------------------------------------------------------------ without the final state, and refusals
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (128, 64), (64, 128)])
+def test_long_sequences_cut_into_segments_without_a_final_state(F, dtype, dk, dv):
+    """Few heads and many tokens: the states of segments are made and scanned, forward and backward."""
+    g = gen(31)
+    q, k, v, go = (randn(g, 1, 3000, 2, d, dtype=dtype) for d in (dk, dk, dv, dv))
+    ld, scale = decays(2), dk ** -0.5
+    o = F.linear_attention(q, k, v, ld)
+    eo, _ = attention64(q, k, v, ld, scale)
+    mo, _ = attention64(q, k, v, ld, scale, absolute=True)
+    close(o, eo, bound(dtype, 3000, mo), "o")
+    assert torch.equal(o, F.linear_attention(q, k, v, ld, return_state=True)[0])
+    got = F.linear_attention_backward(go, q, k, v, ld)
+    exp, maj = attention64(q, k, v, ld, scale, None, None, go), attention64(q, k, v, ld, scale, None, None, go, absolute=True)
+    for n, a, e, m in zip(("dq", "dk", "dv"), got, exp, maj):
+        close(a, e, bound(dtype, 3000, m, 2), n)
+    F.check_operators()
+
+
+@pytest.mark.parametrize("size", [1e-3, 1.0, 200.0])
+def test_fp16_sizes(F, size):
+    """Inputs far from 1 on either side: the powers of two that bring them into fp16's range cost no precision."""
+    g = gen(33)
+    q, k = (randn(g, 1, 500, 2, 64) * size).half(), (randn(g, 1, 500, 2, 64) * size).half()
+    v = (randn(g, 1, 500, 2, 64) * min(1.0, 1 / size)).half()
+    ld, scale = decays(2), 0.125
+    o, s = F.linear_attention(q, k, v, ld, return_state=True)
+    eo, es = attention64(q, k, v, ld, scale)
+    mo, ms = attention64(q, k, v, ld, scale, absolute=True)
+    close(o, eo, bound(torch.float16, 500, mo) + 2.0 ** -25, "o")  # 2^-25: half of fp16's smallest number
+    close(s, es, state_bound(500, ms), "state")
+
+
+def test_refusals_of_tensors(F):
+    from lama_b200 import LamaError
+    z = torch.zeros(1, 4, 2, 64, device="cuda", dtype=torch.bfloat16)
+    ld = torch.zeros(2, device="cuda")
+    st = torch.zeros(1, 2, 64, 64, device="cuda")
+    x = torch.zeros(2, 3, 8, device="cuda")
+    w = torch.ones(8, device="cuda")
+    cases = [
+        (lambda: F.linear_attention(z, z.half(), z, ld), "k has type"),
+        (lambda: F.linear_attention(z.int(), z, z, ld), "has type"),
+        (lambda: F.linear_attention(z[0], z, z, ld), "dimensions"),
+        (lambda: F.linear_attention(z, z[:, :3], z, ld), "does not go with"),
+        (lambda: F.linear_attention(z, z[..., :8], z, ld), "channels a head"),
+        (lambda: F.linear_attention(z, z, z, torch.zeros(3, device="cuda")), "do not divide"),
+        (lambda: F.linear_attention(z, z, z, ld.cpu()), "log_decay is on cpu"),
+        (lambda: F.linear_attention(z, z, z, ld.clone().requires_grad_()), "no gradient"),
+        (lambda: F.linear_attention(z, z, z, ld, initial_state=st[:, :1]), "initial_state has shape"),
+        (lambda: F.linear_attention(z, z, z, ld, lengths=torch.zeros(1, device="cuda")), "lengths has type"),
+        (lambda: F.linear_attention(z, z, z, ld, scale="a"), "not a number"),
+        (lambda: F.linear_attention(torch.zeros(1, 4, 2, 129, device="cuda"), torch.zeros(1, 4, 2, 129, device="cuda"),
+                                    torch.zeros(1, 4, 2, 64, device="cuda"), ld), "1..128"),
+        (lambda: F.linear_attention_backward(z[:, :3], z, z, z, ld), "grad_o has shape"),
+        (lambda: F.linear_attention_step(z[:, 0], z[:, 0], z[:, 0], ld, st[..., :32]), "state is not a contiguous"),
+        (lambda: F.linear_attention_step(z[:, 0], z[:, 0], z[:, 0], ld, st, out_state=st[0]), "out_state has shape"),
+        (lambda: F.linear_attention_step(z[:, 0], z[:, 0], z[:, 0], ld, st, slots=torch.zeros(2, device="cuda",
+                                                                                         dtype=torch.int32)), "slots has shape"),
+        (lambda: F.linear_attention_step(z[:, 0].expand(2, 2, 64), z[:, 0].expand(2, 2, 64), z[:, 0].expand(2, 2, 64), ld, st),
+         "1 states for 2 rows"),
+        (lambda: F.linear_attention_step(z[:, 0].clone().requires_grad_(), z[:, 0], z[:, 0], ld, st), "no gradient"),
+        (lambda: F.gated_residual_norm(x, x[:1]), "y has shape"),
+        (lambda: F.gated_residual_norm(x, x.half()), "y has type"),
+        (lambda: F.gated_residual_norm(x, x, post_weight=w[:4]), "post_weight is not"),
+        (lambda: F.gated_residual_norm(x, x, gate=x[:, :2]), "does not broadcast"),
+        (lambda: F.gated_residual_norm(x, x, gate=x[:1]), "expand it"),
+        (lambda: F.gated_residual_norm(x, x, gate=x.half()), "gate has type"),
+        (lambda: F.gated_residual_norm(x, x, residual_scale=w[:3]), "residual_scale is not"),
+        (lambda: F.gated_residual_norm(x, x, eps=-1), "eps"),
+        (lambda: F.checkpoint_store(x.int()), "has type"),
+        (lambda: F.checkpoint_restore(F.Checkpoint8(x.to(torch.int8), x, torch.float32)), "scales has shape"),
+    ]
+    for f, msg in cases:
+        with pytest.raises(LamaError) as ex:
+            f()
+        assert ex.value.code == -1 and msg in ex.value.msg, (msg, ex.value.msg)
+    _, _, saved = F.gated_residual_norm(x, x, pre_weight=w, save="full")
+    with pytest.raises(LamaError):
+        F.gated_residual_norm_backward(x[:1], None, saved)
+    F.check_operators()
