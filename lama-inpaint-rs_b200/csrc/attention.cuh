@@ -35,7 +35,8 @@ struct Run {
   const float* init;  // [batch][heads] of [da][dc], element (r, c) at r * ir + c * ic
   float* fin;
   long long ir, ic, fr, fc;
-  float* seg;  // [batch*heads][nseg][slabs*64][blocks*64]: states of the segments
+  float* seg;  // [batch*heads][nseg][slabs*64][blocks*64]: states of the segments, element (r, c) of one
+  long long sr, sc;  // at r * sr + c * sc (another run's states may be read transposed)
   int* status;
   float inter, intra, update;  // scales of a E, of the scores, of b c^T
   int batch, tokens, heads, da, dc;
@@ -111,14 +112,37 @@ __device__ __forceinline__ void store_row(T* dst, const float* v, int left, int 
 
 constexpr uint32_t A_MN = 1u << 15, B_MN = 1u << 16;
 
-// The pipelined kernel of attention_pipe.cu.  encode_maps: false where TMA
-// cannot address the operands.  `states`: only the states that the segments
-// add, into r.seg.
+// Runs that go through the kernels together, one after another in the grid:
+// up to three of one sequence length, cut alike.
 struct Maps {
   CUtensorMap a, b, c, o;
 };
+struct Set {
+  Run run[3];
+  Maps maps[3];
+  int n;
+};
+// The run of this CTA; `id` becomes its number within the run.
+__device__ __forceinline__ int run_of(const Set& set, int segs, int& id) {
+  int w = 0;
+  for (; w + 1 < set.n; w++) {
+    const int n = set.run[w].batch * set.run[w].heads * set.run[w].blocks * segs;
+    if (id < n) break;
+    id -= n;
+  }
+  return w;
+}
+inline long long ctas(const Set& set, int segs) {
+  long long n = 0;
+  for (int w = 0; w < set.n; w++) n += (long long)set.run[w].batch * set.run[w].heads * set.run[w].blocks * segs;
+  return n;
+}
+
+// The pipelined kernel of attention_pipe.cu.  encode_maps: false where TMA
+// cannot address the operands.  The runs of a set have one direction and one
+// number of slabs.  `states`: only the states that the segments add, into seg.
 bool encode_maps(Run& r, Maps& m);
-cudaError_t launch_pipe(const Run& r, const Maps& m, int dtype, bool states, cudaStream_t st);
+cudaError_t launch_pipe(const Set& set, int dtype, bool states, cudaStream_t st);
 
 }  // namespace ops
 }  // namespace lama

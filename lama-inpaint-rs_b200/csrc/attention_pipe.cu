@@ -147,8 +147,7 @@ __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t phase, int* err, i
 }
 
 template <class T, int NS, bool OUT, bool REV>
-__global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run r,
-                                                        const __grid_constant__ Maps maps, int segs) {
+__global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set set, int segs) {
   using L = Lay<T, NS, OUT>;
   constexpr int UP = L::UP;
   constexpr bool HALF = std::is_same_v<T, __half>;
@@ -172,24 +171,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
   const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  int id = blockIdx.x;
-  const int slot = id % segs;  // in the order of the recurrence
-  id /= segs;
-  const int blk = id % r.blocks;
-  id /= r.blocks;
-  const int head = id % r.heads, batch = id / r.heads;
-  const float g = r.log_decay[head];
-  int len = r.tokens;
-  if (r.lengths) len = min(max(r.lengths[batch], 0), r.tokens);
-  const int seg_tokens = r.chunks * CH;
-  const int seg = REV ? r.nseg - 1 - slot : slot;
-  const int p0 = seg * seg_tokens;
-  const int mine = min(max(len - p0, 0), seg_tokens);  // tokens of this segment
-  const int live = (mine + CH - 1) / CH;
-  // the c-th chunk of the recurrence starts at token p0 + at(c) and has num(c) tokens
-  auto at = [&](int c) { return (REV ? live - 1 - c : c) * CH; };
-  auto num = [&](int c) { return min(CH, mine - at(c)); };
-
+  pdl_launch_dependents();
   if (warp == 0) tmem_alloc(smem_u32(&tmem_slot), 512);
   if (tid == 32) {
     failed = 0;
@@ -210,6 +192,29 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
     }
     fence_mbar_init();
   }
+  pdl_wait();
+
+  int id = blockIdx.x;
+  const int which = run_of(set, segs, id);
+  const Run& r = set.run[which];
+  const Maps& maps = set.maps[which];
+  const int slot = id % segs;  // in the order of the recurrence
+  id /= segs;
+  const int blk = id % r.blocks;
+  id /= r.blocks;
+  const int head = id % r.heads, batch = id / r.heads;
+  const float g = r.log_decay[head];
+  int len = r.tokens;
+  if (r.lengths) len = min(max(r.lengths[batch], 0), r.tokens);
+  const int seg_tokens = r.chunks * CH;
+  const int seg = REV ? r.nseg - 1 - slot : slot;
+  const int p0 = seg * seg_tokens;
+  const int mine = min(max(len - p0, 0), seg_tokens);  // tokens of this segment
+  const int live = (mine + CH - 1) / CH;
+  // the c-th chunk of the recurrence starts at token p0 + at(c) and has num(c) tokens
+  auto at = [&](int c) { return (REV ? live - 1 - c : c) * CH; };
+  auto num = [&](int c) { return min(CH, mine - at(c)); };
+
   for (int i = tid; i <= CH; i += THREADS) pw[i] = power(g, i);
   for (int i = tid; i < 32; i += THREADS) rv[i] = power(g, 31 - i);
   tc_fence_before();
@@ -335,8 +340,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
       int rows = 0;  // of this thread's state rows, how many are read
       float f = 1.f;
       if (OUT && r.staged) {
-        src = r.seg + ((bh * r.nseg + slot) * (NS * 64) + half * W) * (r.blocks * 64) + ec;
-        step = r.blocks * 64;
+        src = r.seg + (bh * r.nseg + slot) * (NS * 64 * r.blocks * 64) + half * W * r.sr + ec * r.sc;
+        step = r.sr;
         rows = W;
       } else if (OUT && r.init && ec < r.dc) {
         src = r.init + bh * r.da * r.dc + half * W * r.ir + ec * r.ic;
@@ -689,27 +694,27 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Run
 }
 
 template <class T, int NS, bool OUT, bool REV>
-cudaError_t launch(const Run& r, const Maps& maps, int segs, cudaStream_t st) {
+cudaError_t launch(const Set& set, int segs, cudaStream_t st) {
   constexpr int bytes = Lay<T, NS, OUT>::BYTES + 1024;
   static_assert(bytes + 2048 <= 227 * 1024, "shared memory");
   static SmemLimit limit;
   const cudaError_t ce = limit.reach(k_pipe<T, NS, OUT, REV>, bytes);
   if (ce != cudaSuccess) return ce;
-  const long long grid = (long long)r.batch * r.heads * r.blocks * segs;
-  k_pipe<T, NS, OUT, REV><<<(unsigned)grid, THREADS, bytes, st>>>(r, maps, segs);
-  return cudaGetLastError();
+  return launch_chained(k_pipe<T, NS, OUT, REV>, dim3((unsigned)ctas(set, segs)), THREADS, bytes, st, set, segs);
 }
 
 template <class T, int NS, bool REV>
-cudaError_t launch(const Run& r, const Maps& m, bool states, cudaStream_t st) {
+cudaError_t launch(const Set& set, bool states, cudaStream_t st) {
+  const Run& r = set.run[0];
   if (states)  // the last segment's state is needed only where the final state is
-    return launch<T, NS, false, REV>(r, m, r.fin ? r.nseg : r.nseg - 1, st);
-  return launch<T, NS, true, REV>(r, m, r.nseg, st);
+    return launch<T, NS, false, REV>(set, r.fin ? r.nseg : r.nseg - 1, st);
+  return launch<T, NS, true, REV>(set, r.nseg, st);
 }
 template <class T>
-cudaError_t launch(const Run& r, const Maps& m, bool states, cudaStream_t st) {
-  if (r.slabs == 1) return r.reverse ? launch<T, 1, true>(r, m, states, st) : launch<T, 1, false>(r, m, states, st);
-  return r.reverse ? launch<T, 2, true>(r, m, states, st) : launch<T, 2, false>(r, m, states, st);
+cudaError_t launch(const Set& set, bool states, cudaStream_t st) {
+  const bool rev = set.run[0].reverse;
+  if (set.run[0].slabs == 1) return rev ? launch<T, 1, true>(set, states, st) : launch<T, 1, false>(set, states, st);
+  return rev ? launch<T, 2, true>(set, states, st) : launch<T, 2, false>(set, states, st);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -752,8 +757,8 @@ bool encode_maps(Run& r, Maps& m) {
   return (r.oh != 0 || r.heads == 1) && (r.ob != 0 || r.batch == 1) && encode(&m.o, o, r, r.dc);
 }
 
-cudaError_t launch_pipe(const Run& r, const Maps& m, int dtype, bool states, cudaStream_t st) {
-  return dtype == LAMA_F16 ? launch<__half>(r, m, states, st) : launch<__nv_bfloat16>(r, m, states, st);
+cudaError_t launch_pipe(const Set& set, int dtype, bool states, cudaStream_t st) {
+  return dtype == LAMA_F16 ? launch<__half>(set, states, st) : launch<__nv_bfloat16>(set, states, st);
 }
 
 }  // namespace ops

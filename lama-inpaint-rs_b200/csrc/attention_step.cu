@@ -10,6 +10,7 @@
 // summed over the groups by shuffles and one pass through shared memory.
 // Splitting the columns gives a single stream 4 * heads CTAs at dv = 128.
 #include "operators.cuh"
+#include "ptx.cuh"
 
 namespace lama {
 namespace ops {
@@ -35,6 +36,8 @@ struct Step {
 
 template <class T, int ROWS, bool VEC>  // ROWS * GROUPS >= dk
 __global__ void __launch_bounds__(THREADS) k_step(const __grid_constant__ Step p) {
+  pdl_launch_dependents();
+  pdl_wait();
   __shared__ float sq[128], sk[128];
   __shared__ float part[THREADS / 32][COLS];
   const int blocks = (p.dv + COLS - 1) / COLS;
@@ -107,12 +110,12 @@ __global__ void __launch_bounds__(THREADS) k_step(const __grid_constant__ Step p
 
 template <class T>
 cudaError_t go(const Step& p, unsigned grid, bool vec, cudaStream_t st) {
-  if (p.dk <= 4 * GROUPS) {
-    vec ? k_step<T, 4, true><<<grid, THREADS, 0, st>>>(p) : k_step<T, 4, false><<<grid, THREADS, 0, st>>>(p);
-  } else {
-    vec ? k_step<T, 8, true><<<grid, THREADS, 0, st>>>(p) : k_step<T, 8, false><<<grid, THREADS, 0, st>>>(p);
-  }
-  return cudaGetLastError();
+  const dim3 g(grid);
+  if (p.dk <= 4 * GROUPS)
+    return vec ? launch_chained(k_step<T, 4, true>, g, THREADS, 0, st, p)
+               : launch_chained(k_step<T, 4, false>, g, THREADS, 0, st, p);
+  return vec ? launch_chained(k_step<T, 8, true>, g, THREADS, 0, st, p)
+             : launch_chained(k_step<T, 8, false>, g, THREADS, 0, st, p);
 }
 
 }  // namespace

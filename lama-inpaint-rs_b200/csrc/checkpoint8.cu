@@ -2,8 +2,10 @@
 // checkpoint8.cuh).  Both are one pass bound by memory: a half-warp takes a
 // group of 128 channels, a lane 8 of them (16 bytes of a 16-bit type).
 #include <algorithm>
+#include <type_traits>
 
 #include "checkpoint8.cuh"
+#include "ptx.cuh"
 
 namespace lama {
 namespace ops {
@@ -16,6 +18,8 @@ constexpr int PER_CTA = THREADS / 16;  // groups a CTA takes at a time
 template <class T>
 __global__ void __launch_bounds__(THREADS) k_store(const T* x, long long stride, int8_t* codes, float* scales,
                                                    long long rows, int c, int groups, bool vec) {
+  pdl_launch_dependents();
+  pdl_wait();
   const long long total = rows * groups;
   const int lane = threadIdx.x & 15;
   // every lane of a warp stays in the loop together: encode8 shuffles
@@ -36,6 +40,8 @@ __global__ void __launch_bounds__(THREADS) k_store(const T* x, long long stride,
 template <class T>
 __global__ void __launch_bounds__(THREADS) k_restore(const int8_t* codes, const float* scales, T* x, long long stride,
                                                      long long rows, int c, int groups, bool vec) {
+  pdl_launch_dependents();
+  pdl_wait();
   const long long total = rows * groups;
   const int lane = threadIdx.x & 15;
   for (long long g = (long long)blockIdx.x * PER_CTA + (threadIdx.x >> 4); g < total;
@@ -82,8 +88,8 @@ extern "C" int lama_checkpoint_store(const void* x, int dtype, long long rows, i
   cudaError_t ce = dev.status;
   const cudaStream_t st = (cudaStream_t)stream;
   auto run = [&](auto* p) {
-    k_store<<<grid, THREADS, 0, st>>>(p, row_stride, codes, scales, rows, channels, groups, vec);
-    return cudaGetLastError();
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+    return launch_chained(k_store<T>, dim3(grid), THREADS, 0, st, p, row_stride, codes, scales, rows, channels, groups, vec);
   };
   if (ce == cudaSuccess)
     ce = dtype == LAMA_F32   ? run(static_cast<const float*>(x))
@@ -105,8 +111,8 @@ extern "C" int lama_checkpoint_restore(const int8_t* codes, const float* scales,
   cudaError_t ce = dev.status;
   const cudaStream_t st = (cudaStream_t)stream;
   auto run = [&](auto* p) {
-    k_restore<<<grid, THREADS, 0, st>>>(codes, scales, p, row_stride, rows, channels, groups, vec);
-    return cudaGetLastError();
+    using T = std::remove_pointer_t<decltype(p)>;
+    return launch_chained(k_restore<T>, dim3(grid), THREADS, 0, st, codes, scales, p, row_stride, rows, channels, groups, vec);
   };
   if (ce == cudaSuccess)
     ce = dtype == LAMA_F32   ? run(static_cast<float*>(x))

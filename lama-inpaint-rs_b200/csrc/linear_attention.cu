@@ -33,6 +33,7 @@
 // have, the entering state to two (three for fp32 inputs).  For bf16 inputs the
 // scores' one rounding is of the size of the output's own.
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "attention.cuh"
@@ -148,7 +149,7 @@ struct Plan {
 };
 
 template <class T, bool OUT>
-__global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run r) {
+__global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Set set) {
   using PL = Plan<T>;
   constexpr int NP = PL::NP, EP = PL::EP;
   constexpr int MAXS = 2;
@@ -161,8 +162,18 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
   const uint32_t bar = smem_u32(&bar_mem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  const int segs = OUT ? r.nseg : r.nseg - 1;
+  pdl_launch_dependents();
+  if (warp == 0) tmem_alloc(smem_u32(&tmem_slot), 256);
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    fence_mbar_init();
+    failed = 0;
+  }
+  pdl_wait();
+
+  const int segs = OUT ? set.run[0].nseg : set.run[0].nseg - 1;
   int id = blockIdx.x;
+  const Run& r = set.run[run_of(set, segs, id)];
   const int seg = id % segs;
   id /= segs;
   const int blk = id % r.blocks;
@@ -175,12 +186,6 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
   const int seg_tokens = r.chunks * CH;
   const int p0 = seg * seg_tokens;
 
-  if (warp == 0) tmem_alloc(smem_u32(&tmem_slot), 256);
-  if (tid == 0) {
-    mbar_init(bar, 1);
-    fence_mbar_init();
-    failed = 0;
-  }
   for (int i = tid; i <= CH; i += THREADS) pw[i] = power(g, i);
   tc_fence_before();
   __syncthreads();
@@ -206,7 +211,8 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
     float f = 1.f;
     if (OUT && s < r.slabs) {
       if (r.staged) {
-        src = r.seg + ((bh * r.nseg + seg) * (r.slabs * 64) + er) * ld + ec;
+        src = r.seg + (bh * r.nseg + seg) * (r.slabs * 64 * ld) + er * r.sr + ec * r.sc;
+        step = r.sc;
         cols = 16;
       } else if (r.init && er < r.da) {
         src = r.init + bh * r.da * r.dc + er * r.ir + ec * r.ic;
@@ -469,7 +475,10 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Run 
 // seg[s]: the state segment s adds -> the state that enters it (segments in
 // the order of the recurrence).  The pipelined kernel leaves the final state
 // to this kernel.
-__global__ void k_scan(const __grid_constant__ Run r) {
+__global__ void k_scan(const __grid_constant__ Set set) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const Run& r = set.run[blockIdx.z];
   const int rows = r.slabs * 64, cols = r.blocks * 64;
   const long long per = (long long)rows * cols;
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -511,48 +520,77 @@ __global__ void k_scan(const __grid_constant__ Run r) {
   if (r.pipe && r.fin && inside) r.fin[base + er * r.fr + ec * r.fc] = after;
 }
 
-// Sum over the heads that share one head of the operand: src fp32
-// [rows][heads][d] -> dst [rows][heads / per][d] with strides.
+// Sum over the heads that share one head of an operand: src fp32
+// [batch][tokens][heads][d] -> dst [batch][tokens][heads / per][d] with
+// strides; one operand a blockIdx.y.
+struct Share {
+  struct {
+    const float* src;
+    void* dst;
+    long long sb, st, sh;
+    int per, d;
+  } of[3];
+  long long rows;  // batch * tokens
+  int tokens, heads, n;
+};
 template <class T>
-__global__ void k_share(const float* src, T* dst, long long rows, int tokens, int heads, int per, int d, long long sb,
-                        long long st, long long sh) {
-  const int nh = heads / per;
-  const long long total = rows * nh * d;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-    const int c = (int)(i % d);
-    const long long rh = i / d;
-    const int h = (int)(rh % nh);
-    const long long row = rh / nh;
-    const float* s = src + (row * heads + (long long)h * per) * d + c;
-    float v = 0.f;
-    for (int k = 0; k < per; k++) v += s[(long long)k * d];
-    dst[(row / tokens) * sb + (row % tokens) * st + h * sh + c] = from_float<T>(v);
+__global__ void k_share(const __grid_constant__ Share s) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const auto& o = s.of[blockIdx.y];
+  const int nh = s.heads / o.per, row_size = nh * o.d;
+  for (long long row = blockIdx.x; row < s.rows; row += gridDim.x) {
+    const long long batch = row / s.tokens, token = row - batch * s.tokens;
+    T* dst = static_cast<T*>(o.dst) + batch * o.sb + token * o.st;
+    for (int i = threadIdx.x; i < row_size; i += blockDim.x) {
+      const int h = i / o.d, c = i - h * o.d;
+      const float* src = o.src + (row * s.heads + (long long)h * o.per) * o.d + c;
+      float v = 0.f;
+      for (int k = 0; k < o.per; k++) v += src[(long long)k * o.d];
+      dst[h * o.sh + c] = from_float<T>(v);
+    }
   }
 }
 
 template <class T, bool OUT>
-cudaError_t launch_chunks(const Run& r, cudaStream_t st) {
+cudaError_t launch_chunks(const Set& set, cudaStream_t st) {
   const uint32_t bytes = Plan<T>::bytes();
   static SmemLimit limit;
   const cudaError_t ce = limit.reach(k_chunks<T, OUT>, (int)bytes);
   if (ce != cudaSuccess) return ce;
-  const long long grid = (long long)r.batch * r.heads * r.blocks * (OUT ? r.nseg : r.nseg - 1);
-  k_chunks<T, OUT><<<(unsigned)grid, THREADS, bytes, st>>>(r);
-  return cudaGetLastError();
+  const int nseg = set.run[0].nseg;
+  return launch_chained(k_chunks<T, OUT>, dim3((unsigned)ctas(set, OUT ? nseg : nseg - 1)), THREADS, bytes, st, set);
+}
+template <bool OUT>
+cudaError_t launch_chunks(const Set& set, int dtype, cudaStream_t st) {
+  return dtype == LAMA_F32   ? launch_chunks<float, OUT>(set, st)
+         : dtype == LAMA_F16 ? launch_chunks<__half, OUT>(set, st)
+                             : launch_chunks<__nv_bfloat16, OUT>(set, st);
+}
+cudaError_t launch_scan(const Set& set, cudaStream_t st) {
+  int per = 0;
+  for (int w = 0; w < set.n; w++) per = std::max(per, set.run[w].slabs * 64 * set.run[w].blocks * 64);
+  const Run& r = set.run[0];
+  return launch_chained(k_scan, dim3((per + 255) / 256, r.batch * r.heads, set.n), 256, 0, st, set);
 }
 
-// How a sequence is cut: one segment reads everything once, several read b
-// and c twice but fill the GPU.  Takes the least time on the busiest SM,
-// counted in chunk steps.  Pipelined (16-bit types): a CTA costs 4 beside its chunks
-// (set-up, the first loads, the last products), the pass that makes the
+// How the sequences of a call are cut: one segment reads everything once,
+// several read b and c twice but fill the GPU.  Takes the least time on the
+// busiest SM, counted in chunk steps, for `rows` (sequence, head, 64 columns)
+// that run together.  Pipelined (16-bit types): a CTA costs 4 beside its
+// chunks (set-up, the first loads, the last products), the pass that makes the
 // states 0.6 a chunk and, with the scan, two launches of 3 each.  The other
 // kernel's steps are several times longer and do not overlap.
-void cut(Run& r, bool pipe) {
+struct Cut {
+  int nseg = 1, chunks = 1;
+};
+Cut cut(const lama_attention* p, long long rows) {
+  const bool pipe = p->dtype != LAMA_F32;
   const double cta = pipe ? 4 : 1, pass = pipe ? 6 : 1;
   const int slots = 148;
-  const int chunks = (r.tokens + CH - 1) / CH;
-  const long long rows = (long long)r.batch * r.heads * r.blocks;
+  const int chunks = (p->tokens + CH - 1) / CH;
   double best = 1e300;
+  Cut r;
   for (int c = chunks;;) {
     const int nseg = (chunks + c - 1) / c;
     const double waves = (double)((rows * nseg + slots - 1) / slots);
@@ -565,39 +603,22 @@ void cut(Run& r, bool pipe) {
     if (c == 1) break;
     c = std::max(1, std::min(c - 1, (chunks + nseg) / (nseg + 1)));
   }
-  r.staged = r.nseg > 1;
+  return r;
+}
+int blocks_of(int d) { return (d + 63) / 64; }
+Cut cut_forward(const lama_attention* p) { return cut(p, (long long)p->batch * p->heads * blocks_of(p->dv)); }
+// The gradients' runs: dq and dk have blocks of dk, dv those of dv.  The
+// pipelined kernel takes dk and dv together, the other all three.
+Cut cut_backward(const lama_attention* p) {
+  const int k = blocks_of(p->dk), v = blocks_of(p->dv);
+  return cut(p, (long long)p->batch * p->heads * (p->dtype != LAMA_F32 ? k + v : 2 * k + v));
 }
 
-// Room for the segments' states of a run, whatever its alignment turns out to
-// be and whether or not the final state is asked for.
-long long seg_bytes(const lama_attention* p, int da, int dc) {
-  Run r{};
-  r.batch = p->batch, r.heads = p->heads, r.tokens = p->tokens;
-  r.slabs = (da + 63) / 64, r.blocks = (dc + 63) / 64;
-  cut(r, p->dtype != LAMA_F32);
-  if (!r.staged && p->dtype == LAMA_F32) return 0;
-  return (long long)r.batch * r.heads * r.nseg * r.slabs * 64 * r.blocks * 64 * 4;
-}
-
-template <class T>
-cudaError_t go(Run& r, int dtype, cudaStream_t st) {
-  cudaError_t ce = cudaSuccess;
-  Maps maps;
-  r.pipe = dtype != LAMA_F32 && r.a.vec && r.b.vec && r.c.vec && r.out_vec && encode_maps(r, maps);
-  if (r.pipe && r.fin) r.staged = 1;
-  if (r.staged) {
-    if ((ce = r.pipe ? launch_pipe(r, maps, dtype, true, st) : launch_chunks<T, false>(r, st)) != cudaSuccess) return ce;
-    const int per = r.slabs * 64 * r.blocks * 64;
-    k_scan<<<dim3((per + 255) / 256, r.batch * r.heads), 256, 0, st>>>(r);
-    if ((ce = cudaGetLastError()) != cudaSuccess) return ce;
-  }
-  return r.pipe ? launch_pipe(r, maps, dtype, false, st) : launch_chunks<T, true>(r, st);
-}
-
-cudaError_t run(Run& r, int dtype, cudaStream_t st) {
-  return dtype == LAMA_F32   ? go<float>(r, dtype, st)
-         : dtype == LAMA_F16 ? go<__half>(r, dtype, st)
-                             : go<__nv_bfloat16>(r, dtype, st);
+// Room for the segments' states of one run, whatever its alignment turns out
+// to be and whether or not the final state is asked for.
+long long seg_bytes(const lama_attention* p, const Cut& c) {
+  if (c.nseg == 1 && p->dtype == LAMA_F32) return 0;
+  return (long long)p->batch * p->heads * c.nseg * blocks_of(p->dk) * blocks_of(p->dv) * 64 * 64 * 4;
 }
 
 Operand operand(const lama_rows& x, int heads, int d, int dtype) {
@@ -623,16 +644,19 @@ void output(Run& r, const lama_rows& x, int d, int dtype) {
   r.out_f32 = 0;
 }
 
-void roles(Run& r, const Operand& a, const Operand& b, const Operand& c, int da, int dc, int dtype) {
+void roles(Run& r, const Operand& a, const Operand& b, const Operand& c, int da, int dc) {
   r.a = a;
   r.b = b;
   r.c = c;
   r.da = da;
   r.dc = dc;
-  r.slabs = (da + 63) / 64;
-  r.blocks = (dc + 63) / 64;
-  cut(r, dtype != LAMA_F32);
+  r.slabs = blocks_of(da);
+  r.blocks = blocks_of(dc);
+  r.sr = r.blocks * 64;
+  r.sc = 1;
 }
+
+bool aligned(const Run& r) { return r.a.vec && r.b.vec && r.c.vec && r.out_vec; }
 
 const char* check_rows(const lama_rows& x, const lama_attention* p, const char* what, char* buf, size_t n) {
   if (!x.data) {
@@ -668,8 +692,11 @@ int check(const lama_attention* p, char* err, int err_len) {
   return LAMA_OK;
 }
 
-Run common(const lama_attention* p) {
+Run common(const lama_attention* p, const Cut& c) {
   Run r{};
+  r.nseg = c.nseg;
+  r.chunks = c.chunks;
+  r.staged = c.nseg > 1;
   r.log_decay = p->log_decay;
   r.lengths = p->lengths;
   r.batch = p->batch;
@@ -679,9 +706,9 @@ Run common(const lama_attention* p) {
 }
 
 Run forward_run(const lama_attention* p, float* final_state) {
-  Run r = common(p);
+  Run r = common(p, cut_forward(p));
   roles(r, operand(p->q, p->heads, p->dk, p->dtype), operand(p->k, p->heads, p->dk, p->dtype),
-        operand(p->v, p->heads, p->dv, p->dtype), p->dk, p->dv, p->dtype);
+        operand(p->v, p->heads, p->dv, p->dtype), p->dk, p->dv);
   r.fin = final_state;
   r.inter = r.intra = p->scale;
   r.update = 1.f;
@@ -692,20 +719,20 @@ Run forward_run(const lama_attention* p, float* final_state) {
 }
 
 // The three gradient runs: 0 dq, 1 dk, 2 dv.
-Run gradient_run(const lama_attention* p, const lama_attention_grads* g, int which) {
-  Run r = common(p);
+Run gradient_run(const lama_attention* p, const lama_attention_grads* g, const Cut& c, int which) {
+  Run r = common(p, c);
   const Operand q = operand(p->q, p->heads, p->dk, p->dtype), k = operand(p->k, p->heads, p->dk, p->dtype),
                 v = operand(p->v, p->heads, p->dv, p->dtype), d = operand(g->grad_out, p->heads, p->dv, p->dtype);
   if (which == 0) {
-    roles(r, d, v, k, p->dv, p->dk, p->dtype);
+    roles(r, d, v, k, p->dv, p->dk);
     r.inter = r.intra = p->scale;
     r.update = 1.f;
     r.init = p->initial_state;
   } else {
     if (which == 1) {
-      roles(r, v, d, q, p->dv, p->dk, p->dtype);
+      roles(r, v, d, q, p->dv, p->dk);
     } else {
-      roles(r, k, q, d, p->dk, p->dv, p->dtype);
+      roles(r, k, q, d, p->dk, p->dv);
       r.fin = g->grad_initial_state;
     }
     r.inter = 1.f;
@@ -743,13 +770,13 @@ extern "C" long long lama_linear_attention_workspace(const lama_attention* p, in
   if (err && err_len > 0) err[0] = 0;
   const int rc = check(p, err, err_len);
   if (rc != LAMA_OK) return rc;
-  if (!backward) return up(seg_bytes(p, p->dk, p->dv));
-  const long long seg = std::max(seg_bytes(p, p->dk, p->dv), seg_bytes(p, p->dv, p->dk));
-  long long share = 0;
+  if (!backward) return up(seg_bytes(p, cut_forward(p)));
+  // the states of dq's run and of dv's, then the unsummed gradients of shared heads
+  long long bytes = 2 * up(seg_bytes(p, cut_backward(p)));
   const int heads[3] = {p->q.heads, p->k.heads, p->v.heads}, d[3] = {p->dk, p->dk, p->dv};
   for (int w = 0; w < 3; w++)
-    if (heads[w] != p->heads) share = std::max(share, (long long)p->batch * p->tokens * p->heads * d[w] * 4);
-  return up(seg) + up(share);
+    if (heads[w] != p->heads) bytes += up((long long)p->batch * p->tokens * p->heads * d[w] * 4);
+  return bytes;
 }
 
 extern "C" int lama_linear_attention(const lama_attention* p, const lama_rows* out, float* final_state, void* workspace,
@@ -764,11 +791,21 @@ extern "C" int lama_linear_attention(const lama_attention* p, const lama_rows* o
     return fail(err, err_len, LAMA_EINVAL, "workspace of %lld bytes, %lld needed", workspace_bytes, need);
   DeviceGuard dev(device);
   cudaError_t ce = dev.status;
-  Run r = forward_run(p, final_state);
+  const cudaStream_t st = (cudaStream_t)stream;
+  Set set;
+  set.n = 1;
+  Run& r = set.run[0];
+  r = forward_run(p, final_state);
   output(r, *out, p->dv, p->dtype);
   r.seg = static_cast<float*>(workspace);
   if (ce == cudaSuccess) ce = status_word(&r.status);
-  if (ce == cudaSuccess) ce = run(r, p->dtype, (cudaStream_t)stream);
+  r.pipe = p->dtype != LAMA_F32 && aligned(r) && encode_maps(r, set.maps[0]);
+  if (r.pipe && r.fin) r.staged = 1;
+  if (ce == cudaSuccess && r.staged) {
+    ce = r.pipe ? launch_pipe(set, p->dtype, true, st) : launch_chunks<false>(set, p->dtype, st);
+    if (ce == cudaSuccess) ce = launch_scan(set, st);
+  }
+  if (ce == cudaSuccess) ce = r.pipe ? launch_pipe(set, p->dtype, false, st) : launch_chunks<true>(set, p->dtype, st);
   if (ce != cudaSuccess) return fail(err, err_len, LAMA_ECUDA, "linear attention: %s", cudaGetErrorString(ce));
   return LAMA_OK;
 }
@@ -795,41 +832,85 @@ extern "C" int lama_linear_attention_backward(const lama_attention* p, const lam
   int* status = nullptr;
   if (ce == cudaSuccess) ce = status_word(&status);
   const cudaStream_t st = (cudaStream_t)stream;
-  const long long seg = std::max(seg_bytes(p, p->dk, p->dv), seg_bytes(p, p->dv, p->dk));
-  float* shared = reinterpret_cast<float*>(static_cast<char*>(workspace) + up(seg));
-  for (int w = 0; w < 3 && ce == cudaSuccess; w++) {
-    Run r = gradient_run(p, g, w);
+  const Cut c = cut_backward(p);
+  char* room = static_cast<char*>(workspace) + 2 * up(seg_bytes(p, c));
+  Share share{};
+  share.rows = (long long)p->batch * p->tokens;
+  share.tokens = p->tokens, share.heads = p->heads;
+  Run run[3];  // dq, dk, dv
+  bool pipe = p->dtype != LAMA_F32;
+  for (int w = 0; w < 3; w++) {
+    Run& r = run[w] = gradient_run(p, g, c, w);
     const lama_rows& o = *rows[1 + w];
     const int d = w == 2 ? p->dv : p->dk;
-    r.seg = static_cast<float*>(workspace);
     r.status = status;
+    r.seg = reinterpret_cast<float*>(static_cast<char*>(workspace) + (w ? up(seg_bytes(p, c)) : 0));
     if (o.heads == p->heads) {
       output(r, o, d, p->dtype);
-      ce = run(r, p->dtype, st);
     } else {
-      r.out = shared;
+      r.out = room;
       r.out_f32 = 1;
       r.oh = d;
       r.ot = (long long)p->heads * d;
       r.ob = r.ot * p->tokens;
       r.out_vec = d % 8 == 0;
-      ce = run(r, p->dtype, st);
-      if (ce != cudaSuccess) break;
-      const long long n = (long long)p->batch * p->tokens;
-      const int per = p->heads / o.heads;
-      const unsigned grid = (unsigned)std::min<long long>((n * o.heads * d + 255) / 256, 148 * 16);
-      auto share = [&](auto* dst) {
-        k_share<<<grid, 256, 0, st>>>(shared, dst, n, p->tokens, p->heads, per, d, o.batch_stride, o.token_stride,
-                                      o.head_stride);
-      };
-      if (p->dtype == LAMA_F32)
-        share(static_cast<float*>(o.data));
-      else if (p->dtype == LAMA_F16)
-        share(static_cast<__half*>(o.data));
-      else
-        share(static_cast<__nv_bfloat16*>(o.data));
-      ce = cudaGetLastError();
+      auto& s = share.of[share.n++];
+      s.src = reinterpret_cast<float*>(room);
+      s.dst = o.data, s.sb = o.batch_stride, s.st = o.token_stride, s.sh = o.head_stride;
+      s.per = p->heads / o.heads, s.d = d;
+      room += up((long long)p->batch * p->tokens * p->heads * d * 4);
     }
+    pipe = pipe && aligned(r);
+  }
+  // dk's carried state is dv's transposed
+  run[1].sr = 1, run[1].sc = run[2].sr;
+  Set set;
+  auto take = [&](std::initializer_list<int> which) {
+    set.n = 0;
+    for (int w : which) set.run[set.n++] = run[w];
+  };
+  Maps maps[3];
+  for (int w = 0; w < 3 && pipe; w++) pipe = encode_maps(run[w], maps[w]);
+  for (Run& r : run) {
+    r.pipe = pipe;
+    r.staged = r.staged || (pipe && g->grad_initial_state);
+  }
+  if (ce == cudaSuccess && pipe) {
+    auto pass = [&](std::initializer_list<int> which, bool states) {
+      if (ce != cudaSuccess) return;
+      take(which);
+      int i = 0;
+      for (int w : which) set.maps[i++] = maps[w];
+      ce = launch_pipe(set, p->dtype, states, st);
+    };
+    // one set per direction and number of slabs
+    if (run[0].staged) {
+      if (run[0].nseg > 1) pass({0}, true);
+      pass({2}, true);
+      take({0, 2});
+      if (ce == cudaSuccess) ce = launch_scan(set, st);
+    }
+    pass({0}, false);
+    if (run[1].slabs == run[2].slabs) {
+      pass({1, 2}, false);
+    } else {
+      pass({1}, false);
+      pass({2}, false);
+    }
+  } else if (ce == cudaSuccess) {
+    if (run[0].staged) {
+      take({0, 2});
+      ce = launch_chunks<false>(set, p->dtype, st);
+      if (ce == cudaSuccess) ce = launch_scan(set, st);
+    }
+    take({0, 1, 2});
+    if (ce == cudaSuccess) ce = launch_chunks<true>(set, p->dtype, st);
+  }
+  if (ce == cudaSuccess && share.n) {
+    const dim3 grid((unsigned)std::min<long long>(share.rows, 148 * 16), share.n);
+    ce = p->dtype == LAMA_F32   ? launch_chained(k_share<float>, grid, 128, 0, st, share)
+         : p->dtype == LAMA_F16 ? launch_chained(k_share<__half>, grid, 128, 0, st, share)
+                                : launch_chained(k_share<__nv_bfloat16>, grid, 128, 0, st, share);
   }
   if (ce != cudaSuccess) return fail(err, err_len, LAMA_ECUDA, "linear attention backward: %s", cudaGetErrorString(ce));
   return LAMA_OK;

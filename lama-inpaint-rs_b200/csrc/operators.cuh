@@ -71,6 +71,26 @@ struct SmemLimit {
   std::mutex mutex;
 };
 
+// Launch with programmatic stream serialisation: the kernel may start, up to
+// its pdl_wait(), while the one before it on the stream ends.  Every kernel of
+// the operators calls pdl_launch_dependents() first and pdl_wait() before it
+// touches global memory, so the chain of kernels stays ordered.
+template <class... KArgs, class... Args>
+cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st,
+                           const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+
 inline int dtype_size(int t) { return t == LAMA_F32 ? 4 : 2; }
 inline bool dtype_ok(int t) { return t == LAMA_F32 || t == LAMA_F16 || t == LAMA_BF16; }
 

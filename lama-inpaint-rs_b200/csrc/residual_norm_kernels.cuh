@@ -148,6 +148,8 @@ __device__ __forceinline__ uint2 shared_codes(uint32_t at, int n) {
 
 template <class T, int W, int NI, bool SAVE8, int MODE>
 __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const __grid_constant__ Fwd p) {
+  pdl_launch_dependents();
+  pdl_wait();
   constexpr int TEAMS = team_threads<W> / (W * 32);
   __shared__ float slots[TEAMS][2 * W];
   extern __shared__ __align__(16) float factors[];
@@ -308,6 +310,8 @@ struct Saved {
 
 template <class T, int W, int NI, bool SAVE8, int MODE>
 __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(const __grid_constant__ Bwd p) {
+  pdl_launch_dependents();
+  pdl_wait();
   constexpr int TEAMS = team_threads<W> / (W * 32);
   __shared__ float slots[TEAMS][2 * W];
   __shared__ float sums[TEAMS > 1 ? TEAMS : 1][TEAMS > 1 ? W * NI * 256 : 1];
@@ -543,6 +547,8 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
 // are split between sets and parts, added up in a fixed order.
 template <class T>
 __global__ void __launch_bounds__(1024) k_norm_sums(const __grid_constant__ Bwd p) {
+  pdl_launch_dependents();
+  pdl_wait();
   __shared__ float sa[32][33], sb[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
@@ -619,8 +625,7 @@ cudaError_t start(unsigned grid, int threads, size_t smem, cudaStream_t st, cons
     const cudaError_t e = limit.reach(KERNEL, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  KERNEL<<<grid, threads, smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_chained(KERNEL, dim3(grid), (unsigned)threads, smem, st, p);
 }
 
 // Bytes of a CTA's factors and rings, and whether they leave room for a second
@@ -672,8 +677,7 @@ cudaError_t run_backward(const Bwd& b, cudaStream_t st) {
                  : start<k_norm_grad<T, W, NI, false, SCALAR>>(grid, TH, smem, st, b);
   });
   if (e != cudaSuccess) return e;
-  k_norm_sums<T><<<(b.c + 31) / 32, 1024, 0, st>>>(b);
-  return cudaGetLastError();
+  return launch_chained(k_norm_sums<T>, dim3((b.c + 31) / 32), 1024, 0, st, b);
 }
 
 }  // namespace ops
