@@ -204,8 +204,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
   id /= r.blocks;
   const int head = id % r.heads, batch = id / r.heads;
   const float g = r.log_decay[head];
-  int len = r.tokens;
-  if (r.lengths) len = min(max(r.lengths[batch], 0), r.tokens);
+  const int tokens = r.tokens;
+  const bool ragged = r.lengths, out_f32 = r.out_f32;
+  int len = tokens;
+  if (ragged) len = min(max(r.lengths[batch], 0), tokens);
   const int seg_tokens = r.chunks * CH;
   const int seg = REV ? r.nseg - 1 - slot : slot;
   const int p0 = seg * seg_tokens;
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
   };
 
   auto wait_stage = [&](int c) {  // b, and c where its rows may have to be cleared
-    return wait(bars.full, L::AS, c, 13) && (!r.lengths || wait(bars.cfull, L::CS, c, 22));
+    return wait(bars.full, L::AS, c, 13) && (!ragged || wait(bars.cfull, L::CS, c, 22));
   };
   // b~ of chunk c by the CONV warps, t their thread: row j times lam to the chunk's end, UP parts
   auto make_bd = [&](int c, int t) {
@@ -241,7 +243,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
     const uint32_t ab = smem + (c % L::AS) * L::AB, ct = smem + L::C + (c % L::CS) * TILE;
     const uint32_t src = ab + L::B, dst = smem + L::BD + (c % L::KB) * L::BD_BUF;
     const int n = num(c), ck = t & 7;
-    if (r.lengths && n < CH) {  // the boxes hold tokens past the sequence's end
+    if (ragged && n < CH) {  // the boxes hold tokens past the sequence's end
 #pragma unroll 1
       for (uint32_t i = t; i < (L::AB + TILE) / 16; i += TH)
         if ((int)((i >> 3) & 127) >= n) sts16(i < L::AB / 16 ? ab + i * 16 : ct + (i - L::AB / 16) * 16, make_uint4(0, 0, 0, 0));
@@ -297,11 +299,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
     // ------------------------------------------------------------ loads
     if (elect_one()) {
       bool ok = true;
+      const int ha = head / r.a.per * r.a.hs, hb = head / r.b.per * r.b.hs, hc = head / r.c.per * r.c.hs;
+      const int ba = batch * r.a.bs, bb = batch * r.b.bs, bc = batch * r.c.bs;
       int issued = 0, cissued = 0;
 #pragma unroll 1
       for (int c = 0; c < live; c++) {
-        auto tile = [&](uint32_t dst, const CUtensorMap* map, const Operand& o, int d0, uint32_t bar) {
-          tma_load_4d(dst, map, d0, p0 + at(c), (head / o.per) * o.hs, batch * o.bs, bar);
+        auto tile = [&](uint32_t dst, const CUtensorMap* map, int h, int b, int d0, uint32_t bar) {
+          tma_load_4d(dst, map, d0, p0 + at(c), h, b, bar);
         };
         // boxes count in full, past the tensor's end too
         if (c >= L::AS && !(ok = wait(bars.empty, L::AS, c - L::AS, 11))) break;
@@ -309,14 +313,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
         mbar_arrive_expect_tx(bar, L::AB);
 #pragma unroll 1
         for (int s = 0; s < NS; s++) {
-          if (OUT) tile(ab + s * TILE, &maps.a, r.a, s * 64, bar);
-          tile(ab + L::B + s * TILE, &maps.b, r.b, s * 64, bar);
+          if (OUT) tile(ab + s * TILE, &maps.a, ha, ba, s * 64, bar);
+          tile(ab + L::B + s * TILE, &maps.b, hb, bb, s * 64, bar);
         }
         issued = c + 1;
         if (c >= L::CS && !(ok = wait(bars.cempty, L::CS, c - L::CS, 21))) break;
         const uint32_t cbar = smem_u32(&bars.cfull[c % L::CS]);
         mbar_arrive_expect_tx(cbar, TILE);
-        tile(smem + L::C + (c % L::CS) * TILE, &maps.c, r.c, blk * 64, cbar);
+        tile(smem + L::C + (c % L::CS) * TILE, &maps.c, hc, bc, blk * 64, cbar);
         cissued = c + 1;
       }
       // after a wait that ran out, the copies in flight end before the CTA does
@@ -353,11 +357,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
       for (int i = 0; i < W; i++, src += step) E[i] = i < rows ? f * *src : 0.f;
     }
     bool ok = true;
+    const float update = r.update;
     auto take = [&](int c) {  // E: the state after chunk c, and unless it is the last one decayed to the next
       if (!wait(bars.u, L::KB, c, 12)) return false;
       tc_fence_after();
       const float d = pw[num(c) - 1], f = c + 1 < live ? lam : 1.f;
-      const float fe = f * d, fu = f * r.update * (HALF ? bs[c & 3] : 1.f);
+      const float fe = f * d, fu = f * update * (HALF ? bs[c & 3] : 1.f);
 #pragma unroll
       for (int i = 0; i < W; i += 32) {
         float u[32];
@@ -522,13 +527,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
     const int grp = warp >> 2, rb = warp & 3, row = rb * 32 + lane;
     const uint32_t t = tmem + grp * 192 + ((uint32_t)(rb * 32) << 16);
     const long long hb = batch * r.ob + head * r.oh + blk * 64;
+    const float intra = r.intra, inter = r.inter;
     const int width = min(64, r.dc - blk * 64);
     bool ok = true;
     for (int c = grp; c < live; c += 2) {
       if (!(ok = __all_sync(~0u, wait(bars.s, 2, c, 19)))) break;
       tc_fence_after();
       const int n = num(c);
-      float rowf = r.intra, back = 1.f;  // factors of the row's scores, and of its results
+      float rowf = intra, back = 1.f;  // factors of the row's scores, and of its results
       if (HALF) {
         // P in fp16's range: the row's largest score (masked ones included, an
         // upper bound does: fp16 keeps its precision over 2^28) to at most 2^14
@@ -543,7 +549,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
 #pragma unroll
           for (int i = 0; i < 64; i++) m = fmaxf(m, fabsf(v[i]));
         }
-        const int e = (int)(__float_as_uint(m * fabsf(r.intra)) >> 23);
+        const int e = (int)(__float_as_uint(m * fabsf(intra)) >> 23);
         const int shift = min(max(e - 127 - 13, -24), 40);
         rowf *= __uint_as_float((uint32_t)(127 - shift) << 23);
         back = __uint_as_float((uint32_t)(127 + shift) << 23);
@@ -592,7 +598,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
         tmem_st16(t + h * 32 + 16, w + 16);
       }
       const int dist = REV ? n - 1 - row : row;
-      float di = dist >= 0 ? r.inter * pw[dist] : 0.f;
+      float di = dist >= 0 ? inter * pw[dist] : 0.f;
       if (HALF) di *= 1.f / back;
 #pragma unroll 1
       for (int h = 0; h < 2; h++) {
@@ -636,13 +642,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
         if (row >= n)
 #pragma unroll
           for (int i = 0; i < 32; i++) v[i] = 0.f;
-        if (r.out_f32 || !STAGED_OUT) {
-          if (tok < r.tokens) {
+        if (out_f32 || !STAGED_OUT) {
+          if (tok < tokens) {
             const long long dst = hb + (long long)tok * r.ot + h * 32;
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               if (h * 32 + i >= width) break;
-              if (r.out_f32)
+              if (out_f32)
                 store_vec<float, 8>(static_cast<float*>(r.out) + dst + i, v + i);
               else
                 store_vec<T, 8>(static_cast<T*>(r.out) + dst + i, v + i);
@@ -658,10 +664,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
         }
       }
       if (!STAGED_OUT) continue;
-      if (!r.out_f32) fence_async_smem();
+      if (!out_f32) fence_async_smem();
       named_sync(1 + grp, 128);
       if (rb == (REV ? 3 : 0) && lane == 0) {  // the warp with the fewest scores
-        if (!r.out_f32) {
+        if (!out_f32) {
           tma_store_4d(&maps.o, ct, blk * 64, p0 + at(c), head, batch);
           bulk_commit();
           bulk_wait_read0();
@@ -672,12 +678,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
     }
     bulk_wait0();
     // tokens past the sequence's end
-    const int end = min(p0 + seg_tokens, r.tokens);
+    const int end = min(p0 + seg_tokens, tokens);
     for (int i = tid; i < (end - p0 - live * CH) * 64; i += 256) {
       const int c = i & 63;
       if (c >= width) continue;
       const long long dst = hb + (long long)(p0 + live * CH + (i >> 6)) * r.ot + c;
-      if (r.out_f32)
+      if (out_f32)
         static_cast<float*>(r.out)[dst] = 0.f;
       else
         static_cast<T*>(r.out)[dst] = from_float<T>(0.f);

@@ -308,7 +308,7 @@ struct Saved {
   }
 };
 
-template <class T, int W, int NI, bool SAVE8, int MODE>
+template <class T, int W, int NI, bool SAVE8, int MODE, bool TOKEN>  // TOKEN: a gate for each row
 __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(const __grid_constant__ Bwd p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -320,7 +320,8 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
   int turn = 0;
   const float inv_c = 1.f / (float)p.c;
   const Span span = rows_of(p);
-  const bool token_gate = p.gate && p.per == 1, pre = p.w_pre && p.gn;
+  constexpr bool token_gate = TOKEN;
+  const bool pre = p.w_pre && p.gn;
   float sa[NI][8], sb[NI][8];
 #pragma unroll
   for (int i = 0; i < NI; i++)
@@ -406,7 +407,9 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
   fill_factors<T>(p, span.set, p.gate && !token_gate, factors);
   __syncthreads();
   int k = 0;  // rows of the team so far
-  for (; row < span.r1; row += TEAMS, k++) {
+  T *dx = static_cast<T*>(p.dx) + row * p.c + LAMA_CH(0), *dy = static_cast<T*>(p.dy) + row * p.c + LAMA_CH(0);
+  const int left = p.c - LAMA_CH(0);  // of this lane's row from its first channel on
+  for (; row < span.r1; row += TEAMS, k++, dx += TEAMS * p.c, dy += TEAMS * p.c) {
     if (MODE == RING) ring.wait(k, &failed);
     auto from_ring = [&](Saved<T, SAVE8>& s, uint32_t at, uint32_t scales, int c0) {
       if (SAVE8) {
@@ -427,13 +430,19 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
           from_ring(su[i], at + o_u, at + o_end + 8 + 4 * p.groups, c0);
           rn[i] = shared_raw<T>(at + o_n + c0 * sizeof(T), n);
         }
-        rd[i] = shared_raw<T>(at + o_d + c0 * sizeof(T), p.gu ? n : 0);
       }
     }
     float d[NI][8];  // D
+    auto stream = [&] {  // grad_u
 #pragma unroll
-    for (int i = 0; i < NI; i++) rd[i].to(d[i]);
-    if (pre) {
+      for (int i = 0; i < NI; i++) {
+        if (MODE == RING) rd[i] = shared_raw<T>(ring.stage(k) + o_d + LAMA_CH(i) * sizeof(T), p.gu ? p.c - LAMA_CH(i) : 0);
+        rd[i].to(d[i]);
+      }
+    };
+    if (!pre) {
+      stream();
+    } else {
       float uh[NI][8], t[NI][8], q0 = 0.f, q1 = 0.f;
 #pragma unroll
       for (int i = 0; i < NI; i++) {
@@ -449,6 +458,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
         }
       }
       const float q = -ru * (row_sum<W>(q0 + q1, slots[team], turn, team, warp) * inv_c);
+      stream();
 #pragma unroll
       for (int i = 0; i < NI; i++)
 #pragma unroll
@@ -458,7 +468,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
         }
     }
 #pragma unroll
-    for (int i = 0; i < NI; i++) store8(static_cast<T*>(p.dx) + row * p.c + LAMA_CH(i), p.c - LAMA_CH(i), VEC, d[i]);
+    for (int i = 0; i < NI; i++) store8(dx + i * W * 256, left - i * W * 256, VEC, d[i]);
     float y[NI][8], q0 = 0.f, q1 = 0.f;
     if (MODE == RING) {
 #pragma unroll
@@ -513,7 +523,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
         }
     }
 #pragma unroll
-    for (int i = 0; i < NI; i++) store8(static_cast<T*>(p.dy) + row * p.c + LAMA_CH(i), p.c - LAMA_CH(i), VEC, d[i]);
+    for (int i = 0; i < NI; i++) store8(dy + i * W * 256, left - i * W * 256, VEC, d[i]);
   }
   if (MODE == RING && ring.leader && lane == 0 && failed) atomicCAS(p.status, 0, failed);
   // this CTA's column sums: part[cta][0] = sum D yh (times the gate where each token has one), [1] = sum dn uh
@@ -667,14 +677,19 @@ cudaError_t run_backward(const Bwd& b, cudaStream_t st) {
     const size_t kept = (size_t)b.c * (codes ? 1 : sizeof(T)), full = (size_t)b.c * sizeof(T);
     const size_t row = kept * (pre ? 2 : 1) + full * ((b.gu != nullptr) + pre + (b.gate && b.per == 1)) +
                        (8 + (codes ? 8 * (size_t)b.groups : 0) + 15) / 16 * 16;
-    if (b.vec && (!codes || ((uintptr_t)b.cy | (uintptr_t)b.cu | b.c) % 16 == 0) && ring_fits<W>(b.c, row, smem))
-      return codes ? start<k_norm_grad<T, W, NI, true, RING>>(grid, TH, smem, st, b)
-                   : start<k_norm_grad<T, W, NI, false, RING>>(grid, TH, smem, st, b);
-    if (b.vec)
-      return codes ? start<k_norm_grad<T, W, NI, true, VECTOR>>(grid, TH, smem, st, b)
-                   : start<k_norm_grad<T, W, NI, false, VECTOR>>(grid, TH, smem, st, b);
-    return codes ? start<k_norm_grad<T, W, NI, true, SCALAR>>(grid, TH, smem, st, b)
-                 : start<k_norm_grad<T, W, NI, false, SCALAR>>(grid, TH, smem, st, b);
+    const int mode = !b.vec ? SCALAR
+                     : (!codes || ((uintptr_t)b.cy | (uintptr_t)b.cu | b.c) % 16 == 0) && ring_fits<W>(b.c, row, smem) ? RING
+                                                                                                                  : VECTOR;
+    auto go = [&](auto save8, auto token) {
+      constexpr bool S = decltype(save8)::value, G = decltype(token)::value;
+      return mode == RING     ? start<k_norm_grad<T, W, NI, S, RING, G>>(grid, TH, smem, st, b)
+             : mode == VECTOR ? start<k_norm_grad<T, W, NI, S, VECTOR, G>>(grid, TH, smem, st, b)
+                              : start<k_norm_grad<T, W, NI, S, SCALAR, G>>(grid, TH, smem, st, b);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    const bool token = b.gate && b.per == 1;
+    return codes ? (token ? go(yes, yes) : go(yes, no)) : (token ? go(no, yes) : go(no, no));
   });
   if (e != cudaSuccess) return e;
   return launch_chained(k_norm_sums<T>, dim3((b.c + 31) / 32), 1024, 0, st, b);
