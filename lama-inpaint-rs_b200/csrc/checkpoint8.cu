@@ -30,8 +30,9 @@ __global__ void __launch_bounds__(THREADS) k_store(const T* x, long long stride,
     const int grp = (int)(g - row * groups), c0 = grp * GROUP8 + lane * 8;
     const int n = on ? min(8, c - c0) : 0;
     float v[8], scale;
-    load8(x + row * stride + c0, n, vec, v);
-    const uint2 code = encode8(v, scale);
+    const Raw8<T> raw = vec ? load_raw<T, true>(x + row * stride + c0, n) : load_raw<T, false>(x + row * stride + c0, n);
+    raw.to(v);
+    const uint2 code = encode8(raw, v, scale);
     store_codes(codes + row * c + c0, n, vec, code);
     if (on && lane == 0) scales[g] = scale;
   }

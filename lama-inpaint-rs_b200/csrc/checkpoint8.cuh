@@ -23,12 +23,26 @@ constexpr int GROUP8 = 128;
 // Integers up to 127 are rounded (half to even) and read off by adding
 // 1.5 * 2^23, whose last place is 1: the conversion instructions run at a
 // sixteenth of the rate.
-__device__ __forceinline__ uint2 encode8(const float* v, float& scale) {
+// `raw`: the same values as they are in memory (16-bit types are compared as
+// such, two a word).
+template <class T>
+__device__ __forceinline__ uint2 encode8(const Raw8<T>& raw, const float* v, float& scale) {
   uint32_t a = 0;
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
 #pragma unroll
-  for (int i = 0; i < 8; i++) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);  // NaN compares above infinity
+    for (int i = 0; i < 4; i++) a = __vmaxu2(a, w[i] & 0x7fff7fffu);  // NaN compares above infinity
+    a = max(a & 0xffffu, a >> 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);
+  }
 #pragma unroll
   for (int m = 1; m < 16; m <<= 1) a = max(a, __shfl_xor_sync(~0u, a, m));
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t h = (uint16_t)a;
+    a = __float_as_uint(to_float(*reinterpret_cast<const T*>(&h)));
+  }
   const float amax = __uint_as_float(a);
   float inv = 0.f;
   scale = 0.f;

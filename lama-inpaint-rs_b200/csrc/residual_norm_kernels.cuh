@@ -146,7 +146,7 @@ __device__ __forceinline__ uint2 shared_codes(uint32_t at, int n) {
   return c;
 }
 
-template <class T, int W, int NI, bool SAVE8, int MODE>
+template <class T, int W, int NI, bool SAVE8, int MODE, bool TOKEN>  // TOKEN: a gate for each row
 __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const __grid_constant__ Fwd p) {
   pdl_launch_dependents();
   pdl_wait();
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
   int turn = 0;
   const float inv_c = 1.f / (float)p.c;
   const Span span = rows_of(p);
-  const bool token_gate = p.gate && p.per == 1;
+  constexpr bool token_gate = TOKEN;
   constexpr bool VEC = MODE != SCALAR;
   __shared__ uint64_t bars[MODE == RING ? TEAMS * STAGES : 1];
   __shared__ int failed;
@@ -195,7 +195,23 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
   fill_factors<T>(p, span.set, p.gate && !token_gate, factors);
   __syncthreads();
   int k = 0;  // rows of the team so far
-  for (; row < span.r1; row += TEAMS, k++) {
+  const int left = p.c - LAMA_CH(0);  // of this lane's row from its first channel on
+  const long long at0 = row * p.c + LAMA_CH(0);
+  const int step = TEAMS * p.c;
+  T *pu = static_cast<T*>(p.u) + at0, *pn = static_cast<T*>(p.n) + at0;
+  int8_t *cy = p.cy + at0, *cu = p.cu + at0;
+  float *sy = p.sy + row * p.groups + LAMA_CH(0) / GROUP8, *su = p.su + row * p.groups + LAMA_CH(0) / GROUP8;
+  auto codes = [&](const Raw8<T>* raw, const float (*v)[8], int8_t* codes, float* scales) {
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      float scale;
+      const uint2 code = encode8(raw[i], v[i], scale);
+      store_codes(codes + i * W * 256, left - i * W * 256, VEC, code);
+      if ((lane & 15) == 0 && left > i * W * 256) scales[i * W * 2] = scale;
+    }
+  };
+  for (; row < span.r1; row += TEAMS, k++, pu += step, pn += step, cy += step, cu += step, sy += TEAMS * p.groups,
+                        su += TEAMS * p.groups) {
     float x[NI][8], y[NI][8];
     if (MODE == RING) {
       ring.wait(k, &failed);
@@ -226,16 +242,8 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
         for (int j = 0; j < 8; j += 2) fma2(q0, q1, y[i][j], y[i][j + 1], y[i][j], y[i][j + 1]);
       ry = 1.f / sqrtf(row_sum<W>(q0 + q1, slots[team], turn, team, warp) * inv_c + p.eps);
     }
-    if (SAVE8) {
-#pragma unroll
-      for (int i = 0; i < NI; i++) {
-        float scale;
-        const uint2 code = encode8(y[i], scale);
-        const int n = p.c - LAMA_CH(i);
-        store_codes(p.cy + row * p.c + LAMA_CH(i), n, VEC, code);
-        if ((lane & 15) == 0 && n > 0) p.sy[row * p.groups + LAMA_CH(i) / GROUP8] = scale;
-      }
-    }
+    if (SAVE8) codes(ry_, y, cy, sy);
+    Raw8<T> u[NI];
     float q0 = 0.f, q1 = 0.f;
 #pragma unroll
     for (int i = 0; i < NI; i++) {
@@ -247,30 +255,20 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
 #pragma unroll
         for (int j = 0; j < 8; j += 2) mul2(f[j], f[j + 1], g[j], g[j + 1]);
       }
-      Raw8<T> u;
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
         mul2(y[i][j], y[i][j + 1], ry, ry);
         fma2(x[i][j], x[i][j + 1], f[j], f[j + 1], y[i][j], y[i][j + 1]);
-        u.e[j] = from_float<T>(x[i][j]);
-        u.e[j + 1] = from_float<T>(x[i][j + 1]);
+        u[i].e[j] = from_float<T>(x[i][j]);
+        u[i].e[j + 1] = from_float<T>(x[i][j + 1]);
       }
-      u.to(x[i]);  // the stream carries the rounded sum
+      u[i].to(x[i]);  // the stream carries the rounded sum
 #pragma unroll
       for (int j = 0; j < 8; j += 2) fma2(q0, q1, x[i][j], x[i][j + 1], x[i][j], x[i][j + 1]);
-      store8(static_cast<T*>(p.u) + row * p.c + LAMA_CH(i), p.c - LAMA_CH(i), VEC, x[i]);
+      store8(pu + i * W * 256, left - i * W * 256, VEC, x[i]);
     }
     if (MODE != RING && row + TEAMS < span.r1) fetch(row + TEAMS);  // in flight during the second half
-    if (SAVE8 && p.cu) {
-#pragma unroll
-      for (int i = 0; i < NI; i++) {
-        float scale;
-        const uint2 code = encode8(x[i], scale);
-        const int n = p.c - LAMA_CH(i);
-        store_codes(p.cu + row * p.c + LAMA_CH(i), n, VEC, code);
-        if ((lane & 15) == 0 && n > 0) p.su[row * p.groups + LAMA_CH(i) / GROUP8] = scale;
-      }
-    }
+    if (SAVE8 && p.cu) codes(u, x, cu, su);
     if (p.w_pre) {
       const float ru = 1.f / sqrtf(row_sum<W>(q0 + q1, slots[team], turn, team, warp) * inv_c + p.eps);
 #pragma unroll
@@ -282,7 +280,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
           mul2(x[i][j], x[i][j + 1], ru, ru);
           mul2(x[i][j], x[i][j + 1], f[j], f[j + 1]);
         }
-        store8(static_cast<T*>(p.n) + row * p.c + LAMA_CH(i), p.c - LAMA_CH(i), VEC, x[i]);
+        store8(pn + i * W * 256, left - i * W * 256, VEC, x[i]);
       }
       if (p.ru && warp == 0 && lane == 0) p.ru[row] = ru;
     }
@@ -656,14 +654,17 @@ cudaError_t run_forward(const Fwd& f, cudaStream_t st) {
     const unsigned grid = (unsigned)(f.sets * f.parts);
     size_t smem = 2 * sizeof(float) * (size_t)f.c;
     const size_t row = (size_t)f.c * sizeof(T) * (f.gate && f.per == 1 ? 3 : 2);
-    if (f.vec && ring_fits<W>(f.c, row, smem))
-      return f.cy ? start<k_norm<T, W, NI, true, RING>>(grid, TH, smem, st, f)
-                  : start<k_norm<T, W, NI, false, RING>>(grid, TH, smem, st, f);
-    if (f.vec)
-      return f.cy ? start<k_norm<T, W, NI, true, VECTOR>>(grid, TH, smem, st, f)
-                  : start<k_norm<T, W, NI, false, VECTOR>>(grid, TH, smem, st, f);
-    return f.cy ? start<k_norm<T, W, NI, true, SCALAR>>(grid, TH, smem, st, f)
-                : start<k_norm<T, W, NI, false, SCALAR>>(grid, TH, smem, st, f);
+    const int mode = !f.vec ? SCALAR : ring_fits<W>(f.c, row, smem) ? RING : VECTOR;
+    auto go = [&](auto save8, auto token) {
+      constexpr bool S = decltype(save8)::value, G = decltype(token)::value;
+      return mode == RING     ? start<k_norm<T, W, NI, S, RING, G>>(grid, TH, smem, st, f)
+             : mode == VECTOR ? start<k_norm<T, W, NI, S, VECTOR, G>>(grid, TH, smem, st, f)
+                              : start<k_norm<T, W, NI, S, SCALAR, G>>(grid, TH, smem, st, f);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    const bool token = f.gate && f.per == 1;
+    return f.cy ? (token ? go(yes, yes) : go(yes, no)) : (token ? go(no, yes) : go(no, no));
   });
 }
 
