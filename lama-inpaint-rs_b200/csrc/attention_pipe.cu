@@ -10,6 +10,7 @@
 //   warps  8..11  state: b decayed to the chunk's end, rounded, as an MMA
 //                 operand; U = c^T b~ back from TMEM; the state in registers
 //                 (fp32), E' = lam^n E + lam U, and E as two bf16 parts
+//   warps 14, 15  with two slabs, half of the decayed b
 //   warp  13      issues the MMAs: U = c^T b~, S = a b^T, O = a E, O += P c
 //   warps  0..7   two groups that take chunks in turn: scores S from TMEM,
 //                 decay and causal mask, rounded to bf16 P in S's place (the
@@ -43,26 +44,35 @@ namespace ops {
 
 namespace {
 
-constexpr int THREADS = 14 * 32;  // 4 warps a scheduler at most: 128 registers a thread
+
+template <int N>
+using num_of = std::integral_constant<int, N>;
 
 template <class T, int NS, bool OUT>
 struct Lay {
   static constexpr int UP = OUT ? 1 : std::is_same_v<T, __half> ? 2 : 3;  // parts of b~
   // stages of (a, b), free once S and a E are made, and of c, free after P c;
-  // buffers of b~ and of U, and of E
-  static constexpr int AS = OUT ? (NS == 1 ? 3 : 2) : (NS == 1 ? 4 : 2), CS = OUT ? (NS == 1 ? 4 : 2) : (NS == 1 ? 4 : 3);
-  static constexpr int KB = NS == 1 ? 2 : 1, ES = NS == 1 ? 2 : 1;
+  // buffers of b~ (of a chunk, or without outputs of half a chunk), of U and of E
+  static constexpr int AS = OUT ? (NS == 1 ? 3 : 2) : (NS == 1 ? 5 : 2), CS = OUT ? (NS == 1 ? 4 : 2) : (NS == 1 ? 5 : 4);
+  static constexpr int KB = OUT && NS == 2 ? 1 : 2, UB = KB, ES = NS == 1 ? 2 : 1;
   static constexpr uint32_t B = OUT ? NS * TILE : 0, AB = B + NS * TILE;  // a stage's b, its size
-  static constexpr uint32_t C = AS * AB, BD = C + CS * TILE, BD_BUF = UP * NS * TILE;
+  static constexpr uint32_t BTILE = OUT ? TILE : ETILE;                   // one slab and part of b~
+  static constexpr uint32_t C = AS * AB, BD = C + CS * TILE, BD_BUF = UP * NS * BTILE;
   static constexpr uint32_t E = BD + KB * BD_BUF, E_BUF = 2 * NS * ETILE;
   static constexpr uint32_t BYTES = E + (OUT ? ES * E_BUF : 0);
-  static constexpr int CONV = OUT ? 4 : 8;  // warps that make b~
+  // Two more warps make half of b~ where a chunk has two slabs (350 -> 310 us at
+  // 2 x 65536 x 4 x 128); with one the state warps keep up, and the two would
+  // be in the way (train step of 16 x 4096 x 8 x 64: 240 -> 299 us).
+  static constexpr bool MORE = OUT && NS == 2;
+  static constexpr int CONV = OUT ? (MORE ? 6 : 4) : 8;  // warps that make b~
+  static constexpr int THREADS = (MORE ? 16 : 14) * 32;  // 4 warps a scheduler at most: 128 registers a thread
   static constexpr uint32_t T_U = OUT ? 384 : 0;  // TMEM column of U; buffer i of S at 192 i, of O at 192 i + 128
-  static_assert(T_U + KB * 64 * NS <= 512, "TMEM columns");
+  static_assert(T_U + UB * 64 * NS <= 512, "TMEM columns");
 };
 
+constexpr int MAX_STAGES = 5;
 struct Bars {
-  uint64_t full[4], empty[4], cfull[4], cempty[4], bd[2], u[2], e[2], s[2], p[2], o[2], oe[2];
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], cfull[MAX_STAGES], cempty[MAX_STAGES], bd[2], u[2], e[2], s[2], p[2], o[2], oe[2];
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int c0, int c1, int c2, int c3, uint32_t bar) {
@@ -147,15 +157,16 @@ __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t phase, int* err, i
 }
 
 template <class T, int NS, bool OUT, bool REV>
-__global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set set, int segs) {
+__global__ void __launch_bounds__(Lay<T, NS, OUT>::THREADS, 1) k_pipe(const __grid_constant__ Set set, int segs) {
   using L = Lay<T, NS, OUT>;
-  constexpr int UP = L::UP;
+  constexpr int UP = L::UP, THREADS = L::THREADS;
   constexpr bool HALF = std::is_same_v<T, __half>;
   // Results leave through the stage that held c (one TMA store a chunk; per-row
   // stores kept the load/store unit busy: 70 -> 59 us at 128 x 4096 tokens of
   // 64).  With two slabs c has two stages only, and holding them longer costs
   // more (195 -> 213 us): there the rows are stored directly.
   constexpr bool STAGED_OUT = NS == 1;
+  static_assert(L::AS <= MAX_STAGES && L::CS <= MAX_STAGES && L::KB <= 2 && L::UB <= 2 && L::ES <= 2, "barriers");
   extern __shared__ uint8_t raw[];
   __shared__ __align__(16) float pw[CH + 4];
   // fp16: factors 2^e of the columns of E (bf16, chunk c in row c % 4: a group is done with its chunk
@@ -175,7 +186,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
   if (warp == 0) tmem_alloc(smem_u32(&tmem_slot), 512);
   if (tid == 32) {
     failed = 0;
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < MAX_STAGES; i++) {
       mbar_init(smem_u32(&bars.full[i]), 1);
       mbar_init(smem_u32(&bars.empty[i]), 1);
       mbar_init(smem_u32(&bars.cfull[i]), 1);
@@ -186,7 +197,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
       mbar_init(smem_u32(&bars.u[i]), 1);
       mbar_init(smem_u32(&bars.e[i]), 4);
       mbar_init(smem_u32(&bars.s[i]), 1);
-      mbar_init(smem_u32(&bars.p[i]), 4);
+      mbar_init(smem_u32(&bars.p[i]), OUT ? 4 : 1);
       mbar_init(smem_u32(&bars.o[i]), 1);
       mbar_init(smem_u32(&bars.oe[i]), 4);
     }
@@ -224,7 +235,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  // barrier i of a set of n for the c-th chunk: its phase ends once every n chunks
+  // Barrier i of a set of n for the c-th chunk: its phase ends once every n
+  // chunks.  Where a wait runs out, the roles that share named barriers go on
+  // with what is there (every later wait gives up at once, the loops end), so
+  // that none is left waiting for another; the other two roles stop.
   auto wait = [&](uint64_t* set, int n, int c, int code) {
     const uint32_t bar = smem_u32(&set[c % n]), ph = (uint32_t)(c / n) & 1;
     return mbar_try_wait(bar, ph) || wait_long(bar, ph, &failed, code);
@@ -237,25 +251,30 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
   auto wait_stage = [&](int c) {  // b, and c where its rows may have to be cleared
     return wait(bars.full, L::AS, c, 13) && (!ragged || wait(bars.cfull, L::CS, c, 22));
   };
-  // b~ of chunk c by the CONV warps, t their thread: row j times lam to the chunk's end, UP parts
-  auto make_bd = [&](int c, int t) {
-    constexpr int TH = L::CONV * 32;
+  // b~ of chunk c: row j times lam to the chunk's end, in UP parts; ROWS rows (half h
+  // of them, or all) by a team of TH threads, t one of them.
+  float up = 1.f;  // fp16: the scale of b~
+  auto make_rows = [&](int c, int h, int t, auto team, auto rows) {
+    constexpr int TH = decltype(team)::value, ROWS = decltype(rows)::value, LOG = ROWS == 128 ? 7 : 6;
     const uint32_t ab = smem + (c % L::AS) * L::AB, ct = smem + L::C + (c % L::CS) * TILE;
-    const uint32_t src = ab + L::B, dst = smem + L::BD + (c % L::KB) * L::BD_BUF;
+    const uint32_t src = ab + L::B;
+    const uint32_t dst = smem + L::BD + (OUT ? c % L::KB : h) * L::BD_BUF;
     const int n = num(c), ck = t & 7;
     if (ragged && n < CH) {  // the boxes hold tokens past the sequence's end
 #pragma unroll 1
-      for (uint32_t i = t; i < (L::AB + TILE) / 16; i += TH)
-        if ((int)((i >> 3) & 127) >= n) sts16(i < L::AB / 16 ? ab + i * 16 : ct + (i - L::AB / 16) * 16, make_uint4(0, 0, 0, 0));
+      for (uint32_t i = t; i < (L::AB + TILE) / TILE * ROWS * 8; i += TH) {
+        const uint32_t at = (i >> (LOG + 3)) * TILE + h * (TILE / 2) + (i & (ROWS * 8 - 1)) * 16;  // its rows, tile after tile
+        if ((int)((at >> 7) & 127) >= n) sts16(at < L::AB ? ab + at : ct + (at - L::AB), make_uint4(0, 0, 0, 0));
+      }
     }
     // a batch's loads go out before its first use: loads and stores of shared memory stay in program order
-    constexpr int BATCH = UP == 1 ? 8 : 4, ALL = NS * CH * 8 / TH;
-    float up = 1.f;
-    if (HALF) {
-      // b~ = b lam^m may leave fp16's normal numbers at the lower end: where no |b| reaches 2^8, it is made 2^8 times as large
+    constexpr int ALL = NS * ROWS * 8 / TH, MOST = UP == 1 ? 8 : 4, BATCH = ALL < MOST ? ALL : MOST;
+    if (HALF && (OUT || h == 0)) {
+      // b~ = b lam^m may leave fp16's normal numbers at the lower end: where no |b| of the chunk reaches 2^8, it is made
+      // 2^8 times as large
       uint32_t top = 0;
 #pragma unroll 8
-      for (int i = 0; i < ALL; i++) {
+      for (int i = 0; i < NS * CH * 8 / TH; i++) {
         const int k = i * (TH / 8) + (t >> 3);
         uint4 x = lds16(src + (k >> 7) * TILE + swz(k & (CH - 1), ck));
         if ((k & (CH - 1)) >= n) x = make_uint4(0, 0, 0, 0);
@@ -263,8 +282,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
                                      __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
       }
       const uint32_t most = max(top & 0xffffu, top >> 16);
-      if (named_sync_and(3, TH, most < 0x5c00u)) up = 256.f;  // 0x5c00: 2^8
-      if (t == 0) bs[c & 3] = 1.f / up;
+      up = named_sync_and(3 + 2 * (TH == 64), TH, most < 0x5c00u) ? 256.f : 1.f;  // 0x5c00: 2^8
+      if (t == 0 && h == 0) bs[c & 3] = 1.f / up;
     }
 #pragma unroll 1
     for (int i0 = 0; i0 < ALL; i0 += BATCH) {
@@ -272,14 +291,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
       float w[BATCH];
 #pragma unroll
       for (int i = 0; i < BATCH; i++) {
-        const int k = (i0 + i) * (TH / 8) + (t >> 3), j = k & (CH - 1);  // the slabs' rows one after another
-        x[i] = lds16(src + (k >> 7) * TILE + swz(j, ck));
+        const int k = (i0 + i) * (TH / 8) + (t >> 3), j = h * 64 + (k & (ROWS - 1));  // the slabs' rows one after another
+        x[i] = lds16(src + (k >> LOG) * TILE + swz(j, ck));
         w[i] = pw[REV ? j : max(n - 1 - j, 0)];
         if (HALF) w[i] *= up;
       }
 #pragma unroll
       for (int i = 0; i < BATCH; i++) {
-        const int k = (i0 + i) * (TH / 8) + (t >> 3), j = k & (CH - 1);
+        const int k = (i0 + i) * (TH / 8) + (t >> 3), j = h * 64 + (k & (ROWS - 1));
         if (j >= n) x[i] = make_uint4(0, 0, 0, 0);
         float v[8];
         unpack8<T>(x[i], v);
@@ -288,11 +307,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
         uint4 parts[UP];
         split8<UP, T>(v, parts);
 #pragma unroll
-        for (int p = 0; p < UP; p++) sts16(dst + (p * NS + (k >> 7)) * TILE + swz(j, ck), parts[p]);
+        for (int p = 0; p < UP; p++) sts16(dst + (p * NS + (k >> LOG)) * L::BTILE + swz(OUT ? j : j & 63, ck), parts[p]);
       }
     }
     fence_async_smem();
-    arrive(bars.bd, L::KB, c);
+    arrive(bars.bd, L::KB, OUT ? c : 2 * c + h);
   };
 
   if (warp == 12) {
@@ -356,17 +375,17 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
 #pragma unroll
       for (int i = 0; i < W; i++, src += step) E[i] = i < rows ? f * *src : 0.f;
     }
-    bool ok = true;
     const float update = r.update;
     auto take = [&](int c) {  // E: the state after chunk c, and unless it is the last one decayed to the next
-      if (!wait(bars.u, L::KB, c, 12)) return false;
+      wait(bars.u, L::UB, c, 12);
+      __syncwarp();
       tc_fence_after();
       const float d = pw[num(c) - 1], f = c + 1 < live ? lam : 1.f;
       const float fe = f * d, fu = f * update * (HALF ? bs[c & 3] : 1.f);
 #pragma unroll
       for (int i = 0; i < W; i += 32) {
         float u[32];
-        tmem_ld32(tmem + L::T_U + (c % L::KB) * (64 * NS) + lane_base + half * W + i, u);
+        tmem_ld32(tmem + L::T_U + (c % L::UB) * (64 * NS) + lane_base + half * W + i, u);
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
@@ -377,17 +396,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
         }
       }
       tc_fence_before();
-      if (!OUT) arrive(bars.e, L::KB, c);  // U's buffer is free
-      return true;
+      if (!OUT) arrive(bars.e, L::UB, c);  // U's buffer is free
     };
-    for (int c = 0; c < live && ok; c++) {
-      if (OUT && !(ok = __all_sync(~0u, wait_stage(c)))) break;
-      if (L::KB == 1 && c > 0 && !(ok = __all_sync(~0u, take(c - 1)))) break;
-      if (OUT) make_bd(c, t);
-      if (L::KB == 2 && c > 0 && !(ok = __all_sync(~0u, take(c - 1)))) break;
+#pragma unroll 1
+    for (int c = 0; c < live; c++) {
+      if (OUT) {
+        wait_stage(c);
+        __syncwarp();
+      }
+      if (L::KB == 1 && c > 0) take(c - 1);  // the products that read b~'s only buffer
+      if (OUT) make_rows(c, 0, t, num_of<128>(), num_of<L::MORE ? 64 : 128>());
+      if (L::KB == 2 && c > 0) take(c - 1);
       if (OUT) {
         // E's buffer is free once the products of chunk c - ES are done
-        if (c >= L::ES && !(ok = __all_sync(~0u, wait(bars.s, 2, c - L::ES, 14)))) break;
+        if (c >= L::ES) wait(bars.s, 2, c - L::ES, 14);
+        __syncwarp();
         const uint32_t eb = smem + L::E + (c % L::ES) * L::E_BUF;
         float fe = 1.f;
         if (HALF) {
@@ -420,8 +443,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
         arrive(bars.e, L::ES, c);
       }
     }
-    if (ok && live) ok = take(live - 1);
-    if (ok && !OUT) {
+    if (live) take(live - 1);
+    if (!OUT) {
       float* dst = r.seg + ((bh * r.nseg + slot) * (NS * 64) + half * W) * (r.blocks * 64) + ec;
 #pragma unroll
       for (int i = 0; i < W; i++, dst += r.blocks * 64) *dst = E[i];
@@ -457,19 +480,30 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
     for (int c = 0; c < live; c++) {
       const uint32_t st = smem + (c % L::AS) * L::AB;
       if (!ready(bars.cfull, L::CS, c, 23)) break;
-      if (!ready(bars.bd, L::KB, c, 16)) break;  // b~ is made from a full stage
-      if (!OUT && c >= L::KB && !ready(bars.e, L::KB, c - L::KB, 25)) break;
-      if (leader) {
-        const uint32_t tu = tmem + L::T_U + (c % L::KB) * (64 * NS);
-        const uint64_t dc = desc_mn(smem + L::C + (c % L::CS) * TILE, 0);  // 64 columns, read twice to fill the MMA's 128 rows
+      if (!OUT && c >= L::UB && !ready(bars.e, L::UB, c - L::UB, 25)) break;
+      const uint32_t tu = tmem + L::T_U + (c % L::UB) * (64 * NS);
+      constexpr int HALVES = OUT ? 1 : 2, STEPS = 8 / HALVES;  // b~ comes in halves without outputs
 #pragma unroll 1
-        for (int p = UP - 1; p >= 0; p--) {
-          const uint64_t db = desc_mn(smem + L::BD + (c % L::KB) * L::BD_BUF + p * NS * TILE, TILE);
+      for (int h = 0; h < HALVES; h++) {
+        const int u = c * HALVES + h;
+        if (!ready(bars.bd, L::KB, u, 16)) break;  // b~ is made from a full stage
+        if (leader) {
+          // 64 columns, read twice to fill the MMA's 128 rows
+          const uint64_t dc = desc_mn(smem + L::C + (c % L::CS) * TILE + h * (TILE / 2), 0);
+#pragma unroll 1
+          for (int p = UP - 1; p >= 0; p--) {
+            const uint64_t db = desc_mn(smem + L::BD + (u % L::KB) * L::BD_BUF + p * NS * L::BTILE, L::BTILE);
 #pragma unroll 4
-          for (int k = 0; k < 8; k++)
-            mma_bf16(tu, dc + ((2048 * k) >> 4), db + ((2048 * k) >> 4), ID_U, p < UP - 1 || k > 0);
+            for (int k = 0; k < STEPS; k++)
+              mma_bf16(tu, dc + ((2048 * k) >> 4), db + ((2048 * k) >> 4), ID_U, h > 0 || p < UP - 1 || k > 0);
+          }
+          if (!OUT) mma_commit(smem_u32(&bars.p[h]));
         }
-        mma_commit(smem_u32(&bars.u[c % L::KB]));
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (leader) {
+        mma_commit(smem_u32(&bars.u[c % L::UB]));
         if (!OUT) {
           mma_commit(smem_u32(&bars.empty[c % L::AS]));
           mma_commit(smem_u32(&bars.cempty[c % L::CS]));
@@ -517,10 +551,20 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
   } else if (!OUT && warp < 8) {
     // ------------------------------------------------------------ b~ of the kernel without outputs
 #pragma unroll 1
+    for (int u = 0; u < 2 * live; u++) {
+      if ((u & 1) == 0) wait_stage(u >> 1);
+      if (u >= 2) wait(bars.p, 2, u - 2, 24);
+      __syncwarp();
+      make_rows(u >> 1, u & 1, tid, num_of<256>(), num_of<64>());
+    }
+  } else if (L::MORE && warp >= 14) {
+    // ------------------------------------------------------------ the second half of b~
+#pragma unroll 1
     for (int c = 0; c < live; c++) {
-      if (!__all_sync(~0u, wait_stage(c))) break;
-      if (c >= L::KB && !__all_sync(~0u, wait(bars.u, L::KB, c - L::KB, 24))) break;
-      make_bd(c, tid);
+      wait_stage(c);
+      if (c >= L::KB) wait(bars.u, L::UB, c - L::KB, 24);
+      __syncwarp();
+      make_rows(c, 1, tid - 14 * 32, num_of<64>(), num_of<64>());
     }
   } else if (OUT && warp < 8) {
     // ------------------------------------------------------------ scores and outputs
@@ -529,9 +573,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
     const long long hb = batch * r.ob + head * r.oh + blk * 64;
     const float intra = r.intra, inter = r.inter;
     const int width = min(64, r.dc - blk * 64);
-    bool ok = true;
+#pragma unroll 1
     for (int c = grp; c < live; c += 2) {
-      if (!(ok = __all_sync(~0u, wait(bars.s, 2, c, 19)))) break;
+      wait(bars.s, 2, c, 19);
+      __syncwarp();
       tc_fence_after();
       const int n = num(c);
       float rowf = intra, back = 1.f;  // factors of the row's scores, and of its results
@@ -622,7 +667,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_pipe(const __grid_constant__ Set
       tmem_wait_st();
       tc_fence_before();
       arrive(bars.p, 2, c);
-      if (!(ok = __all_sync(~0u, wait(bars.o, 2, c, 20)))) break;
+      wait(bars.o, 2, c, 20);
+      __syncwarp();
       tc_fence_after();
       const int tok = p0 + at(c) + row;
       // the tile of c has been read: the results take its place on their way out
@@ -706,7 +752,7 @@ cudaError_t launch(const Set& set, int segs, cudaStream_t st) {
   static SmemLimit limit;
   const cudaError_t ce = limit.reach(k_pipe<T, NS, OUT, REV>, bytes);
   if (ce != cudaSuccess) return ce;
-  return launch_chained(k_pipe<T, NS, OUT, REV>, dim3((unsigned)ctas(set, segs)), THREADS, bytes, st, set, segs);
+  return launch_chained(k_pipe<T, NS, OUT, REV>, dim3((unsigned)ctas(set, segs)), Lay<T, NS, OUT>::THREADS, bytes, st, set, segs);
 }
 
 template <class T, int NS, bool REV>
