@@ -11,6 +11,7 @@ namespace lama {
 namespace ops {
 
 constexpr int CH = 128;         // tokens of a chunk (the MMA's M)
+constexpr int FINE = 4 * CH;    // tokens up to which the pipelined kernel keeps scores in two parts
 constexpr uint32_t TILE = 128 * 128;  // bytes of 128 rows x 64 bf16, 128-byte swizzle
 constexpr uint32_t ETILE = 64 * 128;  // 64 rows x 64 bf16
 
@@ -44,6 +45,7 @@ struct Run {
   int nseg, chunks;  // segments of a sequence, chunks of a segment
   int pipe;        // attention_pipe.cu runs it: segments stay where they are when it runs backwards
   int staged;      // the segments' states are made first and scanned
+  int fine;        // scores in two parts (attention_pipe.cu)
   int blocks;      // 64-column blocks of c
   int slabs;       // 64-column slabs of a and b
 };

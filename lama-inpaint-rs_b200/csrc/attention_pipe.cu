@@ -29,6 +29,11 @@
 // decayed b in three parts (24 bits): they are fp32 results.  So a final state
 // costs a pass over b and c, and outputs do not depend on asking for it.
 //
+// Sequences of up to FINE tokens take P in two parts: there the scores are
+// most of an output, and the launches cost more than the second product
+// (500 tokens: no difference; 16 x 4096 tokens, forward and backward: 240 us
+// with one part, 285 with two).
+//
 // fp16 has 3 more bits and a narrow range, so what the kernel rounds to it is
 // scaled by powers of two first: the rows of P by the row's largest score, the
 // columns of E by the column's largest entry, b~ by 2^8 where that fits; two
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(Lay<T, NS, OUT>::THREADS, 1) k_pipe(const __gr
   const int head = id % r.heads, batch = id / r.heads;
   const float g = r.log_decay[head];
   const int tokens = r.tokens;
-  const bool ragged = r.lengths, out_f32 = r.out_f32;
+  const bool ragged = r.lengths, out_f32 = r.out_f32, fine = r.fine;
   int len = tokens;
   if (ragged) len = min(max(r.lengths[batch], 0), tokens);
   const int seg_tokens = r.chunks * CH;
@@ -469,8 +474,11 @@ __global__ void __launch_bounds__(Lay<T, NS, OUT>::THREADS, 1) k_pipe(const __gr
       if (leader) {
         const uint32_t t = tmem + (c & 1) * 192;
         const uint64_t dc = desc_mn(smem + L::C + (c % L::CS) * TILE, 0);
+#pragma unroll 1
+        for (int p = fine; p >= 0; p--)
 #pragma unroll 4
-        for (int k = 0; k < 8; k++) mma_ta(t + 128, t + 8 * k, dc + ((2048 * k) >> 4), ID_P, 1);
+          for (int k = 0; k < 8; k++)
+            mma_ta(t + 128, t + (k >> 2) * 64 + p * 32 + (k & 3) * 8, dc + ((2048 * k) >> 4), ID_P, 1);
         mma_commit(smem_u32(&bars.o[c & 1]));
         if (!STAGED_OUT) mma_commit(smem_u32(&bars.cempty[c % L::CS]));
       }
@@ -608,14 +616,16 @@ __global__ void __launch_bounds__(Lay<T, NS, OUT>::THREADS, 1) k_pipe(const __gr
           tmem_ld32(t + h * 64 + 32, v + 32);
           tmem_wait_ld();
         }
-        uint32_t w[32];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           const int b = 2 * h + k;
           float* x = v + k * 32;
+          uint32_t w[16];
           if (REV ? b < rb : b > rb) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) w[k * 16 + i] = 0;
+            for (int i = 0; i < 16; i++) w[i] = 0;
+            tmem_st16(t + h * 64 + k * 16, w);
+            if (fine) tmem_st16(t + h * 64 + 32 + k * 16, w);
             continue;
           }
           if (b == rb) {
@@ -637,10 +647,18 @@ __global__ void __launch_bounds__(Lay<T, NS, OUT>::THREADS, 1) k_pipe(const __gr
             }
           }
 #pragma unroll
-          for (int i = 0; i < 16; i++) w[k * 16 + i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+          for (int i = 0; i < 16; i++) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+          // over this half's columns, which have been read: 32 of the first parts, 32 of the second
+          tmem_st16(t + h * 64 + k * 16, w);
+          if (fine) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const float2 f = unpack2<T>(w[i]);
+              w[i] = pack2<T>(x[2 * i] - f.x, x[2 * i + 1] - f.y);
+            }
+            tmem_st16(t + h * 64 + 32 + k * 16, w);
+          }
         }
-        tmem_st16(t + h * 32, w);  // over columns already read
-        tmem_st16(t + h * 32 + 16, w + 16);
       }
       const int dist = REV ? n - 1 - row : row;
       float di = dist >= 0 ? inter * pw[dist] : 0.f;

@@ -697,6 +697,7 @@ Run common(const lama_attention* p, const Cut& c) {
   r.nseg = c.nseg;
   r.chunks = c.chunks;
   r.staged = c.nseg > 1;
+  r.fine = p->tokens <= FINE;
   r.log_decay = p->log_decay;
   r.lengths = p->lengths;
   r.batch = p->batch;

@@ -37,15 +37,19 @@ constexpr int STAGES = 3;
 // channel of element 0 of part i of this lane
 #define LAMA_CH(i) (((i)*W * 32 + warp * 32 + lane) * 8)
 
-// The per-channel factors of a CTA's rows, in shared memory: [0] s w_post and,
-// where the rows share a gate row, that; [1] w_pre.
-template <class T, class P>
+// The per-channel factors of a CTA's rows, in shared memory: [0] s and, where
+// the rows share a gate row, that; [1] w_pre; [2] w_post.  FOLDED: [0] times
+// w_post, no [2].
+template <class T, bool FOLDED, class P>
 __device__ __forceinline__ void fill_factors(const P& p, int set, bool set_gate, float* f) {
   for (int c = threadIdx.x; c < p.c; c += blockDim.x) {
-    float a = (p.s ? p.s[c] : p.s0) * (p.w_post ? p.w_post[c] : 1.f);
+    float a = p.s ? p.s[c] : p.s0;
+    const float w = p.w_post ? p.w_post[c] : 1.f;
+    if (FOLDED) a *= w;
     if (set_gate) a *= to_float(static_cast<const T*>(p.gate)[set * p.gs + c]);
     f[c] = a;
     f[p.c + c] = p.w_pre ? p.w_pre[c] : 1.f;
+    if (!FOLDED) f[2 * p.c + c] = w;
   }
 }
 __device__ __forceinline__ void factors8(const float* f, int c0, int c, float* v) {
@@ -186,13 +190,13 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
     ring.issued++;
   };
   if (MODE == RING) {
-    ring.init(bars, smem_u32(factors) + 8 * p.c, (token_gate ? 3 : 2) * rb, team, warp == 0, 1);
+    ring.init(bars, smem_u32(factors) + 12 * p.c, (token_gate ? 3 : 2) * rb, team, warp == 0, 1);
     if (ring.leader)
       for (int k = 0; k < STAGES && row + k * TEAMS < span.r1; k++) issue(row + k * TEAMS);
   } else if (row < span.r1) {
     fetch(row);
   }
-  fill_factors<T>(p, span.set, p.gate && !token_gate, factors);
+  fill_factors<T, false>(p, span.set, p.gate && !token_gate, factors);
   __syncthreads();
   int k = 0;  // rows of the team so far
   const int left = p.c - LAMA_CH(0);  // of this lane's row from its first channel on
@@ -240,25 +244,29 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
       for (int i = 0; i < NI; i++)
 #pragma unroll
         for (int j = 0; j < 8; j += 2) fma2(q0, q1, y[i][j], y[i][j + 1], y[i][j], y[i][j + 1]);
-      ry = 1.f / sqrtf(row_sum<W>(q0 + q1, slots[team], turn, team, warp) * inv_c + p.eps);
+      ry = rsqrtf(row_sum<W>(q0 + q1, slots[team], turn, team, warp) * inv_c + p.eps);
     }
     if (SAVE8) codes(ry_, y, cy, sy);
     Raw8<T> u[NI];
     float q0 = 0.f, q1 = 0.f;
 #pragma unroll
     for (int i = 0; i < NI; i++) {
-      float f[8];
+      float f[8], w[8];
       factors8(factors, LAMA_CH(i), p.c, f);
+      factors8(factors + 2 * p.c, LAMA_CH(i), p.c, w);
       if (token_gate) {
         float g[8];
         rg[i].to(g);
 #pragma unroll
         for (int j = 0; j < 8; j += 2) mul2(f[j], f[j + 1], g[j], g[j + 1]);
       }
+      // each operation of x + (s g) ((y r_y) w_post) rounded by itself: u decides codes that a contracted sum would flip
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
         mul2(y[i][j], y[i][j + 1], ry, ry);
-        fma2(x[i][j], x[i][j + 1], f[j], f[j + 1], y[i][j], y[i][j + 1]);
+        mul2(y[i][j], y[i][j + 1], w[j], w[j + 1]);
+        x[i][j] = __fadd_rn(x[i][j], __fmul_rn(f[j], y[i][j]));
+        x[i][j + 1] = __fadd_rn(x[i][j + 1], __fmul_rn(f[j + 1], y[i][j + 1]));
         u[i].e[j] = from_float<T>(x[i][j]);
         u[i].e[j + 1] = from_float<T>(x[i][j + 1]);
       }
@@ -270,7 +278,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
     if (MODE != RING && row + TEAMS < span.r1) fetch(row + TEAMS);  // in flight during the second half
     if (SAVE8 && p.cu) codes(u, x, cu, su);
     if (p.w_pre) {
-      const float ru = 1.f / sqrtf(row_sum<W>(q0 + q1, slots[team], turn, team, warp) * inv_c + p.eps);
+      const float ru = rsqrtf(row_sum<W>(q0 + q1, slots[team], turn, team, warp) * inv_c + p.eps);
 #pragma unroll
       for (int i = 0; i < NI; i++) {
         float f[8];
@@ -402,7 +410,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
       for (int k = 0; k < STAGES && row + k * TEAMS < span.r1; k++) issue(row + k * TEAMS);
   }
   if (MODE != RING && row < span.r1) fetch(row);
-  fill_factors<T>(p, span.set, p.gate && !token_gate, factors);
+  fill_factors<T, true>(p, span.set, p.gate && !token_gate, factors);
   __syncthreads();
   int k = 0;  // rows of the team so far
   T *dx = static_cast<T*>(p.dx) + row * p.c + LAMA_CH(0), *dy = static_cast<T*>(p.dy) + row * p.c + LAMA_CH(0);
@@ -636,12 +644,12 @@ cudaError_t start(unsigned grid, int threads, size_t smem, cudaStream_t st, cons
   return launch_chained(KERNEL, dim3(grid), (unsigned)threads, smem, st, p);
 }
 
-// Bytes of a CTA's factors and rings, and whether they leave room for a second
+// Adds a CTA's rings to its factors' bytes, if they leave room for a second
 // CTA of four warps, or for one of more.
 template <int W>
-bool ring_fits(int c, size_t row_bytes, size_t& smem) {
+bool ring_fits(size_t row_bytes, size_t& smem) {
   constexpr int TEAMS = team_threads<W> / (W * 32);
-  const size_t with = 2 * sizeof(float) * (size_t)c + TEAMS * STAGES * row_bytes;
+  const size_t with = smem + TEAMS * STAGES * row_bytes;
   if (with + STATIC_SMEM > (size_t)(W <= 4 ? 227 * 1024 / 2 : 227 * 1024)) return false;
   smem = with;
   return true;
@@ -652,9 +660,9 @@ cudaError_t run_forward(const Fwd& f, cudaStream_t st) {
   return by_width(f.c, [&](auto w, auto ni) {
     constexpr int W = decltype(w)::value, NI = decltype(ni)::value, TH = team_threads<W>;
     const unsigned grid = (unsigned)(f.sets * f.parts);
-    size_t smem = 2 * sizeof(float) * (size_t)f.c;
+    size_t smem = 3 * sizeof(float) * (size_t)f.c;
     const size_t row = (size_t)f.c * sizeof(T) * (f.gate && f.per == 1 ? 3 : 2);
-    const int mode = !f.vec ? SCALAR : ring_fits<W>(f.c, row, smem) ? RING : VECTOR;
+    const int mode = !f.vec ? SCALAR : ring_fits<W>(row, smem) ? RING : VECTOR;
     auto go = [&](auto save8, auto token) {
       constexpr bool S = decltype(save8)::value, G = decltype(token)::value;
       return mode == RING     ? start<k_norm<T, W, NI, S, RING, G>>(grid, TH, smem, st, f)
@@ -679,7 +687,7 @@ cudaError_t run_backward(const Bwd& b, cudaStream_t st) {
     const size_t row = kept * (pre ? 2 : 1) + full * ((b.gu != nullptr) + pre + (b.gate && b.per == 1)) +
                        (8 + (codes ? 8 * (size_t)b.groups : 0) + 15) / 16 * 16;
     const int mode = !b.vec ? SCALAR
-                     : (!codes || ((uintptr_t)b.cy | (uintptr_t)b.cu | b.c) % 16 == 0) && ring_fits<W>(b.c, row, smem) ? RING
+                     : (!codes || ((uintptr_t)b.cy | (uintptr_t)b.cu | b.c) % 16 == 0) && ring_fits<W>(row, smem) ? RING
                                                                                                                   : VECTOR;
     auto go = [&](auto save8, auto token) {
       constexpr bool S = decltype(save8)::value, G = decltype(token)::value;
