@@ -313,12 +313,14 @@ typedef struct {
 
 /* Linear attention with a decay for each head:
  *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t.
- * log_decay: [heads] fp32 on the device, -inf (no memory) allowed; it is a
- * constant of the layer and has no gradient.  lengths: null, or [batch] int32
+ * log_decay: [heads] fp32 on the device, <= 0 (not checked: it is not on the
+ * host), -inf (no memory) allowed; a constant of the layer without a gradient.  lengths: null, or [batch] int32
  * on the device (values outside 0..tokens are clamped): sequence b consists of
  * its first lengths[b] tokens, later tokens are never read and their outputs
  * and gradients are 0.  initial_state: null (zeros) or [batch][heads][dk][dv]
- * fp32.  dk, dv <= 128; batch * heads <= 65535. */
+ * fp32.  dk, dv <= 128; batch * heads <= 65535.  Results are the same from run
+ * to run, and whether or not the final state is asked for.  An infinity or NaN
+ * in a token reaches the outputs of its whole 128-token chunk. */
 typedef struct {
   int dtype; /* of q, k, v and the output: LAMA_F32, LAMA_F16 or LAMA_BF16 */
   int batch, tokens, heads, dk, dv;

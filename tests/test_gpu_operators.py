@@ -680,3 +680,77 @@ def test_refusals_of_tensors(F):
     with pytest.raises(LamaError):
         F.gated_residual_norm_backward(x[:1], None, saved)
     F.check_operators()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("dk,dv,T", [(8, 8, 130), (16, 40, 260), (72, 24, 300), (24, 120, 1), (104, 128, 700)])
+def test_head_sizes_that_fill_no_tile(F, dtype, dk, dv, T):
+    g = gen(41)
+    q, k, v, go = (randn(g, 2, T, 3, d, dtype=dtype) for d in (dk, dk, dv, dv))
+    ld, scale, s0 = decays(3), dk ** -0.5, randn(g, 2, 3, dk, dv)
+    lengths = torch.tensor([T, max(1, T - 5)], device="cuda", dtype=torch.int32)
+    o, s = F.linear_attention(q, k, v, ld, initial_state=s0, lengths=lengths, return_state=True)
+    eo, es = attention64(q, k, v, ld, scale, s0, lengths)
+    mo, ms = attention64(q, k, v, ld, scale, s0, lengths, absolute=True)
+    close(o, eo, bound(dtype, T, mo) + 2.0 ** -25, "o")
+    close(s, es, state_bound(T, ms), "state")
+    got = F.linear_attention_backward(go, q, k, v, ld, initial_state=s0, lengths=lengths)
+    exp = attention64(q, k, v, ld, scale, s0, lengths, go)
+    maj = attention64(q, k, v, ld, scale, s0, lengths, go, absolute=True)
+    for n, a, e, m in zip(("dq", "dk", "dv"), got, exp, maj):
+        close(a, e, bound(dtype, T, m, 3) + 2.0 ** -25, n)
+    close(got[3], exp[3], state_bound(T, maj[3]), "ds0")
+    F.check_operators()
+
+
+def test_operators_in_a_cuda_graph(F):
+    """Captured after a first call (which sets the kernels up) and replayed on new contents of the same tensors."""
+    g = gen(43)
+    q, k, v = (randn(g, 1, 700, 2, 64, dtype=torch.bfloat16) for _ in range(3))
+    x, y = randn(g, 700, 128, dtype=torch.bfloat16), randn(g, 700, 128, dtype=torch.bfloat16)
+    w, ld = torch.ones(128, device="cuda"), decays(2)
+
+    def work():
+        o, s = F.linear_attention(q, k, v, ld, return_state=True)
+        u, n, saved = F.gated_residual_norm(x, y, post_weight=w, pre_weight=w, save="int8")
+        return (o, s, u, n, *F.linear_attention_backward(o, q, k, v, ld)[:3], F.gated_residual_norm_backward(u, n, saved).y)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for t in (q, k, v, x, y):
+        t.copy_(randn(g, *t.shape, dtype=t.dtype))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(out, work()):
+        assert torch.equal(a, b)
+
+
+def test_calls_from_several_threads(F):
+    """Each thread on its own stream, sizes apart, results as alone."""
+    import threading
+    sizes = [(1, 300, 2, 64), (2, 1500, 1, 128), (1, 4000, 3, 64), (3, 90, 2, 32)]
+    ins = [[randn(gen(50 + i), *s, dtype=torch.bfloat16) for _ in range(3)] for i, s in enumerate(sizes)]
+    alone = [F.linear_attention(*x, decays(x[0].shape[2])) for x in ins]
+    torch.cuda.synchronize()
+    got, bad = [None] * len(ins), []
+
+    def go(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i] = F.linear_attention(*ins[i], decays(ins[i][0].shape[2]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+    ts = [threading.Thread(target=go, args=(i,)) for i in range(len(ins))]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad, bad
+    for a, b in zip(got, alone):
+        assert torch.equal(a, b)
