@@ -99,17 +99,27 @@ struct Fetch {
 };
 template <class T>
 __device__ __noinline__ void load_elements(uint32_t dst, const T* base, long long stride, int n, int left) {
+  // one at a time, 4 heads of 33, 8192 tokens, fp32, forward and backward took 420 us, not 247
+  constexpr int BATCH = 16;  // loads in flight
 #pragma unroll 1
-  for (int i = threadIdx.x; i < CH * 64; i += THREADS) {
-    const int row = i >> 6, col = i & 63;
-    float v = row < n && col < left ? to_float(base[row * stride + col]) : 0.f;
+  for (int i0 = threadIdx.x; i0 < CH * 64; i0 += BATCH * THREADS) {
+    float v[BATCH];
 #pragma unroll
-    for (int p = 0; p < Parts<T>::N; p++) {
-      const __nv_bfloat16 h = __float2bfloat16_rn(v);
-      asm volatile("st.shared.b16 [%0], %1;" ::"r"(dst + p * TILE + swz(row, col >> 3) + (col & 7) * 2),
-                   "h"(__bfloat16_as_ushort(h))
-                   : "memory");
-      v -= __bfloat162float(h);
+    for (int k = 0; k < BATCH; k++) {
+      const int i = i0 + k * THREADS, row = i >> 6, col = i & 63;
+      v[k] = row < n && col < left ? to_float(base[row * stride + col]) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < BATCH; k++) {
+      const int i = i0 + k * THREADS, row = i >> 6, col = i & 63;
+#pragma unroll
+      for (int p = 0; p < Parts<T>::N; p++) {
+        const __nv_bfloat16 h = __float2bfloat16_rn(v[k]);
+        asm volatile("st.shared.b16 [%0], %1;" ::"r"(dst + p * TILE + swz(row, col >> 3) + (col & 7) * 2),
+                     "h"(__bfloat16_as_ushort(h))
+                     : "memory");
+        v[k] -= __bfloat162float(h);
+      }
     }
   }
 }
@@ -155,7 +165,10 @@ struct Plan {
   static constexpr uint32_t bytes() { return E + EP * ETILE + 1024; }
 };
 
-template <class T, bool OUT>
+// ALIGNED: all of a, b and c come in groups of 8.  A kernel of its own, since
+// the call for single elements takes registers from the others (4 heads of 64,
+// 8192 tokens, fp32, forward and backward: 159 us against 184).
+template <class T, bool OUT, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Set set) {
   using PL = Plan<T>;
   constexpr int NP = PL::NP, EP = PL::EP;
@@ -246,14 +259,15 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Set 
   auto at_tile = [&](const Operand& o, long long first, int d0) {
     return static_cast<const T*>(o.p) + batch * o.sb + (head / o.per) * o.sh + first * o.st + d0;
   };
+  auto vec = [](const Operand& o) { return ALIGNED || o.vec; };
   Fetch<T> fa, fb, fc;
   auto fetch = [&](int pos, int s) {  // the tiles of the chunk at pos and slab s
     const int n = min(CH, len - pos);
     if (n <= 0) return;
     const long long first = first_of(pos);
-    if (OUT && r.a.vec) fa.load(at_tile(r.a, first, s * 64), step * r.a.st, n, r.da - s * 64);
-    if (r.b.vec) fb.load(at_tile(r.b, first, s * 64), step * r.b.st, n, r.da - s * 64);
-    if (s == 0 && r.c.vec) fc.load(at_tile(r.c, first, blk * 64), step * r.c.st, n, r.dc - blk * 64);
+    if (OUT && vec(r.a)) fa.load(at_tile(r.a, first, s * 64), step * r.a.st, n, r.da - s * 64);
+    if (vec(r.b)) fb.load(at_tile(r.b, first, s * 64), step * r.b.st, n, r.da - s * 64);
+    if (s == 0 && vec(r.c)) fc.load(at_tile(r.c, first, blk * 64), step * r.c.st, n, r.dc - blk * 64);
   };
   fetch(p0, 0);
 #pragma unroll 1
@@ -263,7 +277,7 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Set 
     if (n <= 0) break;
     const bool last = pos + n == len;
     const long long first = first_of(pos);
-    if (r.c.vec)
+    if (vec(r.c))
       fc.store(smem + PL::C);
     else
       load_elements<T>(smem + PL::C, at_tile(r.c, first, blk * 64), step * r.c.st, n, r.dc - blk * 64);
@@ -280,12 +294,12 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Set 
 #pragma unroll
           for (int p = 0; p < EP; p++) sts16(smem + PL::E + p * ETILE + swz(srow, (scol >> 3) + h), parts[p]);
         }
-        if (r.a.vec)
+        if (vec(r.a))
           fa.store(smem + PL::A);
         else
           load_elements<T>(smem + PL::A, at_tile(r.a, first, s * 64), step * r.a.st, n, r.da - s * 64);
       }
-      if (r.b.vec)
+      if (vec(r.b))
         fb.store(smem + PL::B);
       else
         load_elements<T>(smem + PL::B, at_tile(r.b, first, s * 64), step * r.b.st, n, r.da - s * 64);
@@ -559,20 +573,23 @@ __global__ void k_share(const __grid_constant__ Share s) {
   }
 }
 
-template <class T, bool OUT>
+template <class T, bool OUT, bool ALIGNED>
 cudaError_t launch_chunks(const Set& set, cudaStream_t st) {
   const uint32_t bytes = Plan<T>::bytes();
   static SmemLimit limit;
-  const cudaError_t ce = limit.reach(k_chunks<T, OUT>, (int)bytes);
+  const cudaError_t ce = limit.reach(k_chunks<T, OUT, ALIGNED>, (int)bytes);
   if (ce != cudaSuccess) return ce;
   const int nseg = set.run[0].nseg;
-  return launch_chained(k_chunks<T, OUT>, dim3((unsigned)ctas(set, OUT ? nseg : nseg - 1)), THREADS, bytes, st, set);
+  const dim3 grid((unsigned)ctas(set, OUT ? nseg : nseg - 1));
+  return launch_chained(k_chunks<T, OUT, ALIGNED>, grid, THREADS, bytes, st, set);
 }
 template <bool OUT>
 cudaError_t launch_chunks(const Set& set, int dtype, cudaStream_t st) {
-  return dtype == LAMA_F32   ? launch_chunks<float, OUT>(set, st)
-         : dtype == LAMA_F16 ? launch_chunks<__half, OUT>(set, st)
-                             : launch_chunks<__nv_bfloat16, OUT>(set, st);
+  bool vec = true;
+  for (int w = 0; w < set.n; w++) vec = vec && (!OUT || set.run[w].a.vec) && set.run[w].b.vec && set.run[w].c.vec;
+  if (dtype == LAMA_F16) return launch_chunks<__half, OUT, false>(set, st);
+  if (dtype == LAMA_BF16) return launch_chunks<__nv_bfloat16, OUT, false>(set, st);
+  return vec ? launch_chunks<float, OUT, true>(set, st) : launch_chunks<float, OUT, false>(set, st);
 }
 cudaError_t launch_scan(const Set& set, cudaStream_t st) {
   int per = 0;

@@ -13,12 +13,18 @@ constexpr int MAX_C = 16384;
 
 int teams(int c) { return c <= 512 ? 4 : c <= 1024 ? 2 : 1; }
 
-// CTAs of a set of rows: `most` CTAs in all where there are rows enough.
+// CTAs of a set of rows: `most_ctas` in all where there are rows enough, fewer
+// of the wide ones, which a SM holds fewer of and which fill longer tables of
+// factors (2000 x 8000, bf16, forward and backward: 169 us, 247 with as many).
 void split(const lama_norm* p, int most_ctas, int& sets, int& parts) {
   const bool set_gate = p->gate && p->gate_rows > 1;
   sets = set_gate ? (int)((p->rows + p->gate_rows - 1) / p->gate_rows) : 1;
   const long long rows = set_gate ? std::min<long long>(p->gate_rows, p->rows) : p->rows;
   const long long most = (rows + teams(p->channels) - 1) / teams(p->channels);
+  if (p->channels > 4096)
+    most_ctas = 148;
+  else if (p->channels > 2048)
+    most_ctas = 148 * 2;
   parts = (int)std::max<long long>(1, std::min<long long>(most, most_ctas / sets));
 }
 constexpr int FWD_CTAS = 148 * 5, BWD_CTAS = 148 * 4;

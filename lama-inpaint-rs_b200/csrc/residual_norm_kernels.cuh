@@ -582,10 +582,20 @@ __global__ void __launch_bounds__(1024) k_norm_sums(const __grid_constant__ Bwd 
     float a = 0.f, b = 0.f;
     if (on && set < p.sets) {
       const float* src = p.part + (long long)set * p.parts * 2 * p.c + c;
-#pragma unroll 8
-      for (int i = pi; i < p.parts; i += ps) {
-        a += src[(long long)i * 2 * p.c];
-        b += src[(long long)i * 2 * p.c + p.c];
+      constexpr int BATCH = 10;  // rows whose loads are in flight together
+      for (int i0 = pi; i0 < p.parts; i0 += BATCH * ps) {
+        float x[BATCH], y[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+          const int i = i0 + k * ps;
+          x[k] = i < p.parts ? src[(long long)i * 2 * p.c] : 0.f;
+          y[k] = i < p.parts ? src[(long long)i * 2 * p.c + p.c] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+          a += x[k];
+          b += y[k];
+        }
       }
     }
     sa[warp][lane] = a;
