@@ -26,10 +26,13 @@
 //
 // This file has the general kernel, `k_chunks` (fp32, and 16-bit rows that are
 // not 16-byte aligned), the scan and the host side; 16-bit aligned rows go
-// through the pipelined kernel of attention_pipe.cu.  k_chunks runs its steps one
-// after another, loads excepted; what bounds it is the chain of products and
-// conversions (fp32: six bf16 products for one, about 7000 clocks of MMAs a
-// chunk of 64-wide heads; 2 x 1521 tokens of 4 heads, forward and backward: 86 us).
+// through the pipelined kernel of attention_pipe.cu.  In k_chunks eight warps load
+// and convert one chunk after another, and a warp of its own issues the products,
+// since an issue waits for the products before it: the decayed operand is made
+// during the scores' products, the scores are rounded during those of the state
+// (one warp doing both: 91.7 -> 85.9 us for 2 x 1521 tokens of 4 heads of 64, fp32, forward
+// and backward).  What bounds it is a chunk's chain: loads, conversions, and for
+// fp32 six bf16 products for one (8000 clocks of MMAs of 21500 for one chunk).
 //
 // Precision (k_chunks).  Operands are carried as sums of bf16 parts, as in the
 // generator's convolutions: bf16 inputs are one part (exact), fp16 inputs two
@@ -52,7 +55,11 @@ namespace {
 
 __device__ int g_status;
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256;          // that work on tiles
+constexpr int ALL = THREADS + 128;    // with the warpgroup one warp of which issues k_chunks' products
+// Registers a thread: at launch, of the workers, of the other warpgroup.
+constexpr int LAUNCH_REGS = 168, WORK_REGS = 232, ISSUE_REGS = 40;
+static_assert(THREADS * WORK_REGS + (ALL - THREADS) * ISSUE_REGS <= ALL * LAUNCH_REGS, "registers");
 
 template <class T>
 struct Parts {
@@ -99,7 +106,8 @@ struct Fetch {
 };
 template <class T>
 __device__ __noinline__ void load_elements(uint32_t dst, const T* base, long long stride, int n, int left) {
-  // one at a time, 4 heads of 33, 8192 tokens, fp32, forward and backward took 420 us, not 247
+  // one at a time, 4 heads of 33, 8192 tokens, fp32, forward and backward took 420 us, not 247; inlined
+  // and with the issuing warp, bf16 takes 315 us, not 224
   constexpr int BATCH = 16;  // loads in flight
 #pragma unroll 1
   for (int i0 = threadIdx.x; i0 < CH * 64; i0 += BATCH * THREADS) {
@@ -154,38 +162,43 @@ template <class T>
 struct Plan {
   static constexpr int NP = Parts<T>::N;
   static constexpr int EP = NP == 1 ? 2 : NP;  // parts of the entering state
-  // a, b, c: NP tiles each; the decayed b: 3 tiles; the scores: 2 * NP tiles
-  // over the decayed b (and, for fp32 inputs, which have no room beside it,
-  // the decayed b over b and the scores over a and b); the entering state.
+  // a, b, c: NP tiles each; the decayed b: 3 tiles; the entering state.  The
+  // scores' 2 * NP tiles and then the chunk's outputs take the place of a and b.
   static constexpr uint32_t A = 0, B = NP * TILE, C = 2 * NP * TILE;
-  static constexpr uint32_t BD = NP == 3 ? B : 3 * NP * TILE;
-  static constexpr uint32_t P = NP == 3 ? A : BD;
-  static constexpr uint32_t W = NP == 3 ? 0 : (2 * NP > 3 ? 2 * NP : 3) * TILE;
-  static constexpr uint32_t E = 3 * NP * TILE + W;
+  static constexpr uint32_t P = A, O = A;
+  static constexpr uint32_t BD = 3 * NP * TILE;
+  static constexpr uint32_t E = BD + 3 * TILE;
   static constexpr uint32_t bytes() { return E + EP * ETILE + 1024; }
+  static_assert(bytes() <= 227 * 1024 && CH * 64 * 4 <= C, "shared memory");
 };
 
 // ALIGNED: all of a, b and c come in groups of 8.  A kernel of its own, since
 // the call for single elements takes registers from the others (4 heads of 64,
-// 8192 tokens, fp32, forward and backward: 159 us against 184).
+// 8192 tokens, fp32, forward and backward: 159 us against 184 before the issuing warp).
 template <class T, bool OUT, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Set set) {
+__global__ void __launch_bounds__(ALL, 1) k_chunks(const __grid_constant__ Set set) {
   using PL = Plan<T>;
   constexpr int NP = PL::NP, EP = PL::EP;
   constexpr int MAXS = 2;
   extern __shared__ uint8_t raw[];
   __shared__ float pw[CH + 1];
-  __shared__ uint64_t bar_mem;
+  __shared__ uint64_t bar_mem[5];
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
-  const uint32_t bar = smem_u32(&bar_mem);
+  // products done, and operands ready for them (an arrival a warp)
+  const uint32_t bar_p = smem_u32(&bar_mem[0]), bar_u = smem_u32(&bar_mem[1]);
+  const uint32_t rdy_s = smem_u32(&bar_mem[2]), rdy_u = smem_u32(&bar_mem[3]), rdy_p = smem_u32(&bar_mem[4]);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   pdl_launch_dependents();
   if (warp == 0) tmem_alloc(smem_u32(&tmem_slot), 256);
   if (tid == 0) {
-    mbar_init(bar, 1);
+    mbar_init(bar_p, 1);
+    mbar_init(bar_u, 1);
+    mbar_init(rdy_s, THREADS / 32);
+    mbar_init(rdy_u, THREADS / 32);
+    mbar_init(rdy_p, THREADS / 32);
     fence_mbar_init();
     failed = 0;
   }
@@ -206,7 +219,7 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Set 
   const int seg_tokens = r.chunks * CH;
   const int p0 = seg * seg_tokens;
 
-  for (int i = tid; i <= CH; i += THREADS) pw[i] = power(g, i);
+  if (tid <= CH) pw[tid] = power(g, tid);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -217,272 +230,323 @@ __global__ void __launch_bounds__(THREADS) k_chunks(const __grid_constant__ Set 
   const int srow = row & 63;                         // state row of a slab
   const int scol = ((warp >> 2) * 2 + (row >> 6)) * 16;  // its 16 columns
 
-  // the carried state: 16 columns of row srow of each slab
-  float E[MAXS][16];
-  const int ld = r.blocks * 64;
-  const float lam = pw[1];
-  const long long bh = (long long)batch * r.heads + head;
-#pragma unroll
-  for (int s = 0; s < MAXS; s++) {
-    const int er = s * 64 + srow, ec = blk * 64 + scol;
-    const float* src = nullptr;
-    long long step = 1;
-    int cols = 0;
-    float f = 1.f;
-    if (OUT && s < r.slabs) {
-      if (r.staged) {
-        src = r.seg + (bh * r.nseg + seg) * (r.slabs * 64 * ld) + er * r.sr + ec * r.sc;
-        step = r.sc;
-        cols = 16;
-      } else if (r.init && er < r.da) {
-        src = r.init + bh * r.da * r.dc + er * r.ir + ec * r.ic;
-        step = r.ic;
-        cols = r.dc - ec;
-        if (!r.reverse) f = lam;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 16; i++, src += step) E[s][i] = i < cols ? f * *src : 0.f;
-  }
-
-  uint32_t phase = 0;
   bool ok = true;
-  int done = 0;  // tokens of this segment so far
-  const int step = r.reverse ? -1 : 1;
-  auto wait = [&](int code) {
-    ok = __syncthreads_and(mbar_wait(bar, phase, &failed, code));
-    phase ^= 1;
-    tc_fence_after();
-    return ok;
-  };
-  auto first_of = [&](int pos) { return r.reverse ? (long long)len - 1 - pos : (long long)pos; };
-  auto at_tile = [&](const Operand& o, long long first, int d0) {
-    return static_cast<const T*>(o.p) + batch * o.sb + (head / o.per) * o.sh + first * o.st + d0;
-  };
-  auto vec = [](const Operand& o) { return ALIGNED || o.vec; };
-  Fetch<T> fa, fb, fc;
-  auto fetch = [&](int pos, int s) {  // the tiles of the chunk at pos and slab s
-    const int n = min(CH, len - pos);
-    if (n <= 0) return;
-    const long long first = first_of(pos);
-    if (OUT && vec(r.a)) fa.load(at_tile(r.a, first, s * 64), step * r.a.st, n, r.da - s * 64);
-    if (vec(r.b)) fb.load(at_tile(r.b, first, s * 64), step * r.b.st, n, r.da - s * 64);
-    if (s == 0 && vec(r.c)) fc.load(at_tile(r.c, first, blk * 64), step * r.c.st, n, r.dc - blk * 64);
-  };
-  fetch(p0, 0);
+  if (warp >= THREADS / 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ISSUE_REGS));
+  if (warp == THREADS / 32) {
+    // The issuing warp: a product's issue waits for the products before it, and
+    // the other warps' conversions pass meanwhile.
+    const int chunks = min(r.chunks, (max(len - p0, 0) + CH - 1) / CH);
+    uint32_t phase_s = 0, phase_p = 0;
+    const bool leader = elect_one();
+    auto ready = [&](uint32_t bar, uint32_t phase, int code) {
+      ok = __all_sync(~0u, mbar_wait(bar, phase, &failed, code));
+      tc_fence_after();
+      return ok;
+    };
 #pragma unroll 1
-  for (int ch = 0; ok && ch < r.chunks; ch++) {
-    const int pos = p0 + ch * CH;
-    const int n = min(CH, len - pos);
-    if (n <= 0) break;
-    const bool last = pos + n == len;
-    const long long first = first_of(pos);
-    if (vec(r.c))
-      fc.store(smem + PL::C);
-    else
-      load_elements<T>(smem + PL::C, at_tile(r.c, first, blk * 64), step * r.c.st, n, r.dc - blk * 64);
-#pragma unroll 1
-    for (int s = 0; s < r.slabs; s++) {
-      float e[16];
-#pragma unroll
-      for (int i = 0; i < 16; i++) e[i] = s ? E[1][i] : E[0][i];
-      if (OUT) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          uint4 parts[EP];
-          split8<EP>(e + h * 8, parts);
-#pragma unroll
-          for (int p = 0; p < EP; p++) sts16(smem + PL::E + p * ETILE + swz(srow, (scol >> 3) + h), parts[p]);
-        }
-        if (vec(r.a))
-          fa.store(smem + PL::A);
-        else
-          load_elements<T>(smem + PL::A, at_tile(r.a, first, s * 64), step * r.a.st, n, r.da - s * 64);
-      }
-      if (vec(r.b))
-        fb.store(smem + PL::B);
-      else
-        load_elements<T>(smem + PL::B, at_tile(r.b, first, s * 64), step * r.b.st, n, r.da - s * 64);
-      if (s + 1 < r.slabs)
-        fetch(pos, s + 1);
-      else if (ch + 1 < r.chunks)
-        fetch(pos + CH, 0);
-      // scores and a E before b's place may be taken by the decayed b
-      auto scores = [&] {
-        tc_fence_after();
+    for (int i = 0, s = 0; i < chunks * r.slabs; i++) {
+      const bool last_slab = s + 1 == r.slabs;
+      if (!ready(rdy_s, phase_s, 4)) break;
+      if (OUT && leader) {  // the scores and a E
         mma_parts<NP, NP>(t_p, smem_desc(smem + PL::A, 1024, 2), smem_desc(smem + PL::B, 1024, 2), idesc_bf16_f32(128),
                           1, 32, 0, TILE, 32, 0, TILE, s > 0);
         mma_parts<NP, EP>(t_o, smem_desc(smem + PL::A, 1024, 2), desc_mn(smem + PL::E, 0), idesc_bf16_f32(64) | B_MN, 1,
                           32, 0, TILE, 2048, 0, ETILE, s > 0);
-      };
-      if (OUT && NP == 3) {
-        fence_async_smem();
-        __syncthreads();
-        if (warp == 0 && elect_one()) {
-          scores();
-          mma_commit(bar);
-        }
-        __syncwarp();
-        if (!wait(1)) break;
-      } else {
-        __syncthreads();
+        if (last_slab) mma_commit(bar_p);
       }
-      // decayed b: row j times lam^{n-1-j}, three parts
-#pragma unroll 2
-      for (int it = 0; it < CH * 8 / THREADS; it++) {
-        const int c = it * THREADS + tid, j = c >> 3, ck = c & 7;
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = 0.f;
-#pragma unroll
-        for (int p = 0; p < NP; p++) {
-          const uint4 u = lds16(smem + PL::B + p * TILE + swz(j, ck));
-          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&u);
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            v[2 * i] += __low2float(x[i]);
-            v[2 * i + 1] += __high2float(x[i]);
-          }
-        }
-        const float w = j < n ? pw[n - 1 - j] : 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = j < n ? v[i] * w : 0.f;
-        uint4 parts[3];
-        split8<3>(v, parts);
-#pragma unroll
-        for (int p = 0; p < 3; p++) sts16(smem + PL::BD + p * TILE + swz(j, ck), parts[p]);
-      }
-      fence_async_smem();
-      __syncthreads();
-      if (warp == 0 && elect_one()) {
-        tc_fence_after();
-        if (OUT && NP != 3) scores();
+      __syncwarp();
+      if (!ready(rdy_u, phase_s, 5)) break;
+      if (leader) {
         // both 64-row halves of the MMA's 128 rows read the slab's 64 columns
         mma_parts<3, NP>(t_u, desc_mn(smem + PL::BD, 0), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | A_MN | B_MN, 2,
                          2048, 8192, TILE, 2048, 8192, TILE, false);
-        mma_commit(bar);
+        mma_commit(bar_u);
       }
       __syncwarp();
-      if (!wait(2)) break;
-      float u[16];
-      tmem_ld16(t_u + lane_base + scol, u);
-      tmem_wait_ld();
-      const float dn1 = pw[n - 1];
-#pragma unroll
-      for (int i = 0; i < 16; i++) e[i] = dn1 * e[i] + r.update * u[i];  // the state after the chunk
-      if (OUT && last && r.fin) {
-        const int er = s * 64 + srow, ec = blk * 64 + scol;
-        float* dst = r.fin + bh * r.da * r.dc + er * r.fr + ec * r.fc;
-#pragma unroll
-        for (int i = 0; i < 16; i++, dst += r.fc)
-          if (er < r.da && ec + i < r.dc) *dst = r.reverse ? lam * e[i] : e[i];
+      phase_s ^= 1;
+      if (OUT && last_slab) {
+        if (!ready(rdy_p, phase_p, 6)) break;
+        if (leader) {
+          mma_parts<NP, NP>(t_p, smem_desc(smem + PL::P, 1024, 2), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | B_MN, 2,
+                            32, TILE, 2 * TILE, 2048, 8192, TILE, false);
+          mma_commit(bar_p);
+        }
+        __syncwarp();
+        phase_p ^= 1;
       }
-      const float f = OUT || ch + 1 < r.chunks ? lam : 1.f;
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        e[i] *= f;
-        if (s)
-          E[1][i] = e[i];
-        else
-          E[0][i] = e[i];
-      }
-      tc_fence_before();
-      __syncthreads();  // the next slab's tiles and accumulator
+      s = last_slab ? 0 : s + 1;
     }
-    if (!ok) break;
-    done = pos + n - p0;
-    if (OUT) {
-      // scores: decay and causal mask, rounded to NP parts
-#pragma unroll 1
-      for (int h = 0; h < 2; h++) {
-        const int col0 = (warp >> 2) * 64 + h * 32;
-        float v[32];
-        tmem_ld32(t_p + lane_base + col0, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 32; j++) {
-          const int dist = row - (col0 + j);
-          v[j] = dist >= 0 ? v[j] * pw[max(dist, 0)] : 0.f;
-        }
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          uint4 parts[NP];
-          split8<NP>(v + q * 8, parts);
-#pragma unroll
-          for (int p = 0; p < NP; p++)
-            sts16(smem + PL::P + (p * 2 + (warp >> 2)) * TILE + swz(row, h * 4 + q), parts[p]);
-        }
-      }
+  } else if (warp < THREADS / 32) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(WORK_REGS));
+    uint32_t phase_p = 0, phase_u = 0;
+    bool pending_p = false, pending_u = false;  // products committed and not waited for
+    int done = 0;  // tokens of this segment so far
+    const int step = r.reverse ? -1 : 1;
+    auto wait = [&](uint32_t bar, uint32_t& phase, bool& pending, int code) {
+      ok = named_sync_and(1, THREADS, mbar_wait(bar, phase, &failed, code));
+      if (ok) phase ^= 1, pending = false;
+      tc_fence_after();
+      return ok;
+    };
+    // what this thread wrote (and its TMEM loads) before products that the other warp issues
+    auto hand_over = [&](uint32_t bar) {
       tc_fence_before();
       fence_async_smem();
-      __syncthreads();
-      if (warp == 0 && elect_one()) {
-        tc_fence_after();
-        mma_parts<NP, NP>(t_p, smem_desc(smem + PL::P, 1024, 2), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | B_MN, 2,
-                          32, TILE, 2 * TILE, 2048, 8192, TILE, false);
-        mma_commit(bar);
-      }
       __syncwarp();
-      if (!wait(3)) break;
-      const float di = pw[row] * r.inter;
-      const long long at = batch * r.ob + (first + (long long)row * step) * r.ot + head * r.oh + blk * 64;
-#pragma unroll 1
-      for (int h = 0; h < 2; h++) {
-        const int col0 = (warp >> 2) * 32 + h * 16, left = r.dc - blk * 64 - col0;
-        float x[16], y[16];
-        tmem_ld16(t_o + lane_base + col0, x);
-        tmem_ld16(t_p + lane_base + col0, y);
-        tmem_wait_ld();
-        if (row >= n) continue;
-#pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = di * x[i] + r.intra * y[i];
-#pragma unroll
-        for (int i = 0; i < 16; i += 8)
-          if (r.out_f32)
-            store_row(static_cast<float*>(r.out) + at + col0 + i, x + i, left - i, r.out_vec);
-          else
-            store_row(static_cast<T*>(r.out) + at + col0 + i, x + i, left - i, r.out_vec);
-      }
-      tc_fence_before();
-      __syncthreads();  // the next chunk's tiles
-    }
-  }
+      if (lane == 0) mbar_arrive(bar);
+    };
+    auto first_of = [&](int pos) { return r.reverse ? (long long)len - 1 - pos : (long long)pos; };
+    auto at_tile = [&](const Operand& o, long long first, int d0) {
+      return static_cast<const T*>(o.p) + batch * o.sb + (head / o.per) * o.sh + first * o.st + d0;
+    };
+    auto vec = [](const Operand& o) { return ALIGNED || o.vec; };
+    Fetch<T> fa, fb, fc;
+    auto fetch = [&](int pos, int s) {  // the tiles of the chunk at pos and slab s
+      const int n = min(CH, len - pos);
+      if (n <= 0) return;
+      const long long first = first_of(pos);
+      if (OUT && vec(r.a)) fa.load(at_tile(r.a, first, s * 64), step * r.a.st, n, r.da - s * 64);
+      if (vec(r.b)) fb.load(at_tile(r.b, first, s * 64), step * r.b.st, n, r.da - s * 64);
+      if (s == 0 && vec(r.c)) fc.load(at_tile(r.c, first, blk * 64), step * r.c.st, n, r.dc - blk * 64);
+    };
+    fetch(p0, 0);
 
-  if (ok && OUT) {
-    // tokens past the sequence's end
-    const int end = min(p0 + seg_tokens, r.tokens);
-    const int width = min(64, r.dc - blk * 64);
-#pragma unroll 1
-    for (int i = tid; i < (end - p0 - done) * 64; i += THREADS) {
-      const int t = p0 + done + (i >> 6), c = i & 63;
-      if (c >= width) continue;
-      const long long at = batch * r.ob + (long long)t * r.ot + head * r.oh + blk * 64 + c;
-      if (r.out_f32)
-        static_cast<float*>(r.out)[at] = 0.f;
-      else
-        static_cast<T*>(r.out)[at] = from_float<T>(0.f);
-    }
-    if (len == 0 && seg == 0 && r.fin) {
-#pragma unroll 1
-      for (int i = tid; i < r.da * 64; i += THREADS) {
-        const int er = i >> 6, ec = blk * 64 + (i & 63);
-        const long long base = bh * r.da * r.dc;
-        if (ec < r.dc) r.fin[base + er * r.fr + ec * r.fc] = r.init ? r.init[base + er * r.ir + ec * r.ic] : 0.f;
-      }
-    }
-  }
-  if (ok && !OUT) {
+    // the carried state: 16 columns of row srow of each slab
+    float E[MAXS][16];
+    const int ld = r.blocks * 64;
+    const float lam = pw[1];
+    const long long bh = (long long)batch * r.heads + head;
 #pragma unroll
     for (int s = 0; s < MAXS; s++) {
-      if (s >= r.slabs) break;
-      float* dst = r.seg + ((bh * r.nseg + seg) * (r.slabs * 64) + s * 64 + srow) * ld + blk * 64 + scol;
+      const int er = s * 64 + srow, ec = blk * 64 + scol;
+      const float* src = nullptr;
+      long long step = 1;
+      int cols = 0;
+      float f = 1.f;
+      if (OUT && s < r.slabs) {
+        if (r.staged) {
+          src = r.seg + (bh * r.nseg + seg) * (r.slabs * 64 * ld) + er * r.sr + ec * r.sc;
+          step = r.sc;
+          cols = 16;
+        } else if (r.init && er < r.da) {
+          src = r.init + bh * r.da * r.dc + er * r.ir + ec * r.ic;
+          step = r.ic;
+          cols = r.dc - ec;
+          if (!r.reverse) f = lam;
+        }
+      }
+      if (cols == 16 && step == 1 && r.staged) {
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(E[s][i], E[s][i + 1], E[s][i + 2], E[s][i + 3]);
+        for (int i = 0; i < 16; i += 4) load_vec<float, 4>(src + i, &E[s][i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++, src += step) E[s][i] = i < cols ? f * *src : 0.f;
+      }
     }
-  }
-  if (!ok) {
-    mbar_wait_drain(bar, phase ^ 1);  // the products still in flight
-    if (tid == 0) atomicCAS(r.status, 0, failed);
+
+#pragma unroll 1
+    for (int ch = 0; ok && ch < r.chunks; ch++) {
+      const int pos = p0 + ch * CH;
+      const int n = min(CH, len - pos);
+      if (n <= 0) break;
+      const bool last = pos + n == len;
+      const long long first = first_of(pos);
+      if (vec(r.c))
+        fc.store(smem + PL::C);
+      else
+        load_elements<T>(smem + PL::C, at_tile(r.c, first, blk * 64), step * r.c.st, n, r.dc - blk * 64);
+#pragma unroll 1
+      for (int s = 0; s < r.slabs; s++) {
+        if (OUT) {
+          float e[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) e[i] = s ? E[1][i] : E[0][i];
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            uint4 parts[EP];
+            split8<EP>(e + h * 8, parts);
+#pragma unroll
+            for (int p = 0; p < EP; p++) sts16(smem + PL::E + p * ETILE + swz(srow, (scol >> 3) + h), parts[p]);
+          }
+          if (vec(r.a))
+            fa.store(smem + PL::A);
+          else
+            load_elements<T>(smem + PL::A, at_tile(r.a, first, s * 64), step * r.a.st, n, r.da - s * 64);
+        }
+        if (vec(r.b))
+          fb.store(smem + PL::B);
+        else
+          load_elements<T>(smem + PL::B, at_tile(r.b, first, s * 64), step * r.b.st, n, r.da - s * 64);
+        if (s + 1 < r.slabs)
+          fetch(pos, s + 1);
+        else if (ch + 1 < r.chunks)
+          fetch(pos + CH, 0);
+        const bool last_slab = s + 1 == r.slabs;
+        hand_over(rdy_s);
+        pending_p = OUT && last_slab;
+        if (!vec(r.b)) named_sync(1, THREADS);  // below, a thread reads groups of b, those that it stored itself
+        // decayed b: row j times lam^{n-1-j}, three parts
+#pragma unroll 2
+        for (int it = 0; it < CH * 8 / THREADS; it++) {
+          const int c = it * THREADS + tid, j = c >> 3, ck = c & 7;
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) v[i] = 0.f;
+#pragma unroll
+          for (int p = 0; p < NP; p++) {
+            const uint4 u = lds16(smem + PL::B + p * TILE + swz(j, ck));
+            const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&u);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              v[2 * i] += __low2float(x[i]);
+              v[2 * i + 1] += __high2float(x[i]);
+            }
+          }
+          const float w = j < n ? pw[n - 1 - j] : 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) v[i] = j < n ? v[i] * w : 0.f;
+          uint4 parts[3];
+          split8<3>(v, parts);
+#pragma unroll
+          for (int p = 0; p < 3; p++) sts16(smem + PL::BD + p * TILE + swz(j, ck), parts[p]);
+        }
+        hand_over(rdy_u);
+        pending_u = true;
+        if (OUT && last_slab) {
+          // scores: decay and causal mask, rounded to NP parts
+          if (!wait(bar_p, phase_p, pending_p, 1)) break;
+#pragma unroll 1
+          for (int h = 0; h < 2; h++) {
+            const int col0 = (warp >> 2) * 64 + h * 32;
+            float v[32];
+            tmem_ld32(t_p + lane_base + col0, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              const int dist = row - (col0 + j);
+              v[j] = dist >= 0 ? v[j] * pw[max(dist, 0)] : 0.f;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+              uint4 parts[NP];
+              split8<NP>(v + q * 8, parts);
+#pragma unroll
+              for (int p = 0; p < NP; p++)
+                sts16(smem + PL::P + (p * 2 + (warp >> 2)) * TILE + swz(row, h * 4 + q), parts[p]);
+            }
+          }
+          hand_over(rdy_p);
+          pending_p = true;
+        }
+        if (!wait(bar_u, phase_u, pending_u, 2)) break;
+        float e[16], u[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) e[i] = s ? E[1][i] : E[0][i];
+        tmem_ld16(t_u + lane_base + scol, u);
+        tmem_wait_ld();
+        const float dn1 = pw[n - 1];
+#pragma unroll
+        for (int i = 0; i < 16; i++) e[i] = dn1 * e[i] + r.update * u[i];  // the state after the chunk
+        if (OUT && last && r.fin) {
+          const int er = s * 64 + srow, ec = blk * 64 + scol;
+          float* dst = r.fin + bh * r.da * r.dc + er * r.fr + ec * r.fc;
+#pragma unroll
+          for (int i = 0; i < 16; i++, dst += r.fc)
+            if (er < r.da && ec + i < r.dc) *dst = r.reverse ? lam * e[i] : e[i];
+        }
+        const float f = OUT || ch + 1 < r.chunks ? lam : 1.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          e[i] *= f;
+          if (s)
+            E[1][i] = e[i];
+          else
+            E[0][i] = e[i];
+        }
+      }
+      if (!ok) break;
+      done = pos + n - p0;
+      if (OUT) {
+        if (!wait(bar_p, phase_p, pending_p, 3)) break;
+        const float di = pw[row] * r.inter;
+        // through shared memory, so that eight threads write a row's 64 columns
+#pragma unroll 1
+        for (int h = 0; h < 2; h++) {
+          const int col0 = (warp >> 2) * 32 + h * 16;
+          float x[16], y[16];
+          tmem_ld16(t_o + lane_base + col0, x);
+          tmem_ld16(t_p + lane_base + col0, y);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            uint4 w;
+            w.x = __float_as_uint(di * x[i] + r.intra * y[i]);
+            w.y = __float_as_uint(di * x[i + 1] + r.intra * y[i + 1]);
+            w.z = __float_as_uint(di * x[i + 2] + r.intra * y[i + 2]);
+            w.w = __float_as_uint(di * x[i + 3] + r.intra * y[i + 3]);
+            sts16(smem + PL::O + row * 256 + ((((col0 + i) >> 2) ^ (row & 7)) << 4), w);
+          }
+        }
+        named_sync(1, THREADS);
+#pragma unroll 1
+        for (int it = 0; it < CH * 8 / THREADS; it++) {
+          const int c = it * THREADS + tid, j = c >> 3, ck = c & 7, left = r.dc - blk * 64 - ck * 8;
+          if (j >= n) break;
+          float v[8];
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const uint4 w = lds16(smem + PL::O + j * 256 + (((ck * 2 + h) ^ (j & 7)) << 4));
+            v[4 * h] = __uint_as_float(w.x), v[4 * h + 1] = __uint_as_float(w.y);
+            v[4 * h + 2] = __uint_as_float(w.z), v[4 * h + 3] = __uint_as_float(w.w);
+          }
+          const long long at = batch * r.ob + (first + (long long)j * step) * r.ot + head * r.oh + blk * 64 + ck * 8;
+          if (r.out_f32)
+            store_row(static_cast<float*>(r.out) + at, v, left, r.out_vec);
+          else
+            store_row(static_cast<T*>(r.out) + at, v, left, r.out_vec);
+        }
+        named_sync(1, THREADS);  // the next chunk's tiles
+      }
+    }
+
+    if (ok && OUT) {
+      // tokens past the sequence's end
+      const int end = min(p0 + seg_tokens, r.tokens);
+      const int width = min(64, r.dc - blk * 64);
+#pragma unroll 1
+      for (int i = tid; i < (end - p0 - done) * 64; i += THREADS) {
+        const int t = p0 + done + (i >> 6), c = i & 63;
+        if (c >= width) continue;
+        const long long at = batch * r.ob + (long long)t * r.ot + head * r.oh + blk * 64 + c;
+        if (r.out_f32)
+          static_cast<float*>(r.out)[at] = 0.f;
+        else
+          static_cast<T*>(r.out)[at] = from_float<T>(0.f);
+      }
+      if (len == 0 && seg == 0 && r.fin) {
+#pragma unroll 1
+        for (int i = tid; i < r.da * 64; i += THREADS) {
+          const int er = i >> 6, ec = blk * 64 + (i & 63);
+          const long long base = bh * r.da * r.dc;
+          if (ec < r.dc) r.fin[base + er * r.fr + ec * r.fc] = r.init ? r.init[base + er * r.ir + ec * r.ic] : 0.f;
+        }
+      }
+    }
+    if (ok && !OUT) {
+#pragma unroll
+      for (int s = 0; s < MAXS; s++) {
+        if (s >= r.slabs) break;
+        float* dst = r.seg + ((bh * r.nseg + seg) * (r.slabs * 64) + s * 64 + srow) * ld + blk * 64 + scol;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(E[s][i], E[s][i + 1], E[s][i + 2], E[s][i + 3]);
+      }
+    }
+    if (!ok) {
+      // the products still in flight
+      if (pending_p) mbar_wait_drain(bar_p, phase_p);
+      if (pending_u) mbar_wait_drain(bar_u, phase_u);
+      if (tid == 0) atomicCAS(r.status, 0, failed);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -579,9 +643,16 @@ cudaError_t launch_chunks(const Set& set, cudaStream_t st) {
   static SmemLimit limit;
   const cudaError_t ce = limit.reach(k_chunks<T, OUT, ALIGNED>, (int)bytes);
   if (ce != cudaSuccess) return ce;
+  // setmaxnreg.inc takes from the registers of the launch, and would wait for
+  // more than those for good
+  static const bool fits = [] {
+    cudaFuncAttributes a{};
+    return cudaFuncGetAttributes(&a, k_chunks<T, OUT, ALIGNED>) == cudaSuccess && a.numRegs >= LAUNCH_REGS;
+  }();
+  if (!fits) return cudaErrorLaunchOutOfResources;
   const int nseg = set.run[0].nseg;
   const dim3 grid((unsigned)ctas(set, OUT ? nseg : nseg - 1));
-  return launch_chained(k_chunks<T, OUT, ALIGNED>, grid, THREADS, bytes, st, set);
+  return launch_chained(k_chunks<T, OUT, ALIGNED>, grid, ALL, bytes, st, set);
 }
 template <bool OUT>
 cudaError_t launch_chunks(const Set& set, int dtype, cudaStream_t st) {
