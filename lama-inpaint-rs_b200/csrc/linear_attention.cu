@@ -571,38 +571,46 @@ __global__ void k_scan(const __grid_constant__ Set set) {
   const int bh = blockIdx.y, head = bh % r.heads, batch = bh / r.heads;
   const int er = (int)(i / cols), ec = (int)(i % cols);
   const bool inside = er < r.da && ec < r.dc;
+  float* p = r.seg + (long long)bh * r.nseg * per + i;
+  const int made = r.pipe && r.fin ? r.nseg : r.nseg - 1;  // segments whose states are there
+  // A batch is loaded before anything waits for a load, the next one before
+  // this one's places are written: the kernel is nothing but that latency.
+  constexpr int BATCH = 16;
+  float x[BATCH], next[BATCH];
+  auto load = [&](int s0, float* v) {
+#pragma unroll
+    for (int k = 0; k < BATCH; k++) v[k] = s0 + k < made ? p[(s0 + k) * per] : 0.f;
+  };
+  load(0, x);
+  float e = 0.f;  // the state that enters a segment
+  if (r.init && inside) e = r.init[(long long)bh * r.da * r.dc + er * r.ir + ec * r.ic];
   const float g = r.log_decay[head];
   int len = r.tokens;
   if (r.lengths) len = min(max(r.lengths[batch], 0), r.tokens);
   const float lam = power(g, 1);
-  const long long base = (long long)bh * r.da * r.dc;
-  float e = 0.f, after = 0.f;  // the state that enters a segment, and the one after the last token
-  if (r.init && inside) {
-    e = after = r.init[base + er * r.ir + ec * r.ic];
-    if (!r.reverse) e *= lam;
-  }
-  float* p = r.seg + (long long)bh * r.nseg * per + i;
   const int seg_tokens = r.chunks * CH;
-  const int made = r.pipe && r.fin ? r.nseg : r.nseg - 1;  // segments whose states are there
-  for (int s0 = 0; s0 < r.nseg; s0 += 8) {
-    float x[8];  // loaded ahead: the stores below go to the same array
+  const float through = power(g, seg_tokens - 1);
+  float after = e;  // the state after the last token
+  if (!r.reverse) e *= lam;
+  for (int s0 = 0; s0 < r.nseg; s0 += BATCH) {
+    if (s0 + BATCH < r.nseg) load(s0 + BATCH, next);
 #pragma unroll
-    for (int k = 0; k < 8; k++) x[k] = s0 + k < made ? p[(s0 + k) * per] : 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
+    for (int k = 0; k < BATCH; k++) {
       const int s = s0 + k;
       if (s >= r.nseg) break;
       const int seg = r.pipe && r.reverse ? r.nseg - 1 - s : s;
       const int n = min(max(len - seg * seg_tokens, 0), seg_tokens);
       p[s * per] = e;
       if (n > 0) {
-        after = x[k] + power(g, n - 1) * e;
+        after = x[k] + (n == seg_tokens ? through : power(g, n - 1)) * e;
         e = lam * after;
         if (r.reverse) after = e;
       }
     }
+#pragma unroll
+    for (int k = 0; k < BATCH; k++) x[k] = next[k];
   }
-  if (r.pipe && r.fin && inside) r.fin[base + er * r.fr + ec * r.fc] = after;
+  if (r.pipe && r.fin && inside) r.fin[(long long)bh * r.da * r.dc + er * r.fr + ec * r.fc] = after;
 }
 
 // Sum over the heads that share one head of an operand: src fp32
