@@ -93,6 +93,8 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, leng
     outputs are 0).  Returns o [B,T,H,dv], or (o, state after the last token) with return_state.
     """
     if _grad_enabled() and _learns(q, k, v, initial_state):
+        if _learns(log_decay):  # inside the function gradients are off, and the binding's own check with them
+            _refuse("log_decay has no gradient: the decays are constants of the layer")
         o, state = _LinearAttention.apply(q, k, v, log_decay, scale, initial_state, lengths)
     else:
         o, state = _native.attention(q, k, v, log_decay, scale, initial_state, lengths, bool(return_state))

@@ -1,0 +1,29 @@
+"""What the token-mixer operators refuse or pass on before any GPU is involved: autograd's demands on the
+Python side, pointers and sizes at the C ABI."""
+
+import pytest
+import torch
+
+from lama_b200 import LamaError
+
+EINVAL = -1
+
+
+def refused(f, msg):
+    with pytest.raises(LamaError) as ex:
+        f()
+    assert ex.value.code == EINVAL and msg in ex.value.msg, ex.value.msg
+
+
+# ------------------------------------------------------------------ autograd
+
+def test_decays_that_want_a_gradient_are_refused_in_training_too():
+    """They are constants: a gradient of None would leave a learnable decay as it is without a word."""
+    from lama_b200 import operators as F
+    z = torch.zeros(1, 4, 2, 8)
+    s = torch.zeros(1, 2, 8, 8)
+    ld = torch.zeros(2, requires_grad=True)
+    for kw in (dict(q=1), dict(k=1), dict(v=1), dict(initial_state=1), dict(q=1, k=1, v=1)):
+        t = {n: (s if n == "initial_state" else z).clone().requires_grad_() for n in kw}
+        refused(lambda: F.linear_attention(t.get("q", z), t.get("k", z), t.get("v", z), ld,
+                                           initial_state=t.get("initial_state")), "log_decay has no gradient")
