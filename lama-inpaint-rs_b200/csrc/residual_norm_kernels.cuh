@@ -84,20 +84,28 @@ __device__ __forceinline__ Span rows_of(const P& p) {
 }
 
 // The rows of a team in flight: row k of the team in stage k % STAGES.
+//
+// A stage is filled again only once the loads that read it have been performed,
+// which each warp reports on a second barrier of the stage.  A named barrier or
+// __syncwarp is not enough: it orders the warps' own accesses, which go through one
+// pipe, but a load can still be queued there when a bulk copy, which does not go through it,
+// lands (with those, rows of 5453 x 2048 fp32 were seen with wrong values).
+constexpr int BARS = 2 * STAGES;  // of a team
 template <int W>
 struct Ring {
   uint32_t bars, base, bytes;  // the team's barriers and stages in shared memory, bytes of a stage
-  int team;
   bool leader;     // this thread's warp issues the team's copies
   int issued = 0;  // leader: rows
   __device__ __forceinline__ void init(uint64_t* b, uint32_t data, uint32_t n, int t, bool lead, int arrivals) {
-    bars = smem_u32(b + t * STAGES);
+    bars = smem_u32(b + t * BARS);
     base = data + (uint32_t)t * STAGES * n;
     bytes = n;
-    team = t;
     leader = lead;
     if (leader && (threadIdx.x & 31) == 0) {
-      for (int i = 0; i < STAGES; i++) mbar_init(bars + 8 * i, arrivals);
+      for (int i = 0; i < STAGES; i++) {
+        mbar_init(bars + 8 * i, arrivals);
+        mbar_init(bars + 8 * (STAGES + i), W);
+      }
       fence_mbar_init();
     }
     __syncwarp();
@@ -110,12 +118,20 @@ struct Ring {
     mbar_wait(bar(k), (uint32_t)(k / STAGES) & 1, failed, 31);
     __syncwarp();
   }
-  // every warp of the team has read the stage it held
-  __device__ __forceinline__ void team_sync() const {
-    if (W == 1)
-      __syncwarp();
-    else
-      named_sync(1 + team, W * 32);
+  // this warp has read row k
+  __device__ __forceinline__ void release(int k) const {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar(k) + 8 * STAGES);
+  }
+  // leader: every warp of the team has
+  __device__ __forceinline__ void wait_read(int k, int* failed) const {
+    mbar_wait(bar(k) + 8 * STAGES, (uint32_t)(k / STAGES) & 1, failed, 32);
+    __syncwarp();
+  }
+  // leader, at the end: where a wait ran out, the copies in flight land before the CTA leaves
+  __device__ __forceinline__ void drain() const {
+    for (int k = issued > STAGES ? issued - STAGES : 0; k < issued; k++)
+      mbar_wait_drain(bar(k), (uint32_t)(k / STAGES) & 1);
   }
 };
 __device__ __forceinline__ void copy4(uint32_t dst, const float* src) {
@@ -163,7 +179,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
   const Span span = rows_of(p);
   constexpr bool token_gate = TOKEN;
   constexpr bool VEC = MODE != SCALAR;
-  __shared__ uint64_t bars[MODE == RING ? TEAMS * STAGES : 1];
+  __shared__ uint64_t bars[MODE == RING ? TEAMS * BARS : 1];
   __shared__ int failed;
   if (threadIdx.x == 0) failed = 0;
   Raw8<T> rx[NI], ry_[NI], rg[NI];
@@ -233,10 +249,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
       rx[i].to(x[i]);
       ry_[i].to(y[i]);
     }
-    if (MODE == RING) {
-      ring.team_sync();
-      if (ring.leader && row + STAGES * TEAMS < span.r1) issue(row + STAGES * TEAMS);
-    }
+    if (MODE == RING) ring.release(k);
     float ry = 1.f;
     if (p.w_post) {
       float q0 = 0.f, q1 = 0.f;
@@ -245,6 +258,10 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
 #pragma unroll
         for (int j = 0; j < 8; j += 2) fma2(q0, q1, y[i][j], y[i][j + 1], y[i][j], y[i][j + 1]);
       ry = rsqrtf(row_sum<W>(q0 + q1, slots[team], turn, team, warp) * inv_c + p.eps);
+    }
+    if (MODE == RING && ring.leader && row + STAGES * TEAMS < span.r1) {
+      ring.wait_read(k, &failed);
+      issue(row + STAGES * TEAMS);
     }
     if (SAVE8) codes(ry_, y, cy, sy);
     Raw8<T> u[NI];
@@ -294,7 +311,10 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 5 : 1) k_norm(const 
     }
     if (p.ry && p.w_post && warp == 0 && lane == 0) p.ry[row] = ry;
   }
-  if (MODE == RING && ring.leader && lane == 0 && failed) atomicCAS(p.status, 0, failed);
+  if (MODE == RING && ring.leader && failed) {
+    ring.drain();
+    if (lane == 0) atomicCAS(p.status, 0, failed);
+  }
 }
 
 // y or u of the backward pass, as such or as codes with their scale
@@ -334,7 +354,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
 #pragma unroll
     for (int j = 0; j < 8; j++) sa[i][j] = sb[i][j] = 0.f;
   constexpr bool VEC = MODE != SCALAR;
-  __shared__ uint64_t bars[MODE == RING ? TEAMS * STAGES : 1];
+  __shared__ uint64_t bars[MODE == RING ? TEAMS * BARS : 1];
   __shared__ int failed;
   if (threadIdx.x == 0) failed = 0;
   Raw8<T> rd[NI], rn[NI], rg[NI];
@@ -483,6 +503,7 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
         from_ring(sy[i], at, at + o_end + 8, LAMA_CH(i));
         if (token_gate) rg[i] = shared_raw<T>(at + o_g + LAMA_CH(i) * sizeof(T), p.c - LAMA_CH(i));
       }
+      ring.release(k);
     }
 #pragma unroll
     for (int i = 0; i < NI; i++) {
@@ -514,9 +535,9 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
     }
     const float r = ry;
     if (MODE != RING && row + TEAMS < span.r1) fetch(row + TEAMS);  // in flight during the last sum and the stores
-    if (MODE == RING) {
-      ring.team_sync();
-      if (ring.leader && row + STAGES * TEAMS < span.r1) issue(row + STAGES * TEAMS);
+    if (MODE == RING && ring.leader && row + STAGES * TEAMS < span.r1) {
+      ring.wait_read(k, &failed);
+      issue(row + STAGES * TEAMS);
     }
     if (p.w_post) {
       const float q = -r * (row_sum<W>(q0 + q1, slots[team], turn, team, warp) * inv_c);
@@ -531,7 +552,10 @@ __global__ void __launch_bounds__(team_threads<W>, W <= 4 ? 4 : 1) k_norm_grad(c
 #pragma unroll
     for (int i = 0; i < NI; i++) store8(dy + i * W * 256, left - i * W * 256, VEC, d[i]);
   }
-  if (MODE == RING && ring.leader && lane == 0 && failed) atomicCAS(p.status, 0, failed);
+  if (MODE == RING && ring.leader && failed) {
+    ring.drain();
+    if (lane == 0) atomicCAS(p.status, 0, failed);
+  }
   // this CTA's column sums: part[cta][0] = sum D yh (times the gate where each token has one), [1] = sum dn uh
   float* dst = p.part + (long long)blockIdx.x * 2 * p.c;
 #pragma unroll
