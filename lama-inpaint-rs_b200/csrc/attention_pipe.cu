@@ -35,9 +35,10 @@
 // with one part, 285 with two).
 //
 // fp16 has 3 more bits and a narrow range, so what the kernel rounds to it is
-// scaled by powers of two first: the rows of P by the row's largest score, the
-// columns of E by the column's largest entry, b~ by 2^8 where that fits; two
-// parts of b~ (22 bits) make the states.
+// scaled by powers of two first: the rows of P by the row's largest decayed
+// score, the columns of E by the column's largest entry, b~ by the chunk's
+// largest: a factor is kept to 2^-38 of the largest it is summed with, however
+// strong the decay.  Two parts of b~ (22 bits) make the states.
 //
 // TMEM: two chunks' S (128 columns, P over them) and O (64), and U.
 #include <type_traits>
@@ -180,6 +181,7 @@ __global__ void __launch_bounds__(Lay<T, NS, OUT>::THREADS, 1) k_pipe(const __gr
   __shared__ __align__(16) uint16_t ef[HALF && OUT ? 4 : 1][64];
   __shared__ uint8_t ex[HALF && OUT ? 128 : 1];
   __shared__ float bs[HALF ? 4 : 1];
+  __shared__ uint32_t tops[HALF ? 2 : 1][2][8];  // the largest b~ of each warp of a team, two chunks in turn
   __shared__ __align__(16) float rv[32];  // lam^{31-j}
   __shared__ Bars bars;
   __shared__ uint32_t tmem_slot;
@@ -275,20 +277,26 @@ __global__ void __launch_bounds__(Lay<T, NS, OUT>::THREADS, 1) k_pipe(const __gr
     // a batch's loads go out before its first use: loads and stores of shared memory stay in program order
     constexpr int ALL = NS * ROWS * 8 / TH, MOST = UP == 1 ? 8 : 4, BATCH = ALL < MOST ? ALL : MOST;
     if (HALF && (OUT || h == 0)) {
-      // b~ = b lam^m may leave fp16's normal numbers at the lower end: where no |b| of the chunk reaches 2^8, it is made
-      // 2^8 times as large
-      uint32_t top = 0;
-#pragma unroll 8
+      // b~ = b lam^m in fp16's range: the chunk's largest |b~| to 2^14..2^15 (not more than 2^100 times as large)
+      uint32_t top = 0;  // as bits: an infinity or NaN is above every number
+#pragma unroll 4
       for (int i = 0; i < NS * CH * 8 / TH; i++) {
-        const int k = i * (TH / 8) + (t >> 3);
-        uint4 x = lds16(src + (k >> 7) * TILE + swz(k & (CH - 1), ck));
-        if ((k & (CH - 1)) >= n) x = make_uint4(0, 0, 0, 0);
-        top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
-                                     __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+        const int k = i * (TH / 8) + (t >> 3), j = k & (CH - 1);
+        const uint4 x = lds16(src + (k >> 7) * TILE + swz(j, ck));
+        const uint32_t m = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                                    __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+        const float most = __half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16)));
+        if (j < n) top = max(top, __float_as_uint(most * pw[REV ? j : n - 1 - j]) & 0x7fffffffu);
       }
-      const uint32_t most = max(top & 0xffffu, top >> 16);
-      up = named_sync_and(3 + 2 * (TH == 64), TH, most < 0x5c00u) ? 256.f : 1.f;  // 0x5c00: 2^8
-      if (t == 0 && h == 0) bs[c & 3] = 1.f / up;
+      top = __reduce_max_sync(~0u, top);
+      uint32_t* all = tops[TH == 64][c & 1];
+      if (lane == 0) all[t >> 5] = top;
+      named_sync(3 + 2 * (TH == 64), TH);
+#pragma unroll
+      for (int i = 0; i < TH / 32; i++) top = max(top, all[i]);
+      const int e = (int)(top >> 23), shift = e == 255 ? -1 : min(max(141 - e, -1), 100);  // 2^(14 - (e - 127))
+      up = __uint_as_float((uint32_t)(127 + shift) << 23);
+      if (t == 0 && h == 0) bs[c & 3] = __uint_as_float((uint32_t)(127 - shift) << 23);
     }
 #pragma unroll 1
     for (int i0 = 0; i0 < ALL; i0 += BATCH) {
@@ -588,75 +596,73 @@ __global__ void __launch_bounds__(Lay<T, NS, OUT>::THREADS, 1) k_pipe(const __gr
       tc_fence_after();
       const int n = num(c);
       float rowf = intra, back = 1.f;  // factors of the row's scores, and of its results
-      if (HALF) {
-        // P in fp16's range: the row's largest score (masked ones included, an
-        // upper bound does: fp16 keeps its precision over 2^28) to at most 2^14
-        float m = 0.f;
+      float m = 0.f;                   // fp16: the row's largest score, decayed
+#pragma unroll 1
+      for (int pass = HALF; pass >= 0; pass--) {  // fp16: once for the largest, once for P
+        if (HALF && pass == 0) {
+          // P in fp16's range: its largest to 2^13..2^14 (fp16 keeps its precision over 2^28 below).  The limits: scores
+          // below 2^-60 are nothing in fp16 results, and what is carried in the same sum stays within fp32.
+          const int shift = min(max((int)(__float_as_uint(m) >> 23) - 140, -60), 100);
+          rowf *= __uint_as_float((uint32_t)(127 - shift) << 23);
+          back = __uint_as_float((uint32_t)(127 + shift) << 23);
+        }
 #pragma unroll 1
         for (int h = 0; h < 2; h++) {
-          if (!(REV ? 2 * h + 1 >= rb : 2 * h <= rb)) continue;
           float v[64];
-          tmem_ld32(t + h * 64, v);
-          tmem_ld32(t + h * 64 + 32, v + 32);
-          tmem_wait_ld();
+          const bool some = REV ? 2 * h + 1 >= rb : 2 * h <= rb;
+          if (some) {
+            tmem_ld32(t + h * 64, v);
+            tmem_ld32(t + h * 64 + 32, v + 32);
+            tmem_wait_ld();
+          }
 #pragma unroll
-          for (int i = 0; i < 64; i++) m = fmaxf(m, fabsf(v[i]));
-        }
-        const int e = (int)(__float_as_uint(m * fabsf(intra)) >> 23);
-        const int shift = min(max(e - 127 - 13, -24), 40);
-        rowf *= __uint_as_float((uint32_t)(127 - shift) << 23);
-        back = __uint_as_float((uint32_t)(127 + shift) << 23);
-      }
-#pragma unroll 1
-      for (int h = 0; h < 2; h++) {
-        float v[64];
-        const bool some = REV ? 2 * h + 1 >= rb : 2 * h <= rb;
-        if (some) {
-          tmem_ld32(t + h * 64, v);
-          tmem_ld32(t + h * 64 + 32, v + 32);
-          tmem_wait_ld();
-        }
+          for (int k = 0; k < 2; k++) {
+            const int b = 2 * h + k;
+            float* x = v + k * 32;
+            uint32_t w[16];
+            if (REV ? b < rb : b > rb) {
+              if (HALF && pass) continue;
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-          const int b = 2 * h + k;
-          float* x = v + k * 32;
-          uint32_t w[16];
-          if (REV ? b < rb : b > rb) {
+              for (int i = 0; i < 16; i++) w[i] = 0;
+              tmem_st16(t + h * 64 + k * 16, w);
+              if (fine) tmem_st16(t + h * 64 + 32 + k * 16, w);
+              continue;
+            }
+            if (b == rb) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) w[i] = 0;
+              for (int j = 0; j < 32; j++) {
+                const int d = REV ? j - lane : lane - j;
+                x[j] = d >= 0 ? x[j] * (rowf * pw[max(d, 0)]) : 0.f;
+              }
+            } else {
+              const float base = rowf * pw[REV ? b * 32 - row : row - b * 32 - 31];
+              const float4* f = reinterpret_cast<const float4*>(REV ? pw : rv);
+#pragma unroll
+              for (int j = 0; j < 8; j++) {
+                float4 y = f[j];
+                mul2(y.x, y.y, base, base);
+                mul2(y.z, y.w, base, base);
+                mul2(x[4 * j], x[4 * j + 1], y.x, y.y);
+                mul2(x[4 * j + 2], x[4 * j + 3], y.z, y.w);
+              }
+            }
+            if (HALF && pass) {
+#pragma unroll
+              for (int i = 0; i < 32; i++) m = fmaxf(m, fabsf(x[i]));
+              continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+            // over this half's columns, which have been read: 32 of the first parts, 32 of the second
             tmem_st16(t + h * 64 + k * 16, w);
-            if (fine) tmem_st16(t + h * 64 + 32 + k * 16, w);
-            continue;
-          }
-          if (b == rb) {
+            if (fine) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-              const int d = REV ? j - lane : lane - j;
-              x[j] = d >= 0 ? x[j] * (rowf * pw[max(d, 0)]) : 0.f;
+              for (int i = 0; i < 16; i++) {
+                const float2 f = unpack2<T>(w[i]);
+                w[i] = pack2<T>(x[2 * i] - f.x, x[2 * i + 1] - f.y);
+              }
+              tmem_st16(t + h * 64 + 32 + k * 16, w);
             }
-          } else {
-            const float base = rowf * pw[REV ? b * 32 - row : row - b * 32 - 31];
-            const float4* f = reinterpret_cast<const float4*>(REV ? pw : rv);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-              float4 y = f[j];
-              mul2(y.x, y.y, base, base);
-              mul2(y.z, y.w, base, base);
-              mul2(x[4 * j], x[4 * j + 1], y.x, y.y);
-              mul2(x[4 * j + 2], x[4 * j + 3], y.z, y.w);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 16; i++) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-          // over this half's columns, which have been read: 32 of the first parts, 32 of the second
-          tmem_st16(t + h * 64 + k * 16, w);
-          if (fine) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const float2 f = unpack2<T>(w[i]);
-              w[i] = pack2<T>(x[2 * i] - f.x, x[2 * i + 1] - f.y);
-            }
-            tmem_st16(t + h * 64 + 32 + k * 16, w);
           }
         }
       }

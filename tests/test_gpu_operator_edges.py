@@ -1,16 +1,88 @@
-"""The token-mixer operators where their inner workings could give way: rows that land while others are read.
+"""The token-mixer operators where their inner number formats could give way: weight that lies far back
+in a fast-decaying sequence, long sequences, many gate rows; and what a caller's autograd sees of them.
 
-The bounds are those of test_gpu_operators.py.  2^-25 is half of fp16's smallest number.
+The bounds are those of test_gpu_operators.py.  For fp16 they hold at the lower end too, up to what the scales
+in front of the roundings lose: a score is kept to 2^-38 of its row's largest (decayed, unmasked) one and a decayed
+operand to 2^-39 of its chunk's largest, both far below the fp32 sums' share of the bound where the other
+factor's sizes do not spread as far.  Where that factor is zero for the largest ones (few tokens with a gradient under dense
+queries) the loss itself is the bound.  2^-25 is half of fp16's smallest number.
 """
 
 import pytest
 import torch
 
-from test_gpu_operators import F, UNIT, close, norm64, norm_inputs  # noqa: F401
+from test_gpu_operators import (F, UNIT, attention64, bound, close, decays, gen, norm64, norm_inputs, randn,  # noqa: F401
+                                state_bound)
 
 pytestmark = pytest.mark.gpu
 
 HALF_FLOOR = 2.0 ** -25
+
+
+def sparse(x, tokens):
+    """x with nothing but the given tokens of each run of 128 left."""
+    keep = torch.zeros(x.shape[1], dtype=torch.bool, device="cuda")
+    for t in tokens:
+        keep[t::128] = True
+    return x * keep[None, :, None, None]
+
+
+FAR = [(250, 64, 64, 2), (700, 64, 128, 2), (2500, 128, 64, 1), (300, 128, 128, 2)]
+
+
+@pytest.mark.parametrize("T,dk,dv,hv", FAR)
+def test_fp16_weight_that_lies_far_back(F, T, dk, dv, hv):  # noqa: F811
+    """Large queries and keys, most keys zero, a decay that halves each token: what a row still sees of a key
+    30 to 60 tokens back is far below the products' size, and well inside fp16 as a result."""
+    g = gen(71)
+    q, k = (randn(g, 2, T, 2, dk) * 200).half(), (randn(g, 2, T, 2, dk) * 200).half()
+    v = (randn(g, 2, T, hv, dv) * 0.1).half()
+    k = sparse(k, (1, 84))
+    ld, scale = torch.tensor([-0.7, -0.05], device="cuda"), 0.125
+    o, s = F.linear_attention(q, k, v, ld, scale=scale, return_state=True)
+    eo, es = attention64(q, k, v, ld, scale)
+    mo, ms = attention64(q, k, v, ld, scale, absolute=True)
+    close(o, eo, bound(torch.float16, T, mo) + HALF_FLOOR, "o")
+    close(s, es, state_bound(T, ms), "state")
+    F.check_operators()
+
+
+@pytest.mark.parametrize("T,dk,dv,hv", FAR)
+def test_fp16_gradients_of_weight_that_lies_far_ahead(F, T, dk, dv, hv):  # noqa: F811
+    """The same for the gradients: few tokens have one, and those far before them still feel it."""
+    g = gen(72)
+    q, k = (randn(g, 2, T, 2, dk) * 0.03).half(), (randn(g, 2, T, 2, dk) * 0.03).half()
+    v = (randn(g, 2, T, hv, dv) * 200).half()
+    go = sparse((randn(g, 2, T, 2, dv) * 200).half(), (50, 126))
+    s0 = randn(g, 2, 2, dk, dv)
+    ld, scale = torch.tensor([-0.7, -0.05], device="cuda"), 0.125
+    got = F.linear_attention_backward(go, q, k, v, ld, scale=scale, initial_state=s0)
+    exp = attention64(q, k, v, ld, scale, s0, None, go)
+    maj = attention64(q, k, v, ld, scale, s0, None, go, absolute=True)
+    for n, a, e, m in zip(("dq", "dk", "dv"), got, exp, maj):
+        close(a, e, bound(torch.float16, T, m, 2) + HALF_FLOOR, n)
+    lost = 2.0 ** -38 * scale * q.double().abs().amax() * go.double().abs().sum(1)[:, :, None]  # of q lam^t, times every gradient
+    close(got[3], exp[3], state_bound(T, maj[3]) + lost, "ds0")
+    F.check_operators()
+
+
+@pytest.mark.parametrize("T", [256, 600])
+def test_fp16_later_tokens_cost_earlier_ones_no_precision(F, T):  # noqa: F811
+    """A token whose keys are at the type's upper end, after tokens whose keys are at its lower end."""
+    g = gen(73)
+    q = (randn(g, 1, T, 1, 64) * 2e4).clamp(-6e4, 6e4).half()
+    k = (randn(g, 1, T, 1, 64) * 2.0 ** -14).half()
+    v = randn(g, 1, T, 1, 64, dtype=torch.float16)
+    ld, scale = torch.tensor([-0.01], device="cuda"), 0.125
+    at = T - 100
+    k[:, at:at + 3] = 6e4
+    v[:, at:at + 3] *= 2.0 ** -14
+    o = F.linear_attention(q, k, v, ld, scale=scale)[:, :at]
+    eo, _ = attention64(q[:, :at], k[:, :at], v[:, :at], ld, scale)
+    mo, _ = attention64(q[:, :at], k[:, :at], v[:, :at], ld, scale, absolute=True)
+    close(o, eo, bound(torch.float16, T, mo) + HALF_FLOOR, "o")
+    k[:, at] = float("inf")
+    assert torch.equal(F.linear_attention(q, k, v, ld, scale=scale)[:, :at], o)
 
 
 RINGS = [
