@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -89,9 +90,13 @@ long long call(F&& f) {
 
 // ------------------------------------------------------------------ arguments
 
+// None of the operators has a forward-mode derivative: a dual tensor would lose its tangent here.
 const Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) refuse("%s is not a tensor", name);
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    refuse("%s has a tangent: the operators have no forward-mode derivative", name);
+  return t;
 }
 
 int type_code(const Tensor& t, const char* name) {

@@ -12,8 +12,9 @@ inference and training:
 
 Tensors are torch tensors on one CUDA device, of type float32, float16 or bfloat16; work is queued on
 torch's current stream of that device.  `linear_attention` and `gated_residual_norm` take part in
-autograd.  Wrong arguments and GPU errors raise `LamaError`; a bounded wait of a kernel that ran out
-is reported by `check_operators`.
+autograd (backward mode, once; tensors with forward-mode tangents are refused).  Wrong arguments and
+GPU errors raise `LamaError`; a bounded wait of a kernel that ran out is reported by
+`check_operators`.
 """
 
 from __future__ import annotations

@@ -119,3 +119,27 @@ def test_rows_keep_their_values_while_the_next_ones_land(F, case):  # noqa: F811
         N = wn.double() * U / torch.sqrt((U * U).mean(-1, keepdim=True) + 1e-6)
         close(n, N, (e + e32) * N.abs() + floor + 1e-30, "n")
     F.check_operators()
+
+
+def test_forward_mode_tangents_of_any_tensor_are_refused(F):  # noqa: F811
+    """The kernels have no forward-mode form; results without the tangent would be derivatives of zero."""
+    from lama_b200 import LamaError
+    ad = torch.autograd.forward_ad
+    z, ld, s = torch.randn(1, 4, 2, 8, device="cuda"), torch.zeros(2, device="cuda"), torch.zeros(1, 2, 8, 8, device="cuda")
+    x, w = torch.randn(3, 8, device="cuda"), torch.ones(8, device="cuda")
+    _, _, saved = F.gated_residual_norm(x, x, post_weight=w, pre_weight=w, save="full")
+    with ad.dual_level():
+        d, dx, dw, ds, dl = (ad.make_dual(t, torch.ones_like(t)) for t in (z, x, w, s, ld))
+        for f in (lambda: F.linear_attention(z, d, z, ld), lambda: F.linear_attention(z, z, d[:, :, :1], ld),
+                  lambda: F.linear_attention(z, z, z, dl), lambda: F.linear_attention(z, z, z, ld, initial_state=ds),
+                  lambda: F.linear_attention_backward(d, z, z, z, ld), lambda: F.linear_attention_step(
+                      z[:, 0], z[:, 0], z[:, 0], ld, ds),
+                  lambda: F.gated_residual_norm(x, dx), lambda: F.gated_residual_norm(x, x, gate=dx),
+                  lambda: F.gated_residual_norm(x, x, pre_weight=dw), lambda: F.gated_residual_norm(x, x, residual_scale=dw),
+                  lambda: F.gated_residual_norm_backward(dx, x, saved)):
+            with pytest.raises(LamaError) as ex:
+                f()
+            assert "forward-mode" in ex.value.msg
+        with pytest.raises(Exception):  # in the autograd function torch itself refuses
+            F.linear_attention(d, z.clone().requires_grad_(), z, ld)
+    F.linear_attention(z, z, z, ld)

@@ -27,3 +27,17 @@ def test_decays_that_want_a_gradient_are_refused_in_training_too():
         t = {n: (s if n == "initial_state" else z).clone().requires_grad_() for n in kw}
         refused(lambda: F.linear_attention(t.get("q", z), t.get("k", z), t.get("v", z), ld,
                                            initial_state=t.get("initial_state")), "log_decay has no gradient")
+
+
+def test_forward_mode_tangents_are_refused():
+    """The kernels have no forward-mode form; results without the tangent would be derivatives of zero."""
+    from lama_b200 import operators as F
+    z, ld = torch.randn(1, 4, 2, 8), torch.zeros(2)
+    with torch.autograd.forward_ad.dual_level():
+        d = torch.autograd.forward_ad.make_dual(z, torch.ones_like(z))
+        refused(lambda: F.linear_attention(d, z, z, ld), "forward-mode")
+        refused(lambda: F.linear_attention(d[:, :, :1], z, z, ld), "forward-mode")  # a view has its base's
+        refused(lambda: F.linear_attention_step(d[:, 0], z[:, 0], z[:, 0], ld, torch.zeros(1, 2, 8, 8)), "forward-mode")
+        refused(lambda: F.gated_residual_norm(d, z, save="int8"), "forward-mode")
+        refused(lambda: F.checkpoint_store(d), "forward-mode")
+    refused(lambda: F.linear_attention(z, z, z, ld), "not on a CUDA device")  # plain tensors reach the next check
