@@ -392,6 +392,8 @@ void empty_checkpoint(const Tensor& x, int dev, Tensor& codes, Tensor& scales) {
 // (x) -> (codes, scales)
 PyObject* py_store(PyObject* const* p) {
   int dev, code;
+  if (THPVariable_Check(p[0]) && THPVariable_Unpack(p[0]).requires_grad() && at::GradMode::is_enabled())
+    refuse("a checkpoint has no gradient: call it under torch.no_grad() or on x.detach()");
   const Tensor& x = first(p[0], "x", dev, code);
   if (x.dim() < 1 || x.size(-1) > 0x7fffffff) refuse("x has no channels, or more than 2^31 - 1");
   Tensor codes, scales;

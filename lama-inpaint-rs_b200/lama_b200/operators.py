@@ -135,7 +135,7 @@ class Checkpoint8:
 
 
 def checkpoint_store(x) -> Checkpoint8:
-    """x [...,C] in 8 bits, a scale for each row and group of 128 channels."""
+    """x [...,C] in 8 bits, a scale for each row and group of 128 channels.  Has no gradient."""
     codes, scales = _native.store(x)
     return Checkpoint8(codes, scales, x.dtype)
 

@@ -41,3 +41,13 @@ def test_forward_mode_tangents_are_refused():
         refused(lambda: F.gated_residual_norm(d, z, save="int8"), "forward-mode")
         refused(lambda: F.checkpoint_store(d), "forward-mode")
     refused(lambda: F.linear_attention(z, z, z, ld), "not on a CUDA device")  # plain tensors reach the next check
+
+
+def test_a_checkpoint_of_a_tensor_that_wants_a_gradient_is_refused():
+    """Codes have no gradient: taken from a graph they would cut it without a word."""
+    from lama_b200 import operators as F
+    x = torch.zeros(2, 8, requires_grad=True)
+    refused(lambda: F.checkpoint_store(x), "has no gradient")
+    with torch.no_grad():
+        refused(lambda: F.checkpoint_store(x), "not on a CUDA device")
+    refused(lambda: F.checkpoint_store(x.detach()), "not on a CUDA device")
