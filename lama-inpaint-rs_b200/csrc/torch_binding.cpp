@@ -353,6 +353,8 @@ PyObject* py_attention_step(PyObject* const* p) {
     return L.attention_step(&x.a, &r, ptr<float>(state), ptr<float>(out), (int)state.size(0), ptr<int>(slots), x.dev, st,
                             err, len);
   });
+  // written behind autograd's back: a graph that saved the tensor has to see that it changed
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
   return wrap(o);
 }
 

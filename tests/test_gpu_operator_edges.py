@@ -143,3 +143,25 @@ def test_forward_mode_tangents_of_any_tensor_are_refused(F):  # noqa: F811
         with pytest.raises(Exception):  # in the autograd function torch itself refuses
             F.linear_attention(d, z.clone().requires_grad_(), z, ld)
     F.linear_attention(z, z, z, ld)
+
+
+def test_a_step_is_seen_by_autograd(F):  # noqa: F811
+    """A state that a graph saved and that a step then overwrote is an error in the backward pass, not a wrong gradient."""
+    g = gen(74)
+    q, k, v = (randn(g, 1, 5, 2, 16) for _ in range(3))
+    ld, s = decays(2), randn(g, 1, 2, 16, 16)
+    for out in (False, True):
+        state = s.clone()
+        o = F.linear_attention(q.clone().requires_grad_(), k, v, ld, initial_state=state)
+        before = state._version
+        with torch.no_grad():
+            if out:
+                F.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s, out_state=state)
+            else:
+                F.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state)
+        assert state._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            o.sum().backward()
+    with torch.inference_mode():  # such tensors have no versions
+        state = s.clone()
+        F.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state)
