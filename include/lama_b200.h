@@ -292,7 +292,8 @@ int lama_rfft2_noalloc(int device, const float* d_feat, int batch, int channels,
  * `device` in, work queued on `stream` (a cudaStream_t, null = legacy default
  * stream), the caller's current device restored, nothing allocated and
  * nothing kept after the call (a workspace, where one is needed, is the
- * caller's).  On failure nothing is queued after the failing step, the code
+ * caller's, on a 16-byte boundary; every other pointer is aligned to its
+ * elements, codes to nothing).  On failure nothing is queued after the failing step, the code
  * is returned and a message is written to err (err_len bytes, may be null).
  * Sums, states and statistics are fp32. */
 

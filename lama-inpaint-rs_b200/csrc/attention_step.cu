@@ -132,6 +132,8 @@ extern "C" int lama_linear_attention_step(const lama_attention* a, const lama_ro
   if (err && err_len > 0) err[0] = 0;
   if (!a || !out || !state || !out_state || !a->log_decay) return fail(err, err_len, LAMA_EINVAL, "null argument");
   if (!dtype_ok(a->dtype)) return fail(err, err_len, LAMA_EINVAL, "unknown element type %d", a->dtype);
+  if (misaligned(4, a->log_decay, state, out_state, slots))
+    return fail(err, err_len, LAMA_EINVAL, "log_decay, a state or slots is not aligned to its elements");
   if (a->batch < 1 || a->heads < 1 || a->dk < 1 || a->dv < 1 || num_slots < 1)
     return fail(err, err_len, LAMA_EINVAL, "batch, heads, dk, dv and num_slots must be positive");
   if (a->tokens != 1) return fail(err, err_len, LAMA_EINVAL, "a step takes one token, not %d", a->tokens);

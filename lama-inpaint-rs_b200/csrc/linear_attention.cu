@@ -777,6 +777,14 @@ const char* check_rows(const lama_rows& x, const lama_attention* p, const char* 
   return nullptr;
 }
 
+int check_workspace(const void* workspace, long long bytes, long long need, char* err, int err_len) {
+  if (bytes < need || (need && !workspace))
+    return fail(err, err_len, LAMA_EINVAL, "workspace of %lld bytes, %lld needed", bytes, need);
+  if (need && misaligned(WORKSPACE_ALIGN, workspace))
+    return fail(err, err_len, LAMA_EINVAL, "the workspace is not aligned to %d bytes", WORKSPACE_ALIGN);
+  return LAMA_OK;
+}
+
 int check(const lama_attention* p, char* err, int err_len) {
   if (!p) return fail(err, err_len, LAMA_EINVAL, "null arguments");
   if (!dtype_ok(p->dtype)) return fail(err, err_len, LAMA_EINVAL, "unknown element type %d", p->dtype);
@@ -787,6 +795,8 @@ int check(const lama_attention* p, char* err, int err_len) {
   if (p->tokens > (1 << 30) || (long long)p->batch * p->heads > 65535)
     return fail(err, err_len, LAMA_EUNSUPPORTED, "tokens exceed 2^30 or batch * heads exceeds 65535");
   if (!p->log_decay) return fail(err, err_len, LAMA_EINVAL, "log_decay is null");
+  if (misaligned(4, p->log_decay, p->initial_state, p->lengths))
+    return fail(err, err_len, LAMA_EINVAL, "log_decay, initial_state or lengths is not aligned to its elements");
   char buf[160];
   const char* m = check_rows(p->q, p, "q", buf, sizeof(buf));
   if (!m) m = check_rows(p->k, p, "k", buf, sizeof(buf));
@@ -891,8 +901,8 @@ extern "C" int lama_linear_attention(const lama_attention* p, const lama_rows* o
   char buf[160];
   if (const char* m = check_rows(*out, p, "out", buf, sizeof(buf))) return fail(err, err_len, LAMA_EINVAL, "%s", m);
   if (out->heads != p->heads) return fail(err, err_len, LAMA_EINVAL, "out has %d heads, not %d", out->heads, p->heads);
-  if (workspace_bytes < need || (need && !workspace))
-    return fail(err, err_len, LAMA_EINVAL, "workspace of %lld bytes, %lld needed", workspace_bytes, need);
+  if (misaligned(4, final_state)) return fail(err, err_len, LAMA_EINVAL, "final_state is not aligned to its elements");
+  if (const int rc = check_workspace(workspace, workspace_bytes, need, err, err_len)) return rc;
   DeviceGuard dev(device);
   cudaError_t ce = dev.status;
   const cudaStream_t st = (cudaStream_t)stream;
@@ -929,8 +939,9 @@ extern "C" int lama_linear_attention_backward(const lama_attention* p, const lam
     if (rows[i]->heads != heads[i])
       return fail(err, err_len, LAMA_EINVAL, "%s has %d heads, not %d", names[i], rows[i]->heads, heads[i]);
   }
-  if (workspace_bytes < need || (need && !workspace))
-    return fail(err, err_len, LAMA_EINVAL, "workspace of %lld bytes, %lld needed", workspace_bytes, need);
+  if (misaligned(4, g->grad_final_state, g->grad_initial_state))
+    return fail(err, err_len, LAMA_EINVAL, "a state's gradient is not aligned to its elements");
+  if (const int rc = check_workspace(workspace, workspace_bytes, need, err, err_len)) return rc;
   DeviceGuard dev(device);
   cudaError_t ce = dev.status;
   int* status = nullptr;

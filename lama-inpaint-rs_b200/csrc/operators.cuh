@@ -91,6 +91,13 @@ cudaError_t launch_chained(void (*kernel)(KArgs...), dim3 grid, unsigned threads
   return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 
+// Whether any of the pointers is off a multiple of `bytes` (a null pointer is not).
+template <class... P>
+bool misaligned(int bytes, P... p) {
+  return (((uintptr_t)p | ...) & (uintptr_t)(bytes - 1)) != 0;
+}
+constexpr int WORKSPACE_ALIGN = 16;  // the kernels' widest access
+
 inline int dtype_size(int t) { return t == LAMA_F32 ? 4 : 2; }
 inline bool dtype_ok(int t) { return t == LAMA_F32 || t == LAMA_F16 || t == LAMA_BF16; }
 

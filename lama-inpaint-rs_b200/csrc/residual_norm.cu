@@ -38,6 +38,8 @@ int check(const lama_norm* p, char* err, int err_len) {
     return fail(err, err_len, LAMA_EUNSUPPORTED, "%d channels exceed %d", p->channels, MAX_C);
   if (p->rows > 0x7fffffffLL) return fail(err, err_len, LAMA_EUNSUPPORTED, "rows exceed 2^31 - 1");
   if (p->gate && p->gate_rows < 1) return fail(err, err_len, LAMA_EINVAL, "gate_rows must be positive");
+  if (misaligned(dtype_size(p->dtype), p->gate) || misaligned(4, p->post_weight, p->pre_weight, p->residual_scales))
+    return fail(err, err_len, LAMA_EINVAL, "the gate, a weight or residual_scales is not aligned to its elements");
   if (!(p->eps >= 0.f)) return fail(err, err_len, LAMA_EINVAL, "eps must not be negative");
   return LAMA_OK;
 }
@@ -59,6 +61,8 @@ extern "C" int lama_gated_residual_norm(const lama_norm* p, const void* x, long 
   const int rc = check(p, err, err_len);
   if (rc != LAMA_OK) return rc;
   if (!x || !y || !u || (p->pre_weight && !n)) return fail(err, err_len, LAMA_EINVAL, "x, y, u or n is null");
+  if (misaligned(dtype_size(p->dtype), x, y, u, n) || misaligned(4, post_rstd, pre_rstd, y_scales, u_scales))
+    return fail(err, err_len, LAMA_EINVAL, "a tensor, a statistic or a checkpoint's scales are not aligned to their elements");
   if (x_stride < p->channels || y_stride < p->channels)
     return fail(err, err_len, LAMA_EINVAL, "a row stride is below %d channels", p->channels);
   if ((y_codes && !y_scales) || (u_codes && !u_scales) || (u_codes && !y_codes))
@@ -103,6 +107,12 @@ extern "C" int lama_gated_residual_norm_backward(const lama_norm* p, const lama_
   if (!g || !g->grad_x || !g->grad_y) return fail(err, err_len, LAMA_EINVAL, "grad_x or grad_y is null");
   if (!workspace || workspace_bytes < need)
     return fail(err, err_len, LAMA_EINVAL, "workspace of %lld bytes, %lld needed", workspace_bytes, need);
+  if (misaligned(WORKSPACE_ALIGN, workspace))
+    return fail(err, err_len, LAMA_EINVAL, "the workspace is not aligned to %d bytes", WORKSPACE_ALIGN);
+  if (misaligned(dtype_size(p->dtype), g->grad_u, g->grad_n, g->y, g->u, g->grad_x, g->grad_y, g->grad_gate) ||
+      misaligned(4, g->y_scales, g->u_scales, g->post_rstd, g->pre_rstd, g->grad_post_weight, g->grad_pre_weight,
+                 g->grad_residual_scales))
+    return fail(err, err_len, LAMA_EINVAL, "a tensor, a statistic or a vector's gradient is not aligned to its elements");
   const bool codes = g->y_codes != nullptr, pre = p->pre_weight && g->grad_n;
   if (codes ? !g->y_scales : !g->y) return fail(err, err_len, LAMA_EINVAL, "neither y nor its checkpoint is given");
   if (pre && (codes ? !g->u_codes || !g->u_scales : !g->u))

@@ -1,6 +1,8 @@
 """What the token-mixer operators refuse or pass on before any GPU is involved: autograd's demands on the
 Python side, pointers and sizes at the C ABI."""
 
+import struct
+
 import pytest
 import torch
 
@@ -51,3 +53,49 @@ def test_a_checkpoint_of_a_tensor_that_wants_a_gradient_is_refused():
     with torch.no_grad():
         refused(lambda: F.checkpoint_store(x), "not on a CUDA device")
     refused(lambda: F.checkpoint_store(x.detach()), "not on a CUDA device")
+
+
+# ------------------------------------------------------------------ pointers at the C ABI
+
+def test_unaligned_pointers_are_refused():
+    """A kernel that met one would fault: every pointer is aligned to its elements, workspaces to 16 bytes."""
+    from test_operators import attention, call, norm, rows
+    p, odd = 4096, 4097
+
+    def check(name, *args, msg="not aligned"):
+        rc, text = call(name, *args, 0, None)
+        assert rc == EINVAL and msg in text, (name, args, text)
+    for kw in (dict(decay=odd), dict(init=odd), dict(lengths=odd)):
+        check("lama_linear_attention", attention(**kw), rows(), None, p, 1 << 40)
+        check("lama_linear_attention_backward", attention(**kw), rows() * 4 + struct.pack("@2P", 0, 0), p, 1 << 40)
+    a = attention(tokens=4096)
+    check("lama_linear_attention", a, rows(), odd, p, 1 << 40)
+    for w in (4104, odd):
+        check("lama_linear_attention", a, rows(), None, w, 1 << 40, msg="workspace is not aligned to 16")
+        check("lama_linear_attention_backward", a, rows() * 4 + struct.pack("@2P", 0, 0), w, 1 << 40,
+              msg="workspace is not aligned to 16")
+    for gs in ((odd, 0), (0, odd)):
+        check("lama_linear_attention_backward", a, rows() * 4 + struct.pack("@2P", *gs), p, 1 << 40)
+    one = attention(tokens=1)
+    check("lama_linear_attention_step", attention(tokens=1, decay=odd), rows(), p, p, 4, None)
+    for args in ((odd, odd, 4, None), (p, odd, 4, None), (p, p, 4, odd)):
+        check("lama_linear_attention_step", one, rows(), *args)
+
+    none = (None,) * 6
+    for kw in (dict(gate=odd), dict(post=odd), dict(pre=odd), dict(scales=odd)):
+        check("lama_gated_residual_norm", norm(**kw), p, 64, p, 64, p, p, *none)
+    for i in range(4):
+        t = [odd if j == i else p for j in range(4)]
+        check("lama_gated_residual_norm", norm(), t[0], 64, t[1], 64, t[2], t[3], *none)
+    for i in (0, 1, 3, 5):  # post_rstd, pre_rstd and the scales; codes are bytes
+        check("lama_gated_residual_norm", norm(), p, 64, p, 64, p, p, *(odd if j == i else p for j in range(6)))
+    need, _ = call("lama_gated_residual_norm_workspace", norm())
+    fields = ["gu", "gn", "y", "u", "yc", "uc", "ys", "us", "ry", "ru", "gx", "gy", "gg", "gpost", "gpre", "gs"]
+
+    def grads(bad=None):
+        v = [odd if f == bad else p for f in fields]
+        return struct.pack("@4P4q12P", *v[:4], *(64,) * 4, *v[4:])
+    for f in fields:
+        if f not in ("yc", "uc"):
+            check("lama_gated_residual_norm_backward", norm(), grads(f), p, need)
+    check("lama_gated_residual_norm_backward", norm(), grads(), 4104, need, msg="workspace is not aligned to 16")
