@@ -143,6 +143,9 @@ extern "C" int lama_linear_attention_step(const lama_attention* a, const lama_ro
     return fail(err, err_len, LAMA_EINVAL, "a step takes no initial_state and no lengths");
   if (!slots && num_slots < a->batch)
     return fail(err, err_len, LAMA_EINVAL, "%d slots for %d rows", num_slots, a->batch);
+  const uintptr_t from = (uintptr_t)state, to = (uintptr_t)out_state;
+  if (from != to && (from < to ? to - from : from - to) < (uintptr_t)num_slots * a->heads * a->dk * a->dv * 4)
+    return fail(err, err_len, LAMA_EINVAL, "out_state overlaps state");
   const lama_rows* rows[4] = {&a->q, &a->k, &a->v, out};
   const char* names[4] = {"q", "k", "v", "out"};
   for (int i = 0; i < 4; i++) {

@@ -99,3 +99,12 @@ def test_unaligned_pointers_are_refused():
         if f not in ("yc", "uc"):
             check("lama_gated_residual_norm_backward", norm(), grads(f), p, need)
     check("lama_gated_residual_norm_backward", norm(), grads(), 4104, need, msg="workspace is not aligned to 16")
+
+
+def test_a_step_refuses_states_that_overlap_in_part():
+    """New states over old ones that other threads have yet to read: only the same buffer, or one apart, will do."""
+    from test_operators import attention, call, rows
+    p, size = 1 << 20, 4 * 2 * 64 * 64 * 4
+    for out in (p + 4, p - 4, p + size - 4, p - size + 4):
+        rc, text = call("lama_linear_attention_step", attention(tokens=1), rows(), p, out, 4, None, 0, None)
+        assert rc == EINVAL and "overlaps" in text, out
