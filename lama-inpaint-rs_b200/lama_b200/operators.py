@@ -53,7 +53,10 @@ def _learns(*ts):
 
 def check_operators(device=None) -> None:
     """Wait for the device and raise `LamaError` if a kernel's bounded wait ran out since the last call."""
-    dev = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    dev = torch.device("cuda" if device is None else device)
+    if dev.type != "cuda":
+        _refuse(f"{dev} is not a CUDA device")
+    dev = torch.cuda.current_device() if dev.index is None else dev.index
     err = ctypes.create_string_buffer(256)
     rc = lib().lama_operator_status(dev, err, 256)
     if rc < 0:

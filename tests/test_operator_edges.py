@@ -108,3 +108,22 @@ def test_a_step_refuses_states_that_overlap_in_part():
     for out in (p + 4, p - 4, p + size - 4, p - size + 4):
         rc, text = call("lama_linear_attention_step", attention(tokens=1), rows(), p, out, 4, None, 0, None)
         assert rc == EINVAL and "overlaps" in text, out
+
+
+# ------------------------------------------------------------------ the device of a report
+
+def test_check_operators_reads_the_current_device(monkeypatch):
+    """A device without an index is the current one, as everywhere in torch."""
+    from lama_b200 import operators as F
+    asked = []
+
+    class Lib:
+        def lama_operator_status(self, dev, err, n):
+            asked.append(dev)
+            return 0
+    monkeypatch.setattr(F, "lib", Lib)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    for d in (None, "cuda", torch.device("cuda"), "cuda:1", 2, torch.device("cuda", 0)):
+        F.check_operators(d)
+    assert asked == [3, 3, 3, 1, 2, 0]
+    refused(lambda: F.check_operators("cpu"), "not a CUDA device")
