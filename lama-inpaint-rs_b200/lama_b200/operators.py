@@ -67,22 +67,23 @@ def check_operators(device=None) -> None:
 
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, log_decay, scale, initial_state, lengths):
+    def forward(ctx, q, k, v, log_decay, scale, initial_state, lengths, return_state):
         ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        return _native.attention(q, k, v, log_decay, scale, initial_state, lengths, True)
+        o, state = _native.attention(q, k, v, log_decay, scale, initial_state, lengths, return_state)
+        return (o, state) if return_state else o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_o, grad_state):
+    def backward(ctx, grad_o, grad_state=None):
         q, k, v, log_decay, initial_state, lengths = ctx.saved_tensors
         if grad_o is None:
             grad_o = q.new_zeros(*q.shape[:2], log_decay.numel(), v.shape[-1])
         dq, dk, dv, ds = linear_attention_backward(grad_o, q, k, v, log_decay, scale=ctx.scale,
                                                    initial_state=initial_state, lengths=lengths,
                                                    grad_state=grad_state)
-        return dq, dk, dv, None, None, ds, None
+        return dq, dk, dv, None, None, ds, None, None
 
 
 def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengths=None, return_state=False):
@@ -99,9 +100,8 @@ def linear_attention(q, k, v, log_decay, *, scale=None, initial_state=None, leng
     if _grad_enabled() and _learns(q, k, v, initial_state):
         if _learns(log_decay):  # inside the function gradients are off, and the binding's own check with them
             _refuse("log_decay has no gradient: the decays are constants of the layer")
-        o, state = _LinearAttention.apply(q, k, v, log_decay, scale, initial_state, lengths)
-    else:
-        o, state = _native.attention(q, k, v, log_decay, scale, initial_state, lengths, bool(return_state))
+        return _LinearAttention.apply(q, k, v, log_decay, scale, initial_state, lengths, bool(return_state))
+    o, state = _native.attention(q, k, v, log_decay, scale, initial_state, lengths, bool(return_state))
     return (o, state) if return_state else o
 
 

@@ -165,3 +165,17 @@ def test_a_step_is_seen_by_autograd(F):  # noqa: F811
     with torch.inference_mode():  # such tensors have no versions
         state = s.clone()
         F.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_training_is_the_same_with_and_without_the_final_state(F, dtype):  # noqa: F811
+    g = gen(75)
+    q, k, v, go = (randn(g, 2, 1100, 2, 64, dtype=dtype) for _ in range(4))
+    got = []
+    for state in (False, True):
+        ts = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = F.linear_attention(*ts, decays(2), return_state=state)
+        o = out[0] if state else out
+        o.backward(go)
+        got.append([o, *(t.grad for t in ts)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))

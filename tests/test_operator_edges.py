@@ -55,6 +55,33 @@ def test_a_checkpoint_of_a_tensor_that_wants_a_gradient_is_refused():
     refused(lambda: F.checkpoint_store(x.detach()), "not on a CUDA device")
 
 
+def test_training_asks_for_the_final_state_only_where_the_caller_does(monkeypatch):
+    """It costs a pass over keys and values of its own."""
+    from lama_b200 import operators as F
+    asked = []
+
+    class Native:
+        @staticmethod
+        def attention(q, k, v, log_decay, scale, initial_state, lengths, return_state):
+            asked.append(return_state)
+            return q * 2, q.new_zeros(1, 2, 8, 8) if return_state else None
+
+        @staticmethod
+        def attention_backward(grad_o, q, k, v, log_decay, scale, initial_state, lengths, grad_state):
+            asked.append(grad_state)
+            return grad_o * 2, torch.zeros_like(k), torch.zeros_like(v), None
+    monkeypatch.setattr(F, "_native", Native)
+    z, ld = torch.ones(1, 4, 2, 8), torch.zeros(2)
+    q = z.clone().requires_grad_()
+    o = F.linear_attention(q, z, z, ld)
+    o.sum().backward()
+    assert asked == [False, None] and torch.equal(q.grad, 2 * z)
+    q.grad = None
+    o, state = F.linear_attention(q, z, z, ld, return_state=True)
+    (o.sum() + state.sum()).backward()
+    assert asked[2] is True and torch.equal(asked[3], torch.ones_like(state)) and torch.equal(q.grad, 2 * z)
+
+
 # ------------------------------------------------------------------ pointers at the C ABI
 
 def test_unaligned_pointers_are_refused():
