@@ -154,3 +154,28 @@ def test_check_operators_reads_the_current_device(monkeypatch):
         F.check_operators(d)
     assert asked == [3, 3, 3, 1, 2, 0]
     refused(lambda: F.check_operators("cpu"), "not a CUDA device")
+
+
+# ------------------------------------------------------------------ the build
+
+def test_the_library_builds_without_torch(tmp_path):
+    """The library and the CLI need no torch: the default target leaves the binding out where there is none, `binding` says so."""
+    import os
+    import subprocess
+    import sys
+    csrc = os.path.join(os.path.dirname(__file__), "..", "lama-inpaint-rs_b200", "csrc")
+
+    def make(python, *args):
+        return subprocess.run(["make", "-n", "-B", "-C", csrc, f"PYTHON={python}", *args], capture_output=True, text=True)
+    bare = tmp_path / "python"
+    bare.write_text(f'#!/bin/sh\nexec {sys.executable} -I -S "$@"\n')  # no site-packages: no torch
+    bare.chmod(0o755)
+    for python in (bare, tmp_path / "missing"):
+        r = make(python)
+        assert r.returncode == 0 and "liblama_b200.so" in r.stdout and "torch_binding.cpp" not in r.stdout
+        assert "not built" in r.stdout
+    r = subprocess.run(["make", "-C", csrc, f"PYTHON={bare}", "BINDING=" + str(tmp_path / "b.so"), "binding"],
+                       capture_output=True, text=True)
+    assert r.returncode != 0 and "needs torch" in r.stdout
+    r = make(sys.executable)
+    assert r.returncode == 0 and "torch_binding.cpp" in r.stdout
