@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cudaTypedefs.h>
+#include <type_traits>
 
 #include "operators.cuh"
 #include "ptx.cuh"
@@ -78,8 +79,24 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
 }
 __device__ __forceinline__ uint32_t swz(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
 
-// v[0..7] into N bf16 parts of 16 bytes each (part p holds what parts 0..p-1 left over)
-template <int N>
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(a, b);
+  }
+}
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+  if constexpr (std::is_same_v<T, __half>)
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+  else
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));  // bf16: the upper half of an fp32
+}
+// v[0..7] into N parts of type T, 16 bytes each (part p holds what parts 0..p-1 left over)
+template <int N, class T>
 __device__ __forceinline__ void split8(const float* v, uint4* out) {
   float r[8];
 #pragma unroll
@@ -89,11 +106,11 @@ __device__ __forceinline__ void split8(const float* v, uint4* out) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(r[2 * i], r[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      w[i] = pack2<T>(r[2 * i], r[2 * i + 1]);
       if (p + 1 < N) {
-        r[2 * i] -= __low2float(h);
-        r[2 * i + 1] -= __high2float(h);
+        const float2 h = unpack2<T>(w[i]);
+        r[2 * i] -= h.x;
+        r[2 * i + 1] -= h.y;
       }
     }
     out[p] = make_uint4(w[0], w[1], w[2], w[3]);

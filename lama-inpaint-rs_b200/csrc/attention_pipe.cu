@@ -90,49 +90,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int c
 }
 
 template <class T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same_v<T, __half>) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    return pack_bf16x2(a, b);
-  }
-}
-template <class T>
-__device__ __forceinline__ float2 unpack2(uint32_t x) {
-  if constexpr (std::is_same_v<T, __half>)
-    return __half22float2(*reinterpret_cast<const __half2*>(&x));
-  else
-    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));  // bf16: the upper half of an fp32
-}
-template <class T>
 __device__ __forceinline__ void unpack8(uint4 x, float* v) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     const float2 f = unpack2<T>(w[i]);
     v[2 * i] = f.x, v[2 * i + 1] = f.y;
-  }
-}
-// v[0..7] into N parts of type T
-template <int N, class T>
-__device__ __forceinline__ void split8(const float* v, uint4* out) {
-  float r[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) r[i] = v[i];
-#pragma unroll
-  for (int p = 0; p < N; p++) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      w[i] = pack2<T>(r[2 * i], r[2 * i + 1]);
-      if (p + 1 < N) {
-        const float2 h = unpack2<T>(w[i]);
-        r[2 * i] -= h.x;
-        r[2 * i + 1] -= h.y;
-      }
-    }
-    out[p] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 

@@ -82,17 +82,8 @@ __device__ __forceinline__ void decode8(uint2 c, float scale, float* v) {
   }
 }
 
-// 8 elements from p (or n < 8 where the row ends); `vec`: p is 16-byte (fp32:
+// 8 elements to p (or n < 8 where the row ends); `vec`: p is 16-byte (fp32:
 // two 16-byte words) aligned and n is 8.
-template <class T>
-__device__ __forceinline__ void load8(const T* p, int n, bool vec, float* v) {
-  if (vec && n >= 8) {
-    load_vec<T, 8>(p, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = i < n ? to_float(p[i]) : 0.f;
-  }
-}
 template <class T>
 __device__ __forceinline__ void store8(T* p, int n, bool vec, const float* v) {
   if (vec && n >= 8) {

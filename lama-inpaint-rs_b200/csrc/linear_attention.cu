@@ -98,7 +98,7 @@ struct Fetch {
       float v[8];
       uint4 parts[Parts<T>::N];
       r[it].to(v);
-      split8<Parts<T>::N>(v, parts);
+      split8<Parts<T>::N, __nv_bfloat16>(v, parts);
 #pragma unroll
       for (int p = 0; p < Parts<T>::N; p++) sts16(dst + p * TILE + swz(row, ck), parts[p]);
     }
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(ALL, 1) k_chunks(const __grid_constant__ Set s
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             uint4 parts[EP];
-            split8<EP>(e + h * 8, parts);
+            split8<EP, __nv_bfloat16>(e + h * 8, parts);
 #pragma unroll
             for (int p = 0; p < EP; p++) sts16(smem + PL::E + p * ETILE + swz(srow, (scol >> 3) + h), parts[p]);
           }
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(ALL, 1) k_chunks(const __grid_constant__ Set s
 #pragma unroll
           for (int i = 0; i < 8; i++) v[i] = j < n ? v[i] * w : 0.f;
           uint4 parts[3];
-          split8<3>(v, parts);
+          split8<3, __nv_bfloat16>(v, parts);
 #pragma unroll
           for (int p = 0; p < 3; p++) sts16(smem + PL::BD + p * TILE + swz(j, ck), parts[p]);
         }
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(ALL, 1) k_chunks(const __grid_constant__ Set s
 #pragma unroll
             for (int q = 0; q < 4; q++) {
               uint4 parts[NP];
-              split8<NP>(v + q * 8, parts);
+              split8<NP, __nv_bfloat16>(v + q * 8, parts);
 #pragma unroll
               for (int p = 0; p < NP; p++)
                 sts16(smem + PL::P + (p * 2 + (warp >> 2)) * TILE + swz(row, h * 4 + q), parts[p]);

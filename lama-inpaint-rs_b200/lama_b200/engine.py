@@ -91,7 +91,7 @@ SIGNATURES = [
     ("lama_mask_depth", ctypes.c_int, [_u8p, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
     ("lama_section_rects", ctypes.c_int, [_u8p, ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_int),
                                           ctypes.c_int]),
-    # the operators' structures are passed as packed bytes (operators.py)
+    # the operators (their torch binding calls the same addresses by itself); structures as packed bytes
     ("lama_linear_attention_workspace", ctypes.c_longlong, [ctypes.c_char_p, ctypes.c_int,
                                                             ctypes.c_char_p, ctypes.c_int]),
     ("lama_linear_attention", ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p, _vp, _vp,
