@@ -903,7 +903,7 @@ extern "C" int lama_linear_attention(const lama_attention* p, const lama_rows* o
   if (out->heads != p->heads) return fail(err, err_len, LAMA_EINVAL, "out has %d heads, not %d", out->heads, p->heads);
   if (misaligned(4, final_state)) return fail(err, err_len, LAMA_EINVAL, "final_state is not aligned to its elements");
   if (const int rc = check_workspace(workspace, workspace_bytes, need, err, err_len)) return rc;
-  DeviceGuard dev(device);
+  DeviceGuard dev(device, true);
   cudaError_t ce = dev.status;
   const cudaStream_t st = (cudaStream_t)stream;
   Set set;
@@ -942,7 +942,7 @@ extern "C" int lama_linear_attention_backward(const lama_attention* p, const lam
   if (misaligned(4, g->grad_final_state, g->grad_initial_state))
     return fail(err, err_len, LAMA_EINVAL, "a state's gradient is not aligned to its elements");
   if (const int rc = check_workspace(workspace, workspace_bytes, need, err, err_len)) return rc;
-  DeviceGuard dev(device);
+  DeviceGuard dev(device, true);
   cudaError_t ce = dev.status;
   int* status = nullptr;
   if (ce == cudaSuccess) ce = status_word(&status);

@@ -28,12 +28,15 @@ inline int fail(char* err, int err_len, int code, const char* fmt, ...) {
 }
 
 // Makes `device` current for the duration of a call and restores the caller's.
+// `bind`: the calling thread has the device's context afterwards.  A thread that has
+// made no CUDA call yet has none (the device is current all the same, and a launch would bind
+// it), and the driver encodes no tensor map for it.
 class DeviceGuard {
  public:
-  explicit DeviceGuard(int device) {
-    if ((status = cudaGetDevice(&prev_)) == cudaSuccess && prev_ != device) {
+  explicit DeviceGuard(int device, bool bind = false) {
+    if ((status = cudaGetDevice(&prev_)) == cudaSuccess && (bind || prev_ != device)) {
       status = cudaSetDevice(device);
-      moved_ = status == cudaSuccess;
+      moved_ = status == cudaSuccess && prev_ != device;
     }
     if (status != cudaSuccess) cudaGetLastError();  // not sticky: keep it from the caller's next call
   }

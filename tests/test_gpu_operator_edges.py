@@ -179,3 +179,23 @@ def test_training_is_the_same_with_and_without_the_final_state(F, dtype):  # noq
         o.backward(go)
         got.append([o, *(t.grad for t in ts)])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_a_thread_s_first_call(F, dtype):  # noqa: F811
+    """A thread that has made no CUDA call yet (autograd's own, at a process's first backward pass) runs the same kernels."""
+    import threading
+    g = gen(77)
+    q, k, v, go = (randn(g, 2, 1100, 2, 64, dtype=dtype) for _ in range(4))
+    ld = decays(2)
+
+    def work():
+        return [F.linear_attention(q, k, v, ld), *F.linear_attention_backward(go, q, k, v, ld)[:3]]
+    exp = [t.clone() for t in work()]
+    work()  # its memory stays with the allocator: the thread's call needs no other CUDA call
+    for part in (work, lambda: [exp[0], *F.linear_attention_backward(go, q, k, v, ld)[:3]]):
+        got = []
+        t = threading.Thread(target=lambda: got.extend(part()))
+        t.start()
+        t.join()
+        assert len(got) == 4 and all(torch.equal(a, b) for a, b in zip(got, exp))
