@@ -199,3 +199,87 @@ def test_a_thread_s_first_call(F, dtype):  # noqa: F811
         t.start()
         t.join()
         assert len(got) == 4 and all(torch.equal(a, b) for a, b in zip(got, exp))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_training_is_the_same_with_and_without_the_final_state(F, dtype):  # noqa: F811
+    g = gen(75)
+    q, k, v, go = (randn(g, 2, 1100, 2, 64, dtype=dtype) for _ in range(4))
+    got = []
+    for state in (False, True):
+        ts = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = F.linear_attention(*ts, decays(2), return_state=state)
+        o = out[0] if state else out
+        o.backward(go)
+        got.append([o, *(t.grad for t in ts)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+# ------------------------------------------------------------------ the range's upper end
+
+def chunked64(q, k, v, g, scale):
+    """The recurrence in 64 bits, 256 tokens at a time: (o, final state), differentiable."""
+    H = g.numel()
+    q, k, v = (x.repeat_interleave(H // x.shape[2], 2).transpose(1, 2) for x in (q, k, v))
+    gd = g.double()[None, :, None, None]
+    s = q.new_zeros(q.shape[0], H, q.shape[-1], v.shape[-1])
+    out = []
+    for t in range(0, q.shape[2], 256):
+        a, b, c = (x[:, :, t:t + 256] for x in (q, k, v))
+        i = torch.arange(a.shape[2], device="cuda", dtype=torch.float64)
+        d = (i[:, None] - i[None])[None, None]
+        m = torch.where(d >= 0, torch.exp(gd * d.clamp_min(0)), 0.0)
+        w = torch.exp(gd * (i[None, None, :, None] + 1))
+        out.append(scale * (((a @ b.transpose(-1, -2)) * m) @ c + w * (a @ s)))
+        s = torch.exp(gd * a.shape[2]) * s + (b * torch.exp(gd * (a.shape[2] - 1 - i[None, None, :, None]))).transpose(-1, -2) @ c
+    return torch.cat(out, 2).transpose(1, 2), s
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("T,dk,dv", [(65536, 64, 64), (40001, 128, 80)])
+def test_long_sequences(F, dtype, T, dk, dv):  # noqa: F811
+    """A 2048x2048 image's latent, and an odd length; two heads of keys for four."""
+    g = gen(76)
+    q, k, v = randn(g, 1, T, 4, dk, dtype=dtype), randn(g, 1, T, 2, dk, dtype=dtype), randn(g, 1, T, 4, dv, dtype=dtype)
+    go, gs = randn(g, 1, T, 4, dv, dtype=dtype), randn(g, 1, 4, dk, dv)
+    ld, scale = decays(4), dk ** -0.5
+    o, s = F.linear_attention(q, k, v, ld, return_state=True)
+    got = F.linear_attention_backward(go, q, k, v, ld, grad_state=gs)
+    sums = []
+    for f in (lambda x: x.double(), lambda x: x.double().abs()):
+        ts = [f(x).requires_grad_() for x in (q, k, v)]
+        eo, es = chunked64(*ts, ld, scale)
+        sums.append([eo.detach(), es.detach(), *torch.autograd.grad([eo, es], ts, [f(go), f(gs)])])
+    exp, maj = sums
+    floor = HALF_FLOOR if dtype == torch.float16 else 0.0
+    close(o, exp[0], bound(dtype, T, maj[0]) + floor, "o")
+    close(s, exp[1], state_bound(T, maj[1]), "state")
+    for n, a, e, m in zip(("dq", "dk", "dv"), got, exp[2:], maj[2:]):
+        close(a, e, bound(dtype, T, m, 4) + floor, n)
+    F.check_operators()
+
+
+@pytest.mark.parametrize("dtype,shape", [(torch.bfloat16, (5000, 3, 128)), (torch.float32, (1500, 2, 520)),
+                                         (torch.float16, (700, 40, 257))], ids=str)
+def test_a_gate_for_each_of_many_images(F, dtype, shape):  # noqa: F811
+    """More gate rows than the kernels have CTAs: every one with its own sums."""
+    case = (dtype, shape, (shape[0], 1, shape[2]), True, True, True)
+    x, y, wp, wn, gate, s, gu, gn = norm_inputs(case)
+    kw = dict(post_weight=wp, pre_weight=wn, residual_scale=s, save="full")
+    u, n, saved = F.gated_residual_norm(x, y, gate=gate, **kw)
+    g1 = F.gated_residual_norm_backward(gu, gn, saved)
+    # a gate for each token holds the same numbers: the same rows, and its gradient summed over an image's tokens
+    wide = gate.expand(shape).contiguous()
+    u2, n2, saved = F.gated_residual_norm(x, y, gate=wide, **kw)
+    g2 = F.gated_residual_norm_backward(gu, gn, saved)
+    e, e32, rows = UNIT[dtype], 4 * (shape[2] + 32) * UNIT[torch.float32], shape[0] * shape[1]
+    floor = HALF_FLOOR if dtype == torch.float16 else 0.0
+    for a, b in ((u, u2), (n, n2), (g1.x, g2.x), (g1.y, g2.y)):
+        # one order of the same products apart: a last place of the results where they round the other way
+        close(a, b.double(), 2 * e * b.double().abs() + e32 * (b.double().abs() + 1) + floor)
+    dg = g2.gate.double()
+    close(g1.gate[:, 0], dg.sum(1), 2 * e * dg.abs().sum(1) + e32 * (dg.abs().sum(1) + 1) + floor * shape[1], "dgate")
+    U = u.double()
+    uh = U / torch.sqrt((U * U).mean(-1, keepdim=True) + 1e-6)
+    t = gn.double() * uh
+    close(g1.pre_weight, t.sum((0, 1)), (e32 + rows * 2.0 ** -23) * t.abs().sum((0, 1)), "dw_pre")
