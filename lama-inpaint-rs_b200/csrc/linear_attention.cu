@@ -39,9 +39,9 @@
 // (exact), fp32 inputs three (24 bits), and a product keeps the pairs of
 // parts above the last part's size.  What the kernel computes itself and
 // feeds back as an operand is rounded: the decayed b to three parts always
-// (the state is an fp32 result), the scores to as many parts as the inputs
-// have, the entering state to two (three for fp32 inputs).  For bf16 inputs the
-// scores' one rounding is of the size of the output's own.
+// (the state is an fp32 result), the scores and the entering state to two
+// (three for fp32 inputs).  Scores in one part would add an error of the size of a
+// bf16 output's own rounding.
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -161,12 +161,12 @@ __device__ __forceinline__ void mma_parts(uint32_t d, uint64_t a, uint64_t b, ui
 template <class T>
 struct Plan {
   static constexpr int NP = Parts<T>::N;
-  static constexpr int EP = NP == 1 ? 2 : NP;  // parts of the entering state
+  static constexpr int EP = NP == 1 ? 2 : NP;  // parts of the entering state and of the scores
   // a, b, c: NP tiles each; the decayed b: 3 tiles; the entering state.  The
-  // scores' 2 * NP tiles and then the chunk's outputs take the place of a and b.
-  static constexpr uint32_t A = 0, B = NP * TILE, C = 2 * NP * TILE;
+  // scores' 2 * EP tiles and then the chunk's outputs take the place of a and b.
+  static constexpr uint32_t A = 0, B = NP * TILE, C = 2 * EP * TILE;
   static constexpr uint32_t P = A, O = A;
-  static constexpr uint32_t BD = 3 * NP * TILE;
+  static constexpr uint32_t BD = C + NP * TILE;
   static constexpr uint32_t E = BD + 3 * TILE;
   static constexpr uint32_t bytes() { return E + EP * ETILE + 1024; }
   static_assert(bytes() <= 227 * 1024 && CH * 64 * 4 <= C, "shared memory");
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(ALL, 1) k_chunks(const __grid_constant__ Set s
       if (OUT && last_slab) {
         if (!ready(rdy_p, phase_p, 6)) break;
         if (leader) {
-          mma_parts<NP, NP>(t_p, smem_desc(smem + PL::P, 1024, 2), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | B_MN, 2,
+          mma_parts<EP, NP>(t_p, smem_desc(smem + PL::P, 1024, 2), desc_mn(smem + PL::C, 0), idesc_bf16_f32(64) | B_MN, 2,
                             32, TILE, 2 * TILE, 2048, 8192, TILE, false);
           mma_commit(bar_p);
         }
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(ALL, 1) k_chunks(const __grid_constant__ Set s
         hand_over(rdy_u);
         pending_u = true;
         if (OUT && last_slab) {
-          // scores: decay and causal mask, rounded to NP parts
+          // scores: decay and causal mask, rounded to EP parts
           if (!wait(bar_p, phase_p, pending_p, 1)) break;
 #pragma unroll 1
           for (int h = 0; h < 2; h++) {
@@ -428,10 +428,10 @@ __global__ void __launch_bounds__(ALL, 1) k_chunks(const __grid_constant__ Set s
             }
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-              uint4 parts[NP];
-              split8<NP, __nv_bfloat16>(v + q * 8, parts);
+              uint4 parts[EP];
+              split8<EP, __nv_bfloat16>(v + q * 8, parts);
 #pragma unroll
-              for (int p = 0; p < NP; p++)
+              for (int p = 0; p < EP; p++)
                 sts16(smem + PL::P + (p * 2 + (warp >> 2)) * TILE + swz(row, h * 4 + q), parts[p]);
             }
           }

@@ -283,3 +283,18 @@ def test_a_gate_for_each_of_many_images(F, dtype, shape):  # noqa: F811
     uh = U / torch.sqrt((U * U).mean(-1, keepdim=True) + 1e-6)
     t = gn.double() * uh
     close(g1.pre_weight, t.sum((0, 1)), (e32 + rows * 2.0 ** -23) * t.abs().sum((0, 1)), "dw_pre")
+
+
+@pytest.mark.parametrize("T,dk,dv", [(100, 33, 33), (26, 33, 16), (1000, 33, 20), (128, 64, 64), (60, 128, 72)])
+def test_bf16_results_are_rounded_once(F, T, dk, dv):  # noqa: F811
+    """Where the scores and what is carried keep 16 bits or more (heads of any odd size, and a chunk of the others) a result is
+    its sum rounded once: e |result|, and 2^-16 M for the two parts beside the fp32 sums."""
+    g = gen(78)
+    q, k, v, go = (randn(g, 2, T, 2, d, dtype=torch.bfloat16) for d in (dk, dk, dv, dv))
+    ld, scale = decays(2), dk ** -0.5
+    got = F.linear_attention(q, k, v, ld), *F.linear_attention_backward(go, q, k, v, ld)[:3]
+    exp = attention64(q, k, v, ld, scale)[:1] + attention64(q, k, v, ld, scale, None, None, go)[:3]
+    maj = attention64(q, k, v, ld, scale, absolute=True)[:1] + attention64(q, k, v, ld, scale, None, None, go, absolute=True)[:3]
+    e = UNIT[torch.bfloat16]
+    for n, a, x, m in zip(("o", "dq", "dk", "dv"), got, exp, maj):
+        close(a, x, e * x.abs() + 2.0 ** -16 * m + bound(torch.float32, T, m, 2), n)
