@@ -683,7 +683,9 @@ cudaError_t launch_scan(const Set& set, cudaStream_t st) {
 // that run together.  Pipelined (16-bit types): a CTA costs 4 beside its
 // chunks (set-up, the first loads, the last products), the pass that makes the
 // states 0.6 a chunk and, with the scan, two launches of 3 each.  The other
-// kernel's steps are several times longer and do not overlap.
+// kernel's steps are several times longer and do not overlap; 16-bit rows that go
+// through it are cut by the first costs all the same, since a workspace is sized before the output's
+// place is known.
 struct Cut {
   int nseg = 1, chunks = 1;
 };

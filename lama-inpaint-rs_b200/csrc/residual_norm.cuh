@@ -25,9 +25,9 @@
 // row per CTA, which a second kernel adds in a fixed order: results do not
 // change from run to run.
 //
-// Measured: 131072 x 512 bf16 with 8-bit checkpoints, forward 150 us (4.5
-// TB/s), backward 142 us (4.7 TB/s) and 8 us for the vectors; 4096 x 512
-// forward 6.5 us.  Four or five CTAs of four one-row teams a SM; two warps a
+// Measured: 131072 x 512 bf16 with 8-bit checkpoints, forward 157 us (4.3
+// TB/s), backward 147 us (4.6 TB/s) and 10 us for the vectors; 4096 x 512
+// forward 6.8 us.  Four or five CTAs of four one-row teams a SM; two warps a
 // row of 512 channels (half the registers) measured 1.4-1.8 times slower.
 //
 // Checkpoints in 8 bits: the forward pass can store y and u as codes, made
