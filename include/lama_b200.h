@@ -293,9 +293,9 @@ int lama_rfft2_noalloc(int device, const float* d_feat, int batch, int channels,
  * stream), the caller's current device restored, nothing allocated and
  * nothing kept after the call (a workspace, where one is needed, is the
  * caller's, on a 16-byte boundary; every other pointer is aligned to its
- * elements, codes to nothing).  On failure nothing is queued after the failing step, the code
- * is returned and a message is written to err (err_len bytes, may be null).
- * Sums, states and statistics are fp32. */
+ * elements, codes to nothing).  On failure nothing is queued after the failing
+ * step, the code is returned and a message is written to err (err_len bytes,
+ * may be null).  Sums, states and statistics are fp32. */
 
 /* Element types of the operators' tensors. */
 enum { LAMA_F32 = 0, LAMA_F16 = 1, LAMA_BF16 = 2 };
@@ -321,7 +321,9 @@ typedef struct {
  * and gradients are 0.  initial_state: null (zeros) or [batch][heads][dk][dv]
  * fp32.  dk, dv <= 128; batch * heads <= 65535.  Results are the same from run
  * to run, and whether or not the final state is asked for.  An infinity or NaN
- * in a token reaches the outputs of its whole 128-token chunk. */
+ * in a token reaches the outputs of its whole 128-token chunk.  With fp16
+ * inputs a factor below 2^-38 of the largest one that it is summed with (over a
+ * row of scores, or a chunk) is lost. */
 typedef struct {
   int dtype; /* of q, k, v and the output: LAMA_F32, LAMA_F16 or LAMA_BF16 */
   int batch, tokens, heads, dk, dv;
